@@ -491,6 +491,63 @@ int pccnn_point_conv_weight_var(int64_t num_pts, const float* basis, int hidden,
                                 float* out_variance, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------- */
+/* Attention between packed clouds (no counterpart in the reference)          */
+/* ------------------------------------------------------------------------- */
+
+/* Features are float32, or bfloat16 where is_bf16 != 0; every sum, statistic and probability is float32 and a bf16
+ * result is rounded once.  Features of heads are [rows, heads, size] with contiguous sizes and any row and head
+ * stride in elements (int64 host arrays {row, head}); outputs are contiguous. */
+
+/* Layer norm over the channels: out = (feats - mean) * rstd * weights + bias with the biased variance,
+ * rstd = 1 / sqrt(variance + eps).  feats [rows, channels] with row stride ld_feats; weights, bias [channels]
+ * float32; out [rows, channels]; out_mean, out_rstd [rows] float32. */
+int pccnn_layer_norm(int64_t rows, int channels, const void* feats, int64_t ld_feats, int is_bf16, const float* weights,
+                     const float* bias, float eps, void* out, float* out_mean, float* out_rstd, void* stream);
+/* Its gradients: features [rows, channels], weights and bias [channels] float32 (sums in a fixed order). */
+size_t pccnn_layer_norm_grads_workspace_bytes(int64_t rows, int channels);
+int pccnn_layer_norm_grads(int64_t rows, int channels, const void* feats, int64_t ld_feats, int is_bf16, const float* weights,
+                           const float* mean, const float* rstd, const void* in_grads, int64_t ld_grads, void* out_feat_grads,
+                           float* out_weight_grads, float* out_bias_grads, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rotary positions: neighboring features (2j, 2j + 1) of every head are turned by pts[row, axis(j)] * frequencies[j]
+ * radians.  pts [rows, num_axes] float32, 1 <= num_axes <= 6; axis_pairs_host[a] pairs belong to axis a, in order;
+ * frequencies [sum of axis_pairs] float32; features behind the last pair pass unchanged.  size <= 1024. */
+int pccnn_rotary_positions(int64_t rows, int heads, int size, const void* feats, int64_t row_stride, int64_t head_stride,
+                           int is_bf16, int num_axes, const float* pts, const float* frequencies, const int32_t* axis_pairs_host,
+                           void* out, void* stream);
+/* Its gradients: features [rows, heads, size] and, where out_pt_grads is not null, points [rows, num_axes]. */
+int pccnn_rotary_positions_grads(int64_t rows, int heads, int size, const void* feats, int64_t row_stride, int64_t head_stride,
+                                 int is_bf16, int num_axes, const float* pts, const float* frequencies,
+                                 const int32_t* axis_pairs_host, const void* in_grads, int64_t grad_row_stride,
+                                 int64_t grad_head_stride, void* out_feat_grads, float* out_pt_grads, void* stream);
+
+/* Cross attention: cloud b owns the query rows [query_ends[b-1], query_ends[b]) and the key rows [key_ends[b-1],
+ * key_ends[b]); its queries attend to its keys, out = softmax(scale q k^T) v per head.  query_ends, key_ends [clouds]
+ * int32 on the device, non-decreasing and within the number of rows (offsets that are not are clamped: no access leaves
+ * the tensors, but the result is not defined).  heads is a multiple of kv_heads; head h reads key head
+ * h / (heads / kv_heads).  size <= 256.  out [num_queries, heads, size], out_lse [heads, num_queries] float32 (natural
+ * logarithm).  A query without keys (an empty cloud, a row behind the last cloud) gets zeros and an lse of minus infinity. */
+size_t pccnn_cross_attention_workspace_bytes(int64_t num_queries, int64_t num_keys, int clouds, int heads, int kv_heads, int size,
+                                             int is_bf16);
+int pccnn_cross_attention(int64_t num_queries, int64_t num_keys, int clouds, int heads, int kv_heads, int size, int is_bf16,
+                          const void* queries, const int64_t* query_strides_host, const void* keys,
+                          const int64_t* key_strides_host, const void* values, const int64_t* value_strides_host,
+                          const int32_t* query_ends, const int32_t* key_ends, float scale, void* out, float* out_lse,
+                          void* workspace, size_t workspace_bytes, void* stream);
+/* Its gradients from out and lse of the forward call and in_grads [num_queries, heads, size]: queries
+ * [num_queries, heads, size], keys and values [num_keys, kv_heads, size] (heads that share keys are added up).  Rows
+ * that take part in no attention get zeros.  Every sum is taken in a fixed order. */
+size_t pccnn_cross_attention_grads_workspace_bytes(int64_t num_queries, int64_t num_keys, int clouds, int heads, int kv_heads,
+                                                   int size, int is_bf16);
+int pccnn_cross_attention_grads(int64_t num_queries, int64_t num_keys, int clouds, int heads, int kv_heads, int size, int is_bf16,
+                                const void* queries, const int64_t* query_strides_host, const void* keys,
+                                const int64_t* key_strides_host, const void* values, const int64_t* value_strides_host,
+                                const int32_t* query_ends, const int32_t* key_ends, float scale, const void* out,
+                                const float* lse, const void* in_grads, const int64_t* grad_strides_host,
+                                void* out_query_grads, void* out_key_grads, void* out_value_grads, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------- */
 /* Dense contraction on the tensor cores                                      */
 /* ------------------------------------------------------------------------- */
 

@@ -104,6 +104,21 @@ SIGNATURES = {
                                         _ptr, _ptr, _ptr, _ptr, _size, _ptr]),
     "pccnn_point_conv_weight_var": (_c_int, [_c_i64, _ptr, _c_int, _ptr, _c_int, _c_i64, _ptr, _ptr, _ptr, _ptr, _size,
                                              _ptr]),
+    "pccnn_layer_norm": (_c_int, [_c_i64, _c_int, _ptr, _c_i64, _c_int, _ptr, _ptr, ctypes.c_float, _ptr, _ptr, _ptr, _ptr]),
+    "pccnn_layer_norm_grads_workspace_bytes": (_size, [_c_i64, _c_int]),
+    "pccnn_layer_norm_grads": (_c_int, [_c_i64, _c_int, _ptr, _c_i64, _c_int, _ptr, _ptr, _ptr, _ptr, _c_i64, _ptr, _ptr, _ptr,
+                                        _ptr, _size, _ptr]),
+    "pccnn_rotary_positions": (_c_int, [_c_i64, _c_int, _c_int, _ptr, _c_i64, _c_i64, _c_int, _c_int, _ptr, _ptr, _ptr, _ptr,
+                                        _ptr]),
+    "pccnn_rotary_positions_grads": (_c_int, [_c_i64, _c_int, _c_int, _ptr, _c_i64, _c_i64, _c_int, _c_int, _ptr, _ptr, _ptr,
+                                              _ptr, _c_i64, _c_i64, _ptr, _ptr, _ptr]),
+    "pccnn_cross_attention_workspace_bytes": (_size, [_c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int]),
+    "pccnn_cross_attention": (_c_int, [_c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr,
+                                       _ptr, _ptr, ctypes.c_float, _ptr, _ptr, _ptr, _size, _ptr]),
+    "pccnn_cross_attention_grads_workspace_bytes": (_size, [_c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int]),
+    "pccnn_cross_attention_grads": (_c_int, [_c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr, _ptr, _ptr, _ptr, _ptr,
+                                             _ptr, _ptr, _ptr, ctypes.c_float, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _size,
+                                             _ptr]),
     "pccnn_gemm_workspace_bytes": (_size, [_c_i64, _c_int, _c_int]),
     "pccnn_gemm_f32": (_c_int, [_c_i64, _c_int, _c_int, _ptr, _c_i64, _ptr, _c_i64, _ptr, _c_i64, _c_int, _ptr,
                                 _size, _ptr]),

@@ -1,0 +1,635 @@
+// Cross attention between packed clouds: every query of cloud b attends to the keys of cloud b.
+//
+//   out = softmax(scale q k^T) v,  lse = log sum exp(scale q k^T)      per head; heads / kv_heads heads share keys and values
+//   p = exp(scale q k^T - lse), dp = g v^T, ds = p (dp - sum(g out)):  dq = scale ds k,  dk = scale ds^T q,  dv = p^T g
+//
+// The kernels of this file work on rows: a block owns one query (or, for the keys' gradients, one key) and streams the other
+// side of its cloud.  They serve any head size up to 256, any stride and alignment, and are the ones for few queries: with
+// one query per cloud the call is bound by reading keys and values once, and a query's keys are then split over several
+// blocks whose results are joined by a second kernel.  Sums, maxima and probabilities are 32-bit floats.
+#include <cuda_bf16.h>
+
+#include "attention.cuh"
+#include "common.cuh"
+#include "features.cuh"
+
+namespace pccnn {
+
+constexpr int kRowThreads = 256;
+constexpr int kRowWarps = kRowThreads / 32;
+constexpr int kMaxHeadSize = 256;
+constexpr int kMaxSplits = 64;
+
+// ---- layout of a block: LPK lanes of a warp share a streamed row (V elements each, NC times), 32 / LPK rows per warp ----
+template <class T, int V, int NC>
+__device__ __forceinline__ void load_row(const T* __restrict__ p, int lane_in_row, int lanes_per_row, int size, float (&x)[NC][V]) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int d = (c * lanes_per_row + lane_in_row) * V;
+        if (d < size) {
+            load_vec<T, V>(p + d, x[c]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[c][e] = 0.f;
+        }
+    }
+}
+template <int V, int NC>
+__device__ __forceinline__ float dot(const float (&a)[NC][V], const float (&b)[NC][V]) {
+    float s = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < V; ++e) s = fmaf(a[c][e], b[c][e], s);
+    return s;
+}
+__device__ __forceinline__ float sum_lanes(float v, int lanes) {
+    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+    return v;
+}
+
+// Adds x over the row groups of the block (fixed order); threads of warp 0's first group hold the result.
+template <int V, int NC>
+__device__ __forceinline__ void add_over_block(float (&x)[NC][V], int lanes_per_row, float* scratch) {
+    for (int o = lanes_per_row; o < 32; o <<= 1) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[c][e] += __shfl_xor_sync(kFullMask, x[c][e], o);
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    __syncthreads();
+    if (lane < lanes_per_row) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int e = 0; e < V; ++e) scratch[((warp * NC + c) * 32 + lane) * V + e] = x[c][e];
+    }
+    __syncthreads();
+    if (warp == 0 && lane < lanes_per_row) {
+#pragma unroll
+        for (int w = 1; w < kRowWarps; ++w)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[c][e] += scratch[((w * NC + c) * 32 + lane) * V + e];
+    }
+}
+
+// The part of [begin, end) that split s of `splits` works on.
+__device__ __forceinline__ void split_range(int64_t& begin, int64_t& end, int s, int splits) {
+    const int64_t per = (end - begin + splits - 1) / splits;
+    const int64_t lo = begin + s * per, hi = lo + per;
+    end = hi < end ? hi : end;
+    begin = lo < end ? lo : end;
+}
+
+// ---- forward: block = one query x GH heads that share keys x one split of the keys ------------------------------
+// Without splits the output and lse are written; with splits the block leaves its unnormalised sum (relative to its own
+// maximum), the maximum and the sum of the probabilities.
+template <class T, int V, int NC, int GH>
+__global__ void __launch_bounds__(kRowThreads)
+attention_row_kernel(AttentionCall a, int lanes_per_row, int splits, T* __restrict__ out, float* __restrict__ lse,
+                     float* __restrict__ part_out, float2* __restrict__ part_stat) {
+    constexpr int kUnroll = NC * V * GH > 32 ? 2 : 4;
+    __shared__ float scratch[kRowWarps * NC * 32 * V];
+    __shared__ float stat[kRowWarps][2];
+    const int64_t m = blockIdx.x;
+    const int group = a.heads / a.kv_heads, parts = (group + GH - 1) / GH;
+    const int kv = blockIdx.y / parts, h0 = kv * group + (blockIdx.y % parts) * GH;
+    const int heads_here = min(GH, (kv + 1) * group - h0), split = blockIdx.z;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int in_row = lane % lanes_per_row, sub = lane / lanes_per_row, per_warp = 32 / lanes_per_row;
+
+    const int b = cloud_of_row(a.query_ends, a.clouds, m);
+    int64_t begin = 0, end = 0;
+    if (b < a.clouds) {
+        begin = cloud_begin(a.key_ends, b, a.num_keys);
+        end = cloud_end(a.key_ends, b, a.clouds, a.num_keys);
+    }
+    split_range(begin, end, split, splits);
+
+    const float c2 = a.scale * kLog2e;
+    float q[GH][NC][V], acc[GH][NC][V], top[GH], total[GH];
+#pragma unroll
+    for (int g = 0; g < GH; ++g) {
+        top[g] = -INFINITY;
+        total[g] = 0.f;
+        load_row<T, V, NC>((const T*)a.q.data + m * a.q.row + (h0 + min(g, heads_here - 1)) * a.q.head, in_row, lanes_per_row, a.size, q[g]);
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[g][c][e] = 0.f;
+    }
+    const T* keys = (const T*)a.k.data + kv * a.k.head;
+    const T* values = (const T*)a.v.data + kv * a.v.head;
+    const int step = kRowWarps * per_warp;
+    for (int64_t first = begin + warp * per_warp; first < end; first += (int64_t)step * kUnroll) {  // the same for the warp's lanes
+        float s[GH][kUnroll], val[kUnroll][NC][V];
+        {
+            float key[kUnroll][NC][V];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                const int64_t n = first + u * step + sub;
+                if (n < end) {
+                    load_row<T, V, NC>(keys + n * a.k.row, in_row, lanes_per_row, a.size, key[u]);
+                    load_row<T, V, NC>(values + n * a.v.row, in_row, lanes_per_row, a.size, val[u]);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < NC; ++c)
+#pragma unroll
+                        for (int e = 0; e < V; ++e) key[u][c][e] = val[u][c][e] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < GH; ++g)
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u) s[g][u] = sum_lanes(dot<V, NC>(q[g], key[u]), lanes_per_row) * c2;
+        }
+#pragma unroll
+        for (int g = 0; g < GH; ++g) {
+            float now = top[g];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                if (first + u * step + sub >= end) s[g][u] = -INFINITY;
+                now = fmaxf(now, s[g][u]);
+            }
+            const float from = now == -INFINITY ? 0.f : now;
+            const float fade = exp2_fast(top[g] - from);
+            top[g] = now;
+            total[g] *= fade;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[g][c][e] *= fade;
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                const float p = exp2_fast(s[g][u] - from);
+                total[g] += p;
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) acc[g][c][e] = fmaf(p, val[u][c][e], acc[g][c][e]);
+            }
+        }
+    }
+    // join the row groups of the block
+#pragma unroll
+    for (int g = 0; g < GH; ++g) {
+        if (g >= heads_here) break;  // the same for the whole block
+        float now = top[g];
+        for (int o = lanes_per_row; o < 32; o <<= 1) now = fmaxf(now, __shfl_xor_sync(kFullMask, now, o));
+        if (lane == 0) stat[warp][0] = now;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kRowWarps; ++w) now = fmaxf(now, stat[w][0]);
+        const float from = now == -INFINITY ? 0.f : now;
+        const float fade = exp2_fast(top[g] - from);
+        float sum = total[g] * fade;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[g][c][e] *= fade;
+        for (int o = lanes_per_row; o < 32; o <<= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+        if (lane == 0) stat[warp][1] = sum;
+        add_over_block<V, NC>(acc[g], lanes_per_row, scratch);  // synchronises, so `stat` is complete
+        if (warp == 0) {
+            sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kRowWarps; ++w) sum += stat[w][1];
+            const int64_t at = m * a.heads + h0 + g;
+            if (splits > 1) {
+                const int64_t slot = (int64_t)split * a.num_queries * a.heads + at;
+                if (lane == 0) part_stat[slot] = make_float2(now, sum);
+                if (lane < lanes_per_row) {
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        const int d = (c * lanes_per_row + lane) * V;
+                        if (d < a.size) store_vec<float, V>(part_out + slot * a.size + d, acc[g][c]);
+                    }
+                }
+            } else {
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                if (lane == 0) lse[(int64_t)(h0 + g) * a.num_queries + m] = sum == 0.f ? -INFINITY : (now + log2f(sum)) * kLn2;
+                if (lane < lanes_per_row) {
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        const int d = (c * lanes_per_row + lane) * V;
+#pragma unroll
+                        for (int e = 0; e < V; ++e) acc[g][c][e] *= inv;
+                        if (d < a.size) store_vec<T, V>(out + at * a.size + d, acc[g][c]);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Joins the splits of a query: one warp per (query, head).
+template <class T>
+__global__ void __launch_bounds__(256)
+attention_join_kernel(int64_t num_queries, int heads, int size, int splits, const float* __restrict__ part_out,
+                      const float2* __restrict__ part_stat, T* __restrict__ out, float* __restrict__ lse) {
+    const int64_t rows = num_queries * heads, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= rows) return;
+    float top = -INFINITY;
+    for (int s = 0; s < splits; ++s) top = fmaxf(top, part_stat[s * rows + row].x);
+    const float from = top == -INFINITY ? 0.f : top;
+    float total = 0.f, acc[kMaxHeadSize / 32];
+#pragma unroll
+    for (int i = 0; i < kMaxHeadSize / 32; ++i) acc[i] = 0.f;
+    for (int s = 0; s < splits; ++s) {
+        const float2 st = part_stat[s * rows + row];
+        if (st.y == 0.f) continue;  // a split without keys: its sum is not read
+        const float f = exp2_fast(st.x - from);
+        total += st.y * f;
+#pragma unroll
+        for (int i = 0; i < kMaxHeadSize / 32; ++i)
+            if (i * 32 + lane < size) acc[i] = fmaf(f, part_out[(s * rows + row) * size + i * 32 + lane], acc[i]);
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    if (lane == 0) lse[(row % heads) * num_queries + row / heads] = total == 0.f ? -INFINITY : (top + log2f(total)) * kLn2;
+#pragma unroll
+    for (int i = 0; i < kMaxHeadSize / 32; ++i)
+        if (i * 32 + lane < size) out[row * size + i * 32 + lane] = from_float<T>(acc[i] * inv);
+}
+
+// ---- backward ---------------------------------------------------------------------------------------------------
+// delta[h, m] = sum_d out g: one warp per (query, head).
+template <class T>
+__global__ void __launch_bounds__(256)
+attention_delta_kernel(int64_t num_queries, int heads, int size, const T* __restrict__ out, HeadRows grads, float* __restrict__ delta) {
+    const int64_t rows = num_queries * heads, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= rows) return;
+    const int64_t m = row / heads;
+    const int h = (int)(row % heads);
+    const T* g = (const T*)grads.data + m * grads.row + h * grads.head;
+    float s = 0.f;
+    for (int d = lane; d < size; d += 32) s = fmaf(to_float(out[row * size + d]), to_float(g[d]), s);
+    s = warp_sum(s);
+    if (lane == 0) delta[(int64_t)h * num_queries + m] = s;
+}
+
+// Queries' gradient: block = one query and head x one split of its keys.
+template <class T, int V, int NC>
+__global__ void __launch_bounds__(kRowThreads)
+attention_query_grads_row_kernel(AttentionCall a, HeadRows grads, int lanes_per_row, int splits, const float* __restrict__ lse,
+                                 const float* __restrict__ delta, T* __restrict__ out, float* __restrict__ part) {
+    __shared__ float scratch[kRowWarps * NC * 32 * V];
+    const int64_t m = blockIdx.x;
+    const int h = blockIdx.y, kv = h / (a.heads / a.kv_heads), split = blockIdx.z;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int in_row = lane % lanes_per_row, sub = lane / lanes_per_row, per_warp = 32 / lanes_per_row;
+    const int b = cloud_of_row(a.query_ends, a.clouds, m);
+    int64_t begin = 0, end = 0;
+    if (b < a.clouds) {
+        begin = cloud_begin(a.key_ends, b, a.num_keys);
+        end = cloud_end(a.key_ends, b, a.clouds, a.num_keys);
+    }
+    split_range(begin, end, split, splits);
+    const float c2 = a.scale * kLog2e;
+    const float row_lse = lse[(int64_t)h * a.num_queries + m], base = row_lse == -INFINITY ? INFINITY : row_lse * kLog2e;
+    const float row_delta = delta[(int64_t)h * a.num_queries + m];
+    float q[NC][V], g[NC][V], acc[NC][V];
+    load_row<T, V, NC>((const T*)a.q.data + m * a.q.row + h * a.q.head, in_row, lanes_per_row, a.size, q);
+    load_row<T, V, NC>((const T*)grads.data + m * grads.row + h * grads.head, in_row, lanes_per_row, a.size, g);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[c][e] = 0.f;
+    const T* keys = (const T*)a.k.data + kv * a.k.head;
+    const T* values = (const T*)a.v.data + kv * a.v.head;
+    for (int64_t first = begin + warp * per_warp; first < end; first += kRowWarps * per_warp) {
+        const int64_t n = first + sub;
+        const bool in = n < end;
+        float key[NC][V], val[NC][V];
+        load_row<T, V, NC>(keys + (in ? n : begin) * a.k.row, in_row, lanes_per_row, a.size, key);
+        load_row<T, V, NC>(values + (in ? n : begin) * a.v.row, in_row, lanes_per_row, a.size, val);
+        const float s = sum_lanes(dot<V, NC>(q, key), lanes_per_row);
+        const float dp = sum_lanes(dot<V, NC>(g, val), lanes_per_row);
+        const float ds = exp2_fast(s * c2 - base) * (dp - row_delta);
+        if (in) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[c][e] = fmaf(ds, key[c][e], acc[c][e]);
+        }
+    }
+    add_over_block<V, NC>(acc, lanes_per_row, scratch);
+    if (warp == 0 && lane < lanes_per_row) {
+        const int64_t at = (m * a.heads + h) * a.size;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int d = (c * lanes_per_row + lane) * V;
+            if (d >= a.size) break;
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[c][e] *= a.scale;
+            if (splits > 1) store_vec<float, V>(part + (int64_t)split * a.num_queries * a.heads * a.size + at + d, acc[c]);
+            else store_vec<T, V>(out + at + d, acc[c]);
+        }
+    }
+}
+
+// Keys' and values' gradients: block = one key and its head x one split of the queries; the heads that share it are added.
+template <class T, int V, int NC>
+__global__ void __launch_bounds__(kRowThreads)
+attention_key_grads_row_kernel(AttentionCall a, HeadRows grads, int lanes_per_row, int splits, const float* __restrict__ lse,
+                               const float* __restrict__ delta, T* __restrict__ out_k, T* __restrict__ out_v,
+                               float* __restrict__ part_k, float* __restrict__ part_v) {
+    __shared__ float scratch[kRowWarps * NC * 32 * V];
+    const int64_t n = blockIdx.x;
+    const int kv = blockIdx.y, group = a.heads / a.kv_heads, split = blockIdx.z;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int in_row = lane % lanes_per_row, sub = lane / lanes_per_row, per_warp = 32 / lanes_per_row;
+    const int b = cloud_of_row(a.key_ends, a.clouds, n);
+    int64_t begin = 0, end = 0;
+    if (b < a.clouds) {
+        begin = cloud_begin(a.query_ends, b, a.num_queries);
+        end = cloud_end(a.query_ends, b, a.clouds, a.num_queries);
+    }
+    split_range(begin, end, split, splits);
+    const float c2 = a.scale * kLog2e;
+    float key[NC][V], val[NC][V], dk[NC][V], dv[NC][V];
+    load_row<T, V, NC>((const T*)a.k.data + n * a.k.row + kv * a.k.head, in_row, lanes_per_row, a.size, key);
+    load_row<T, V, NC>((const T*)a.v.data + n * a.v.row + kv * a.v.head, in_row, lanes_per_row, a.size, val);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < V; ++e) dk[c][e] = dv[c][e] = 0.f;
+    for (int h = kv * group; h < (kv + 1) * group; ++h) {
+        const T* queries = (const T*)a.q.data + h * a.q.head;
+        const T* g_rows = (const T*)grads.data + h * grads.head;
+        for (int64_t first = begin + warp * per_warp; first < end; first += kRowWarps * per_warp) {
+            const bool in = first + sub < end;
+            const int64_t m = in ? first + sub : begin;
+            float q[NC][V], g[NC][V];
+            load_row<T, V, NC>(queries + m * a.q.row, in_row, lanes_per_row, a.size, q);
+            load_row<T, V, NC>(g_rows + m * grads.row, in_row, lanes_per_row, a.size, g);
+            const float row_lse = lse[(int64_t)h * a.num_queries + m];
+            const float s = sum_lanes(dot<V, NC>(q, key), lanes_per_row);
+            const float dp = sum_lanes(dot<V, NC>(g, val), lanes_per_row);
+            const float p = exp2_fast(s * c2 - (row_lse == -INFINITY ? INFINITY : row_lse * kLog2e));
+            const float ds = p * (dp - delta[(int64_t)h * a.num_queries + m]);
+            if (in) {
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        dk[c][e] = fmaf(ds, q[c][e], dk[c][e]);
+                        dv[c][e] = fmaf(p, g[c][e], dv[c][e]);
+                    }
+            }
+        }
+    }
+    add_over_block<V, NC>(dk, lanes_per_row, scratch);
+    __syncthreads();
+    add_over_block<V, NC>(dv, lanes_per_row, scratch);
+    if (warp == 0 && lane < lanes_per_row) {
+        const int64_t at = (n * a.kv_heads + kv) * a.size, shift = (int64_t)split * a.num_keys * a.kv_heads * a.size;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int d = (c * lanes_per_row + lane) * V;
+            if (d >= a.size) break;
+#pragma unroll
+            for (int e = 0; e < V; ++e) dk[c][e] *= a.scale;
+            if (splits > 1) {
+                store_vec<float, V>(part_k + shift + at + d, dk[c]);
+                store_vec<float, V>(part_v + shift + at + d, dv[c]);
+            } else {
+                store_vec<T, V>(out_k + at + d, dk[c]);
+                store_vec<T, V>(out_v + at + d, dv[c]);
+            }
+        }
+    }
+}
+
+// out = the sum of the splits' parts, in ascending order.
+template <class T>
+__global__ void __launch_bounds__(256)
+add_splits_kernel(int64_t count, int splits, const float* __restrict__ part, T* __restrict__ out) {
+    for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+        float v = 0.f;
+        for (int s = 0; s < splits; ++s) v += part[s * count + i];
+        out[i] = from_float<T>(v);
+    }
+}
+
+// ---- host: choice of the kernel -----------------------------------------------------------------------------------
+// 16-byte vectors need a head size and strides that are multiples of one and 16-byte aligned data; anything else goes
+// element by element.
+static bool vector_heads(const HeadRows& x, int v) { return aligned16(x.data) && x.row % v == 0 && x.head % v == 0; }
+
+struct RowLayout {
+    bool vectors;
+    int chunks, lanes;
+};
+static RowLayout row_layout(const AttentionCall& a, const HeadRows* grads) {
+    const int v = a.is_bf16 ? 8 : 4;
+    RowLayout l;
+    l.vectors = a.size % v == 0 && vector_heads(a.q, v) && vector_heads(a.k, v) && vector_heads(a.v, v) && (!grads || vector_heads(*grads, v));
+    const int n = l.vectors ? a.size / v : a.size;
+    l.lanes = 1;
+    while (l.lanes < 32 && l.lanes < n) l.lanes *= 2;
+    l.chunks = 1;
+    while (l.chunks * l.lanes < n) l.chunks *= 2;
+    return l;
+}
+
+// How many blocks share the `streamed` rows of a cloud (on average) when there are `units` blocks without a split: enough to
+// give every SM about four blocks, as long as a block keeps at least 256 rows.
+static int choose_splits(int64_t units, int64_t streamed_per_cloud) {
+    const int64_t want = (int64_t)sm_count() * 4;
+    int64_t s = units > 0 ? (want + units - 1) / units : 1;
+    const int64_t most = streamed_per_cloud / 256;
+    if (s > most) s = most;
+    return (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
+}
+
+static int64_t mean_rows(int64_t n, int clouds) { return n / (clouds > 0 ? clouds : 1); }
+
+// GH heads that share keys are served by one pass over them where there are at least two.
+static int forward_parts(const AttentionCall& a) {
+    const int group = a.heads / a.kv_heads;
+    return group >= 2 ? (group + 3) / 4 : 1;
+}
+
+static int forward_splits(const AttentionCall& a) {
+    return choose_splits(a.num_queries * a.kv_heads * forward_parts(a), mean_rows(a.num_keys, a.clouds));
+}
+static int query_grad_splits(const AttentionCall& a) {
+    return choose_splits(a.num_queries * a.heads, mean_rows(a.num_keys, a.clouds));
+}
+static int key_grad_splits(const AttentionCall& a) {
+    return choose_splits(a.num_keys * a.kv_heads, mean_rows(a.num_queries, a.clouds));
+}
+
+template <class T, int V, int NC>
+static int launch_rows(const AttentionCall& a, const RowLayout& l, void* out, float* lse, char* ws, cudaStream_t s) {
+    const int splits = forward_splits(a);
+    float2* stat = (float2*)ws;
+    float* part = (float*)(ws + align_up((size_t)splits * a.num_queries * a.heads * sizeof(float2)));
+    const dim3 grid((unsigned)a.num_queries, (unsigned)(a.kv_heads * forward_parts(a)), (unsigned)splits);
+    if (a.heads > a.kv_heads) attention_row_kernel<T, V, NC, 4><<<grid, kRowThreads, 0, s>>>(a, l.lanes, splits, (T*)out, lse, part, stat);
+    else attention_row_kernel<T, V, NC, 1><<<grid, kRowThreads, 0, s>>>(a, l.lanes, splits, (T*)out, lse, part, stat);
+    PCCNN_LAUNCH_CHECK();
+    if (splits > 1) {
+        attention_join_kernel<T><<<(unsigned)((a.num_queries * a.heads + 7) / 8), 256, 0, s>>>(a.num_queries, a.heads, a.size, splits, part,
+                                                                                             stat, (T*)out, lse);
+        PCCNN_LAUNCH_CHECK();
+    }
+    return PCCNN_OK;
+}
+
+template <class T>
+static int add_splits(int64_t count, int splits, const float* part, void* out, cudaStream_t s) {
+    add_splits_kernel<T><<<grid_for(count, 256, 8), 256, 0, s>>>(count, splits, part, (T*)out);
+    PCCNN_LAUNCH_CHECK();
+    return PCCNN_OK;
+}
+
+template <class T, int V, int NC>
+static int launch_grad_rows(const AttentionCall& a, const HeadRows& grads, const RowLayout& l, const float* lse, const float* delta,
+                            void* dq, void* dk, void* dv, char* ws, cudaStream_t s) {
+    float* part = (float*)ws;
+    if (a.num_queries > 0) {
+        const int splits = query_grad_splits(a);
+        attention_query_grads_row_kernel<T, V, NC><<<dim3((unsigned)a.num_queries, (unsigned)a.heads, (unsigned)splits), kRowThreads, 0, s>>>(
+            a, grads, l.lanes, splits, lse, delta, (T*)dq, part);
+        PCCNN_LAUNCH_CHECK();
+        if (splits > 1)
+            if (int rc = add_splits<T>(a.num_queries * a.heads * a.size, splits, part, dq, s)) return rc;
+    }
+    if (a.num_keys > 0) {
+        const int splits = key_grad_splits(a);
+        const int64_t count = a.num_keys * a.kv_heads * a.size;
+        attention_key_grads_row_kernel<T, V, NC><<<dim3((unsigned)a.num_keys, (unsigned)a.kv_heads, (unsigned)splits), kRowThreads, 0, s>>>(
+            a, grads, l.lanes, splits, lse, delta, (T*)dk, (T*)dv, part, part + splits * count);
+        PCCNN_LAUNCH_CHECK();
+        if (splits > 1) {
+            if (int rc = add_splits<T>(count, splits, part, dk, s)) return rc;
+            if (int rc = add_splits<T>(count, splits, part + splits * count, dv, s)) return rc;
+        }
+    }
+    return PCCNN_OK;
+}
+
+template <class T, class F>
+static int dispatch_rows(const RowLayout& l, const F& f) {
+    constexpr int kV = 16 / sizeof(T);
+    if (l.vectors) return l.chunks == 1 ? f.template run<T, kV, 1>() : f.template run<T, kV, 2>();
+    if (l.chunks == 1) return f.template run<T, 1, 1>();
+    if (l.chunks == 2) return f.template run<T, 1, 2>();
+    return l.chunks == 4 ? f.template run<T, 1, 4>() : f.template run<T, 1, 8>();
+}
+
+struct ForwardRows {
+    const AttentionCall& a; RowLayout l; void* out; float* lse; char* ws; cudaStream_t s;
+    template <class T, int V, int NC> int run() const { return launch_rows<T, V, NC>(a, l, out, lse, ws, s); }
+};
+struct BackwardRows {
+    const AttentionCall& a; const HeadRows& grads; RowLayout l; const float *lse, *delta; void *dq, *dk, *dv; char* ws; cudaStream_t s;
+    template <class T, int V, int NC> int run() const { return launch_grad_rows<T, V, NC>(a, grads, l, lse, delta, dq, dk, dv, ws, s); }
+};
+
+static int check_call(const char* who, const AttentionCall& a) {
+    PCCNN_CHECK_ARG(a.num_queries >= 0 && a.num_queries < 0x7fffffffLL && a.num_keys >= 0 && a.num_keys < 0x7fffffffLL && a.clouds >= 0,
+                    "%s: bad number of rows", who);
+    PCCNN_CHECK_ARG(a.heads > 0 && a.heads <= 1024 && a.kv_heads > 0 && a.heads % a.kv_heads == 0,
+                    "%s: %d heads cannot share %d key heads (at most 1024 heads, a multiple of the key heads)", who, a.heads, a.kv_heads);
+    PCCNN_CHECK_ARG(a.size > 0 && a.size <= kMaxHeadSize, "%s: head size %d outside [1, %d]", who, a.size, kMaxHeadSize);
+    PCCNN_CHECK_ARG(a.clouds == 0 || (a.query_ends && a.key_ends), "%s: null pointer", who);
+    PCCNN_CHECK_ARG((a.num_queries == 0 || a.q.data) && (a.num_keys == 0 || (a.k.data && a.v.data)), "%s: null pointer", who);
+    return PCCNN_OK;
+}
+
+static AttentionCall describe(int64_t num_queries, int64_t num_keys, int clouds, int heads, int kv_heads, int size, int is_bf16,
+                              const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                              const int64_t* v_strides, const int32_t* query_ends, const int32_t* key_ends, float scale) {
+    AttentionCall a{num_queries, num_keys, clouds, heads, kv_heads, size, is_bf16, {q, 0, 0}, {k, 0, 0}, {v, 0, 0}, query_ends, key_ends, scale};
+    if (q_strides) a.q.row = q_strides[0], a.q.head = q_strides[1];
+    if (k_strides) a.k.row = k_strides[0], a.k.head = k_strides[1];
+    if (v_strides) a.v.row = v_strides[0], a.v.head = v_strides[1];
+    return a;
+}
+
+}  // namespace pccnn
+
+using namespace pccnn;
+
+extern "C" {
+
+size_t pccnn_cross_attention_workspace_bytes(int64_t num_queries, int64_t num_keys, int clouds, int heads, int kv_heads, int size,
+                                             int is_bf16) {
+    if (num_queries <= 0 || num_keys <= 0 || heads <= 0 || kv_heads <= 0 || size <= 0) return 256;
+    const AttentionCall a = describe(num_queries, num_keys, clouds, heads, kv_heads, size, is_bf16, nullptr, nullptr, nullptr, nullptr,
+                                     nullptr, nullptr, nullptr, nullptr, 1.f);
+    const int splits = forward_splits(a);
+    if (splits == 1) return 256;
+    const size_t rows = (size_t)splits * num_queries * heads;
+    return align_up(rows * sizeof(float2)) + align_up(rows * size * 4);
+}
+
+int pccnn_cross_attention(int64_t num_queries, int64_t num_keys, int clouds, int heads, int kv_heads, int size, int is_bf16,
+                          const void* queries, const int64_t* query_strides_host, const void* keys, const int64_t* key_strides_host,
+                          const void* values, const int64_t* value_strides_host, const int32_t* query_ends, const int32_t* key_ends,
+                          float scale, void* out, float* out_lse, void* workspace, size_t workspace_bytes, void* stream) {
+    const AttentionCall a = describe(num_queries, num_keys, clouds, heads, kv_heads, size, is_bf16, queries, query_strides_host, keys,
+                                     key_strides_host, values, value_strides_host, query_ends, key_ends, scale);
+    if (int rc = check_call("cross_attention", a)) return rc;
+    PCCNN_CHECK_ARG(query_strides_host && key_strides_host && value_strides_host, "cross_attention: null pointer");
+    if (num_queries == 0) return PCCNN_OK;
+    PCCNN_CHECK_ARG(out && out_lse, "cross_attention: null pointer");
+    const size_t need = pccnn_cross_attention_workspace_bytes(num_queries, num_keys, clouds, heads, kv_heads, size, is_bf16);
+    if (!workspace || workspace_bytes < need) {
+        set_error("cross_attention: workspace of %zu bytes, need %zu", workspace_bytes, need);
+        return PCCNN_ERR_WORKSPACE;
+    }
+    const ForwardRows f{a, row_layout(a, nullptr), out, out_lse, (char*)workspace, (cudaStream_t)stream};
+    return is_bf16 ? dispatch_rows<__nv_bfloat16>(f.l, f) : dispatch_rows<float>(f.l, f);
+}
+
+size_t pccnn_cross_attention_grads_workspace_bytes(int64_t num_queries, int64_t num_keys, int clouds, int heads, int kv_heads, int size,
+                                                   int is_bf16) {
+    if (num_queries < 0 || num_keys < 0 || heads <= 0 || kv_heads <= 0 || size <= 0) return 256;
+    const AttentionCall a = describe(num_queries, num_keys, clouds, heads, kv_heads, size, is_bf16, nullptr, nullptr, nullptr, nullptr,
+                                     nullptr, nullptr, nullptr, nullptr, 1.f);
+    const size_t sq = query_grad_splits(a), sk = key_grad_splits(a);
+    const size_t pq = sq > 1 ? sq * num_queries * heads * size * 4 : 0, pk = sk > 1 ? 2 * sk * num_keys * kv_heads * size * 4 : 0;
+    return align_up((size_t)num_queries * heads * 4 + 256) + align_up(pq > pk ? pq : pk);
+}
+
+int pccnn_cross_attention_grads(int64_t num_queries, int64_t num_keys, int clouds, int heads, int kv_heads, int size, int is_bf16,
+                                const void* queries, const int64_t* query_strides_host, const void* keys,
+                                const int64_t* key_strides_host, const void* values, const int64_t* value_strides_host,
+                                const int32_t* query_ends, const int32_t* key_ends, float scale, const void* out, const float* lse,
+                                const void* in_grads, const int64_t* grad_strides_host, void* out_query_grads, void* out_key_grads,
+                                void* out_value_grads, void* workspace, size_t workspace_bytes, void* stream) {
+    const AttentionCall a = describe(num_queries, num_keys, clouds, heads, kv_heads, size, is_bf16, queries, query_strides_host, keys,
+                                     key_strides_host, values, value_strides_host, query_ends, key_ends, scale);
+    if (int rc = check_call("cross_attention_grads", a)) return rc;
+    PCCNN_CHECK_ARG(query_strides_host && key_strides_host && value_strides_host && grad_strides_host, "cross_attention_grads: null pointer");
+    PCCNN_CHECK_ARG((num_queries == 0 || (out && lse && in_grads && out_query_grads)) && (num_keys == 0 || (out_key_grads && out_value_grads)),
+                    "cross_attention_grads: null pointer");
+    const size_t need = pccnn_cross_attention_grads_workspace_bytes(num_queries, num_keys, clouds, heads, kv_heads, size, is_bf16);
+    if (!workspace || workspace_bytes < need) {
+        set_error("cross_attention_grads: workspace of %zu bytes, need %zu", workspace_bytes, need);
+        return PCCNN_ERR_WORKSPACE;
+    }
+    cudaStream_t s = (cudaStream_t)stream;
+    const HeadRows grads{in_grads, grad_strides_host[0], grad_strides_host[1]};
+    float* delta = (float*)workspace;
+    char* rest = (char*)workspace + align_up((size_t)num_queries * heads * 4 + 256);
+    if (num_queries > 0) {
+        const unsigned blocks = (unsigned)((num_queries * heads + 7) / 8);
+        if (is_bf16) attention_delta_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(num_queries, heads, size, (const __nv_bfloat16*)out, grads, delta);
+        else attention_delta_kernel<float><<<blocks, 256, 0, s>>>(num_queries, heads, size, (const float*)out, grads, delta);
+        PCCNN_LAUNCH_CHECK();
+    }
+    const BackwardRows b{a, grads, row_layout(a, &grads), lse, delta, out_query_grads, out_key_grads, out_value_grads, rest, s};
+    return is_bf16 ? dispatch_rows<__nv_bfloat16>(b.l, b) : dispatch_rows<float>(b.l, b);
+}
+
+}  // extern "C"

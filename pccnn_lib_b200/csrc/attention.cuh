@@ -1,0 +1,61 @@
+// What the kernels of cross attention on packed clouds share: the description of a call, the rows of a cloud, and the
+// launchers that attention.cu chooses from.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace pccnn {
+
+// [rows, heads, size] with any row and head stride (in elements) and contiguous features.
+struct HeadRows {
+    const void* data;
+    int64_t row, head;
+};
+
+struct AttentionCall {
+    int64_t num_queries, num_keys;
+    int clouds, heads, kv_heads, size, is_bf16;
+    HeadRows q, k, v;
+    const int32_t *query_ends, *key_ends;
+    float scale;
+};
+
+#ifdef __CUDACC__
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// 2^x as the hardware computes it (relative error 2^-22, subnormal results become zero).
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Rows of cloud b: [begin, end).  Whatever the end offsets hold, the range lies inside [0, n).  Cloud `clouds` is
+// the rest: rows behind the last cloud.
+__device__ __forceinline__ int64_t cloud_begin(const int32_t* __restrict__ ends, int b, int64_t n) {
+    const int64_t e = b > 0 ? (int64_t)ends[b - 1] : 0;
+    return e < 0 ? 0 : e < n ? e : n;
+}
+__device__ __forceinline__ int64_t cloud_end(const int32_t* __restrict__ ends, int b, int clouds, int64_t n) {
+    if (b >= clouds) return n;
+    const int64_t lo = cloud_begin(ends, b, n), e = (int64_t)ends[b];
+    return e < lo ? lo : e < n ? e : n;
+}
+
+// First cloud whose end lies behind `row` (`clouds`: none).
+__device__ __forceinline__ int cloud_of_row(const int32_t* __restrict__ ends, int clouds, int64_t row) {
+    int lo = 0, hi = clouds;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if ((int64_t)ends[mid] > row) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+#endif  // __CUDACC__
+
+}  // namespace pccnn

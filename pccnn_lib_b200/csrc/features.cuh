@@ -1,0 +1,64 @@
+// Loads and stores of feature vectors in float32 or bfloat16: V consecutive elements as one 16-byte access where V says
+// so, as single elements for V = 1 (and element by element for the other small V).  Arithmetic is 32-bit throughout.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <stdint.h>
+
+namespace pccnn {
+
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+#ifdef __CUDACC__
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <class T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
+// The one rounding of a bf16 result: to nearest, from a 32-bit value.
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+template <class T, int V>
+__device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&v)[V]) {
+    if constexpr (sizeof(T) == 4 && V % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            const float4 r = *reinterpret_cast<const float4*>(p + i);
+            v[i] = r.x, v[i + 1] = r.y, v[i + 2] = r.z, v[i + 3] = r.w;
+        }
+    } else if constexpr (sizeof(T) == 2 && V == 8) {
+        const uint4 r = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = to_float(p[i]);
+    }
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <class T, int V>
+__device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&v)[V]) {
+    if constexpr (sizeof(T) == 4 && V % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    } else if constexpr (sizeof(T) == 2 && V == 8) {
+        *reinterpret_cast<uint4*>(p) =
+            make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) p[i] = from_float<T>(v[i]);
+    }
+}
+
+#endif  // __CUDACC__
+
+}  // namespace pccnn

@@ -1,0 +1,386 @@
+// Layer norm over the channels of packed point features, forward and backward.
+//
+//   y = (x - mu) r w + b            mu = mean_c x,  r = 1 / sqrt(mean_c (x - mu)^2 + eps)
+//   dx = r (g w - mean_c(g w) - xhat mean_c(g w xhat)),   dw = sum_n g xhat,   db = sum_n g,   xhat = (x - mu) r
+//
+// Both directions are bound by HBM: the forward pass reads x and writes y once, the backward pass reads x and g and
+// writes dx once.  A row is held in the registers of TPR threads (a part of a warp, a warp, or a block), so the variance
+// is taken around the finished mean without a second read.  The backward kernel keeps the column sums of its rows in
+// registers, every block writes one row of partial sums, and a second small kernel adds the blocks' rows in ascending
+// order: no atomics, the same bits on every run.  Statistics and sums are 32-bit floats whatever the features' type.
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+#include "features.cuh"
+
+namespace pccnn {
+
+constexpr int kNormThreads = 256;
+
+// Sum over the TPR consecutive threads that share a row; every one of them gets it.  TPR = 256 uses shared memory
+// (one slot set per call site parity) and needs all threads of the block.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* slots) {
+    constexpr int kLanes = TPR < 32 ? TPR : 32;
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+    if (TPR > 32) {
+        __syncthreads();
+        if (lane_id() == 0) slots[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kNormThreads / 32; ++w) v += slots[w];
+    }
+    return v;
+}
+
+// One row per TPR threads, K vectors of V elements per thread.
+template <class T, int V, int TPR, int K>
+__global__ void __launch_bounds__(kNormThreads)
+layer_norm_kernel(int64_t rows, int channels, const T* __restrict__ feats, int64_t ld, const float* __restrict__ weights,
+                  const float* __restrict__ bias, float eps, T* __restrict__ out, float* __restrict__ out_mean,
+                  float* __restrict__ out_rstd) {
+    __shared__ float slots[kNormThreads / 32];
+    const int t = threadIdx.x % TPR;
+    const int64_t row = (int64_t)blockIdx.x * (kNormThreads / TPR) + threadIdx.x / TPR;
+    const bool live = row < rows;
+    const T* src = feats + (live ? row : 0) * ld;
+    float x[K][V];
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int c = (k * TPR + t) * V;
+        if (live && c < channels) {
+            load_vec<T, V>(src + c, x[k]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[k][e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum += x[k][e];
+    }
+    const float mean = row_sum<TPR>(sum, slots) / (float)channels;
+    float sq = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const bool in = (k * TPR + t) * V < channels;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float d = x[k][e] - mean;
+            sq += in ? d * d : 0.f;
+        }
+    }
+    const float rstd = 1.f / sqrtf(row_sum<TPR>(sq, slots) / (float)channels + eps);
+    if (!live) return;
+    if (t == 0) {
+        out_mean[row] = mean;
+        out_rstd[row] = rstd;
+    }
+    T* dst = out + row * channels;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int c = (k * TPR + t) * V;
+        if (c >= channels) break;
+        float w[V], b[V], y[V];
+        load_vec<float, V>(weights + c, w);
+        load_vec<float, V>(bias + c, b);
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[e] = (x[k][e] - mean) * rstd * w[e] + b[e];
+        store_vec<T, V>(dst + c, y);
+    }
+}
+
+// Rows that do not fit the registers of a block: three passes over the row, which the first one leaves in the caches.
+template <class T>
+__global__ void __launch_bounds__(kNormThreads)
+layer_norm_wide_kernel(int channels, const T* __restrict__ feats, int64_t ld, const float* __restrict__ weights,
+                       const float* __restrict__ bias, float eps, T* __restrict__ out, float* __restrict__ out_mean,
+                       float* __restrict__ out_rstd) {
+    __shared__ float slots[kNormThreads / 32];
+    const int64_t row = blockIdx.x;
+    const T* src = feats + row * ld;
+    float sum = 0.f, sq = 0.f;
+    for (int c = threadIdx.x; c < channels; c += kNormThreads) sum += to_float(src[c]);
+    const float mean = row_sum<kNormThreads>(sum, slots) / (float)channels;
+    for (int c = threadIdx.x; c < channels; c += kNormThreads) {
+        const float d = to_float(src[c]) - mean;
+        sq += d * d;
+    }
+    const float rstd = 1.f / sqrtf(row_sum<kNormThreads>(sq, slots) / (float)channels + eps);
+    if (threadIdx.x == 0) {
+        out_mean[row] = mean;
+        out_rstd[row] = rstd;
+    }
+    for (int c = threadIdx.x; c < channels; c += kNormThreads)
+        out[row * channels + c] = from_float<T>((to_float(src[c]) - mean) * rstd * weights[c] + bias[c]);
+}
+
+// Backward: the block's row groups walk the rows with a stride of the whole grid; column sums stay in registers and are
+// added over the groups of the block, in ascending order, at the end.
+template <class T, int V, int TPR, int K>
+__global__ void __launch_bounds__(kNormThreads)
+layer_norm_grads_kernel(int64_t rows, int channels, const T* __restrict__ feats, int64_t ld, const float* __restrict__ weights,
+                        const float* __restrict__ mean, const float* __restrict__ rstd, const T* __restrict__ grads,
+                        int64_t ld_g, T* __restrict__ out, float* __restrict__ partial) {
+    constexpr int kGroups = kNormThreads / TPR;
+    extern __shared__ float sums[];  // [2][channels], where several rows share a block (at most 1024 channels: 8 KB)
+    __shared__ float slots[kNormThreads / 32];
+    const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    float w[K][V], dw[K][V], db[K][V];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int c = (k * TPR + t) * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[k][e] = dw[k][e] = db[k][e] = 0.f;
+        if (c < channels) load_vec<float, V>(weights + c, w[k]);
+    }
+    const float inv = 1.f / (float)channels;
+    for (int64_t base = (int64_t)blockIdx.x * kGroups; base < rows; base += (int64_t)gridDim.x * kGroups) {
+        const int64_t row = base + group;
+        const bool live = row < rows;  // every thread of the warp stays for the shuffles
+        const float mu = live ? mean[row] : 0.f, r = live ? rstd[row] : 0.f;
+        float x[K][V], g[K][V];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c = (k * TPR + t) * V;
+            if (live && c < channels) {
+                load_vec<T, V>(feats + row * ld + c, x[k]);
+                load_vec<T, V>(grads + row * ld_g + c, g[k]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[k][e] = mu, g[k][e] = 0.f;
+            }
+        }
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float hat = (x[k][e] - mu) * r;
+                dw[k][e] += g[k][e] * hat;
+                db[k][e] += g[k][e];
+                x[k][e] = hat;
+                g[k][e] *= w[k][e];
+                s1 += g[k][e];
+                s2 += g[k][e] * hat;
+            }
+        }
+        s1 = row_sum<TPR>(s1, slots) * inv;
+        s2 = row_sum<TPR>(s2, slots) * inv;
+        if (!live) continue;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c = (k * TPR + t) * V;
+            if (c >= channels) break;
+            float y[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) y[e] = r * (g[k][e] - s1 - x[k][e] * s2);
+            store_vec<T, V>(out + row * channels + c, y);
+        }
+    }
+    float* dst = partial + (int64_t)blockIdx.x * 2 * channels;
+    if constexpr (kGroups == 1) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int c = (k * TPR + t) * V;
+            if (c >= channels) break;
+#pragma unroll
+            for (int e = 0; e < V; ++e) dst[c + e] = dw[k][e], dst[channels + c + e] = db[k][e];
+        }
+    } else {
+        for (int turn = 0; turn < kGroups; ++turn) {
+            if (group == turn) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        const int c = (k * TPR + t) * V + e;
+                        if (c < channels) {
+                            sums[c] = turn ? sums[c] + dw[k][e] : dw[k][e];
+                            sums[channels + c] = turn ? sums[channels + c] + db[k][e] : db[k][e];
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < 2 * channels; c += kNormThreads) dst[c] = sums[c];
+    }
+}
+
+// Rows too wide for the registers: the block's row of partial sums is its accumulator.
+template <class T>
+__global__ void __launch_bounds__(kNormThreads)
+layer_norm_grads_wide_kernel(int64_t rows, int channels, const T* __restrict__ feats, int64_t ld,
+                             const float* __restrict__ weights, const float* __restrict__ mean, const float* __restrict__ rstd,
+                             const T* __restrict__ grads, int64_t ld_g, T* __restrict__ out, float* __restrict__ partial) {
+    __shared__ float slots[kNormThreads / 32];
+    float* dw = partial + (int64_t)blockIdx.x * 2 * channels;
+    float* db = dw + channels;
+    for (int c = threadIdx.x; c < channels; c += kNormThreads) dw[c] = db[c] = 0.f;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const float mu = mean[row], r = rstd[row];
+        const T *x = feats + row * ld, *g = grads + row * ld_g;
+        float s1 = 0.f, s2 = 0.f;
+        for (int c = threadIdx.x; c < channels; c += kNormThreads) {
+            const float hat = (to_float(x[c]) - mu) * r, gr = to_float(g[c]);
+            dw[c] += gr * hat;  // a column belongs to one thread
+            db[c] += gr;
+            s1 += gr * weights[c];
+            s2 += gr * weights[c] * hat;
+        }
+        s1 = row_sum<kNormThreads>(s1, slots) / (float)channels;
+        s2 = row_sum<kNormThreads>(s2, slots) / (float)channels;
+        for (int c = threadIdx.x; c < channels; c += kNormThreads) {
+            const float hat = (to_float(x[c]) - mu) * r;
+            out[row * channels + c] = from_float<T>(r * (to_float(g[c]) * weights[c] - s1 - hat * s2));
+        }
+    }
+}
+
+// Column sums of the blocks' rows: 32 columns x 8 row strides per block, added in a fixed order.
+__global__ void __launch_bounds__(256)
+column_sums_kernel(int num_rows, int columns, const float* __restrict__ partial, int channels, float* __restrict__ weight_grads,
+                   float* __restrict__ bias_grads) {
+    __shared__ float part[8][33];
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    float sum = 0.f;
+    if (c < columns)
+        for (int r = slice; r < num_rows; r += 8) sum += partial[(int64_t)r * columns + c];
+    part[slice][lane] = sum;
+    __syncthreads();
+    if (slice == 0 && c < columns) {
+        for (int s = 1; s < 8; ++s) sum += part[s][lane];
+        if (c < channels) weight_grads[c] = sum;
+        else bias_grads[c - channels] = sum;
+    }
+}
+
+constexpr int kNormMaxBlocksPerSm = 4;
+
+static int norm_blocks(int64_t rows, int rows_per_block) {
+    const int64_t need = (rows + rows_per_block - 1) / rows_per_block, cap = (int64_t)sm_count() * kNormMaxBlocksPerSm;
+    return (int)(need < 1 ? 1 : need < cap ? need : cap);
+}
+
+// The vector width, threads per row and vectors per thread of a row: 16-byte vectors where every row starts on a 16-byte
+// boundary, single elements otherwise; as few threads per row as keep it to at most 8 vectors (16 single elements) each.
+template <class T, class Launch>
+static int dispatch_norm(int channels, bool vectors, const Launch& launch) {
+    constexpr int kV = 16 / sizeof(T);
+    if (vectors) {
+        const int n = channels / kV;
+        if (n <= 8) return launch.template run<T, kV, 8, 1>();
+        if (n <= 16) return launch.template run<T, kV, 8, 2>();
+        if (n <= 32) return launch.template run<T, kV, 32, 1>();
+        if (n <= 64) return launch.template run<T, kV, 32, 2>();
+        if (n <= 128) return launch.template run<T, kV, 32, 4>();
+        if (n <= 1024) return launch.template run<T, kV, 256, 4>();
+        return launch.template wide<T>();
+    }
+    if (channels <= 32) return launch.template run<T, 1, 8, 4>();
+    if (channels <= 128) return launch.template run<T, 1, 32, 4>();
+    if (channels <= 512) return launch.template run<T, 1, 32, 16>();
+    if (channels <= 1024) return launch.template run<T, 1, 256, 4>();
+    if (channels <= 4096) return launch.template run<T, 1, 256, 16>();
+    return launch.template wide<T>();
+}
+
+struct NormForward {
+    int64_t rows; int channels; const void* feats; int64_t ld; const float *weights, *bias; float eps;
+    void* out; float *mean, *rstd; cudaStream_t s;
+    template <class T, int V, int TPR, int K> int run() const {
+        const int64_t blocks = (rows + kNormThreads / TPR - 1) / (kNormThreads / TPR);
+        layer_norm_kernel<T, V, TPR, K><<<(unsigned)blocks, kNormThreads, 0, s>>>(rows, channels, (const T*)feats, ld, weights, bias,
+                                                                                 eps, (T*)out, mean, rstd);
+        PCCNN_LAUNCH_CHECK();
+        return PCCNN_OK;
+    }
+    template <class T> int wide() const {
+        layer_norm_wide_kernel<T><<<(unsigned)rows, kNormThreads, 0, s>>>(channels, (const T*)feats, ld, weights, bias, eps, (T*)out,
+                                                                         mean, rstd);
+        PCCNN_LAUNCH_CHECK();
+        return PCCNN_OK;
+    }
+};
+
+struct NormBackward {
+    int64_t rows; int channels; const void* feats; int64_t ld; const float *weights, *mean, *rstd; const void* grads;
+    int64_t ld_g; void* out; float *weight_grads, *bias_grads, *partial; cudaStream_t s;
+    int sums(int blocks) const {
+        column_sums_kernel<<<(2 * channels + 31) / 32, 256, 0, s>>>(blocks, 2 * channels, partial, channels, weight_grads, bias_grads);
+        PCCNN_LAUNCH_CHECK();
+        return PCCNN_OK;
+    }
+    template <class T, int V, int TPR, int K> int run() const {
+        const int blocks = norm_blocks(rows, kNormThreads / TPR);
+        layer_norm_grads_kernel<T, V, TPR, K><<<blocks, kNormThreads, TPR < kNormThreads ? (size_t)2 * channels * 4 : 0, s>>>(
+            rows, channels, (const T*)feats, ld, weights, mean, rstd, (const T*)grads, ld_g, (T*)out, partial);
+        PCCNN_LAUNCH_CHECK();
+        return sums(blocks);
+    }
+    template <class T> int wide() const {
+        const int blocks = norm_blocks(rows, 1);
+        layer_norm_grads_wide_kernel<T><<<blocks, kNormThreads, 0, s>>>(rows, channels, (const T*)feats, ld, weights, mean, rstd,
+                                                                       (const T*)grads, ld_g, (T*)out, partial);
+        PCCNN_LAUNCH_CHECK();
+        return sums(blocks);
+    }
+};
+
+}  // namespace pccnn
+
+using namespace pccnn;
+
+extern "C" {
+
+int pccnn_layer_norm(int64_t rows, int channels, const void* feats, int64_t ld_feats, int is_bf16, const float* weights,
+                     const float* bias, float eps, void* out, float* out_mean, float* out_rstd, void* stream) {
+    PCCNN_CHECK_ARG(rows >= 0 && rows < 0x7fffffffLL && channels > 0 && channels <= (1 << 20),
+                    "layer_norm: bad shape (%lld rows of %d channels)", (long long)rows, channels);
+    PCCNN_CHECK_ARG(ld_feats >= channels || rows <= 1, "layer_norm: row stride %lld below the %d channels", (long long)ld_feats, channels);
+    PCCNN_CHECK_ARG(eps >= 0.f, "layer_norm: eps must not be negative");
+    if (rows == 0) return PCCNN_OK;
+    PCCNN_CHECK_ARG(feats && weights && bias && out && out_mean && out_rstd, "layer_norm: null pointer");
+    const NormForward f{rows, channels, feats, ld_feats, weights, bias, eps, out, out_mean, out_rstd, (cudaStream_t)stream};
+    const int v = is_bf16 ? 8 : 4;
+    const bool vec = channels % v == 0 && ld_feats % v == 0 && aligned16(feats) && aligned16(weights) && aligned16(bias) && aligned16(out);
+    return is_bf16 ? dispatch_norm<__nv_bfloat16>(channels, vec, f) : dispatch_norm<float>(channels, vec, f);
+}
+
+size_t pccnn_layer_norm_grads_workspace_bytes(int64_t rows, int channels) {
+    if (rows < 0 || channels <= 0) return 256;
+    const int64_t cap = (int64_t)sm_count() * kNormMaxBlocksPerSm, blocks = rows < cap ? (rows > 0 ? rows : 1) : cap;
+    return align_up((size_t)blocks * 2 * channels * 4);
+}
+
+int pccnn_layer_norm_grads(int64_t rows, int channels, const void* feats, int64_t ld_feats, int is_bf16, const float* weights,
+                           const float* mean, const float* rstd, const void* in_grads, int64_t ld_grads, void* out_feat_grads,
+                           float* out_weight_grads, float* out_bias_grads, void* workspace, size_t workspace_bytes, void* stream) {
+    PCCNN_CHECK_ARG(rows >= 0 && rows < 0x7fffffffLL && channels > 0 && channels <= (1 << 20),
+                    "layer_norm_grads: bad shape (%lld rows of %d channels)", (long long)rows, channels);
+    PCCNN_CHECK_ARG((ld_feats >= channels && ld_grads >= channels) || rows <= 1, "layer_norm_grads: row strides below the %d channels",
+                    channels);
+    PCCNN_CHECK_ARG(out_weight_grads && out_bias_grads, "layer_norm_grads: null pointer");
+    cudaStream_t s = (cudaStream_t)stream;
+    if (rows == 0) {
+        PCCNN_CUDA(cudaMemsetAsync(out_weight_grads, 0, (size_t)channels * 4, s));
+        PCCNN_CUDA(cudaMemsetAsync(out_bias_grads, 0, (size_t)channels * 4, s));
+        return PCCNN_OK;
+    }
+    PCCNN_CHECK_ARG(feats && weights && mean && rstd && in_grads && out_feat_grads, "layer_norm_grads: null pointer");
+    if (!workspace || workspace_bytes < pccnn_layer_norm_grads_workspace_bytes(rows, channels)) {
+        set_error("layer_norm_grads: workspace of %zu bytes, need %zu", workspace_bytes,
+                  pccnn_layer_norm_grads_workspace_bytes(rows, channels));
+        return PCCNN_ERR_WORKSPACE;
+    }
+    const NormBackward b{rows, channels, feats, ld_feats, weights, mean, rstd, in_grads, ld_grads, out_feat_grads,
+                         out_weight_grads, out_bias_grads, (float*)workspace, s};
+    const int v = is_bf16 ? 8 : 4;
+    const bool vec = channels % v == 0 && ld_feats % v == 0 && ld_grads % v == 0 && aligned16(feats) && aligned16(weights) &&
+                     aligned16(in_grads) && aligned16(out_feat_grads);
+    return is_bf16 ? dispatch_norm<__nv_bfloat16>(channels, vec, b) : dispatch_norm<float>(channels, vec, b);
+}
+
+}  // extern "C"

@@ -11,3 +11,6 @@ from .compute_kpconv import ComputeKPConv, ComputeKPConvWeightVar
 from .compute_kpconvn import ComputeKPConvN, ComputeKPConvNWeightVar
 from .compute_sphconv import ComputeSPHConv, ComputeSPHConvWeightVar
 from .compute_pccnn import ComputePCCNN, ComputePCCNNWeightVar
+from .compute_layer_norm import ComputeLayerNorm
+from .compute_rotary_positions import ComputeRotaryPositions
+from .compute_cross_attention import ComputeCrossAttention

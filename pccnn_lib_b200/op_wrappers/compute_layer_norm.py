@@ -1,0 +1,19 @@
+import torch
+
+from .. import ops
+
+
+class ComputeLayerNorm(torch.autograd.Function):
+    """Layer norm over the channels with gradients for features, weights and bias (no counterpart in the reference)."""
+
+    @staticmethod
+    def forward(ctx, p_features, p_weights, p_bias, p_eps=1e-5):
+        out, mean, rstd = ops.layer_norm(p_features, p_weights, p_bias, p_eps)
+        ctx.save_for_backward(p_features, p_weights, mean, rstd)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, p_grads):
+        feat_grads, weight_grads, bias_grads = ops.layer_norm_grads(*ctx.saved_tensors, p_grads)
+        return feat_grads, weight_grads, bias_grads, None

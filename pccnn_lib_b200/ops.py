@@ -957,3 +957,200 @@ def point_conv_weight_var(basis, feats, neighbors, start_ids):
                                                      _p(start_ids), out.data_ptr(), ws.data_ptr(), ws.numel(), _stream()),
                     "point_conv_weight_var")
     return out
+
+
+# ---- attention between packed clouds -----------------------------------------------------------
+# No counterpart in the reference.  Features are float32 or bfloat16, [rows, channels] or [rows, heads, size]; rows of a
+# batch of clouds are packed, cloud b owns the rows [ends[b-1], ends[b]).
+_FEATURE_TYPES = (torch.float32, torch.bfloat16)
+
+
+def _feature_rows(t, name, ndim, dtype=None):
+    """A feature tensor whose last dimension is contiguous and whose other strides the kernels take as they are: views of
+    a wider tensor are read in place, anything else (transposed, expanded) is copied."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch.Tensor" % name)
+    if not t.is_cuda:
+        raise RuntimeError("%s must be a CUDA tensor (pccnn_lib_b200 has no CPU path)" % name)
+    if t.dtype not in (_FEATURE_TYPES if dtype is None else (dtype,)):
+        raise RuntimeError("%s must have dtype %s, got %s" % (name, " or ".join(str(d) for d in _FEATURE_TYPES) if dtype is None
+                                                              else dtype, t.dtype))
+    if t.dim() != ndim:
+        raise RuntimeError("%s must have %d dimensions, got %d" % (name, ndim, t.dim()))
+    if t.is_contiguous():
+        return t
+    in_place = t.stride(-1) == 1 and all(t.stride(i) >= t.shape[-1] for i in range(ndim - 1))
+    return t if in_place else t.contiguous()
+
+
+def _same_device(**tensors):
+    devices = {t.device for t in tensors.values()}
+    if len(devices) > 1:
+        raise RuntimeError("%s must be on one device, got %s" % (", ".join(tensors), sorted(str(d) for d in devices)))
+
+
+def _head_strides(t):
+    return (ctypes.c_int64 * 2)(t.stride(0), t.stride(1))
+
+
+def layer_norm(features, weights, bias, eps=1e-5):
+    """Layer norm over the channels -> [out [N, C], mean [N], rstd [N]]; weights and bias [C] and the statistics are float32."""
+    features = _feature_rows(features, "features", 2)
+    weights = _need(weights, "weights", torch.float32, 1)
+    bias = _need(bias, "bias", torch.float32, 1)
+    _same_device(features=features, weights=weights, bias=bias)
+    n, c = features.shape
+    if c == 0 or weights.shape[0] != c or bias.shape[0] != c:
+        raise RuntimeError("weights and bias must have one entry for each of the %d (at least one) channels" % c)
+    out = torch.empty((n, c), dtype=features.dtype, device=features.device)
+    stats = torch.empty((2, n), dtype=torch.float32, device=features.device)
+    mean, rstd = stats[0], stats[1]
+    with _on(features.device):
+        _capi.check(_lib.pccnn_layer_norm(n, c, _p(features), features.stride(0), features.dtype == torch.bfloat16, _p(weights),
+                                          _p(bias), float(eps), _p(out), _p(mean), _p(rstd), _stream()), "layer_norm")
+    return [out, mean, rstd]
+
+
+def layer_norm_grads(features, weights, mean, rstd, in_grads):
+    """[dFeatures [N, C], dWeights [C], dBias [C]] of layer_norm; the sums over the rows are float32, in a fixed order."""
+    features = _feature_rows(features, "features", 2)
+    in_grads = _feature_rows(in_grads, "in_grads", 2, features.dtype)
+    weights = _need(weights, "weights", torch.float32, 1)
+    mean, rstd = _need(mean, "mean", torch.float32, 1), _need(rstd, "rstd", torch.float32, 1)
+    _same_device(features=features, weights=weights, mean=mean, rstd=rstd, in_grads=in_grads)
+    n, c = features.shape
+    if c == 0 or weights.shape[0] != c or mean.shape[0] != n or rstd.shape[0] != n or tuple(in_grads.shape) != (n, c):
+        raise RuntimeError("layer_norm_grads: weights [C], mean and rstd [N] and in_grads [N, C] must match features [N, C]")
+    d_f = torch.empty((n, c), dtype=features.dtype, device=features.device)
+    d_w, d_b = (torch.empty((c,), dtype=torch.float32, device=features.device) for _ in range(2))
+    with _on(features.device):
+        ws = _workspace(_lib.pccnn_layer_norm_grads_workspace_bytes(n, c), features.device)
+        _capi.check(_lib.pccnn_layer_norm_grads(n, c, _p(features), features.stride(0), features.dtype == torch.bfloat16,
+                                                _p(weights), _p(mean), _p(rstd), _p(in_grads), in_grads.stride(0), _p(d_f), _p(d_w),
+                                                _p(d_b), ws.data_ptr(), ws.numel(), _stream()), "layer_norm_grads")
+    return [d_f, d_w, d_b]
+
+
+def _rotary_args(features, pts, frequencies, axis_pairs):
+    features = _feature_rows(features, "features", 3)
+    pts = _need(pts, "pts", torch.float32, 2)
+    frequencies = _need(frequencies, "frequencies", torch.float32, 1)
+    _same_device(features=features, pts=pts, frequencies=frequencies)
+    pairs = [int(p) for p in axis_pairs]
+    if pts.shape[0] != features.shape[0] or pts.shape[1] != len(pairs):
+        raise RuntimeError("pts must be [%d, %d]: a coordinate of every row for each entry of axis_pairs"
+                           % (features.shape[0], len(pairs)))
+    if min(pairs, default=0) < 0 or sum(pairs) != frequencies.shape[0] or 2 * sum(pairs) > features.shape[2]:
+        raise RuntimeError("axis_pairs %s must add up to the %d frequencies and to at most half the head size %d"
+                           % (pairs, frequencies.shape[0], features.shape[2]))
+    return features, pts, frequencies, (ctypes.c_int32 * max(len(pairs), 1))(*pairs), len(pairs)
+
+
+def rotary_positions(features, pts, frequencies, axis_pairs):
+    """Turns neighboring features (2j, 2j + 1) of every head of features [N, H, D] by pts[n, a] * frequencies[j] radians;
+    axis_pairs[a] pairs, in order, belong to the axis a of pts [N, A]; features behind the last pair pass unchanged."""
+    features, pts, frequencies, pairs, axes = _rotary_args(features, pts, frequencies, axis_pairs)
+    n, h, d = features.shape
+    out = torch.empty((n, h, d), dtype=features.dtype, device=features.device)
+    with _on(features.device):
+        _capi.check(_lib.pccnn_rotary_positions(n, h, d, _p(features), features.stride(0), features.stride(1),
+                                                features.dtype == torch.bfloat16, axes, _p(pts), _p(frequencies), pairs, _p(out),
+                                                _stream()), "rotary_positions")
+    return out
+
+
+def rotary_positions_grads(features, pts, frequencies, axis_pairs, in_grads, with_pts=True):
+    """[dFeatures [N, H, D], dPts [N, A] (None where with_pts is false)] of rotary_positions."""
+    features, pts, frequencies, pairs, axes = _rotary_args(features, pts, frequencies, axis_pairs)
+    in_grads = _feature_rows(in_grads, "in_grads", 3, features.dtype)
+    _same_device(features=features, in_grads=in_grads)
+    n, h, d = features.shape
+    if tuple(in_grads.shape) != (n, h, d):
+        raise RuntimeError("in_grads must be [N, H, D] as features")
+    d_f = torch.empty((n, h, d), dtype=features.dtype, device=features.device)
+    d_p = torch.empty_like(pts) if with_pts else None
+    with _on(features.device):
+        _capi.check(_lib.pccnn_rotary_positions_grads(n, h, d, _p(features), features.stride(0), features.stride(1),
+                                                      features.dtype == torch.bfloat16, axes, _p(pts), _p(frequencies), pairs,
+                                                      _p(in_grads), in_grads.stride(0), in_grads.stride(1), _p(d_f), _p(d_p),
+                                                      _stream()), "rotary_positions_grads")
+    return [d_f, d_p]
+
+
+def _attention_args(queries, keys, values, query_ends, key_ends, scale):
+    queries = _feature_rows(queries, "queries", 3)
+    keys = _feature_rows(keys, "keys", 3, queries.dtype)
+    values = _feature_rows(values, "values", 3, queries.dtype)
+    query_ends = _need(query_ends, "query_ends", torch.int32, 1)
+    key_ends = _need(key_ends, "key_ends", torch.int32, 1)
+    _same_device(queries=queries, keys=keys, values=values, query_ends=query_ends, key_ends=key_ends)
+    m, h, d = queries.shape
+    if keys.shape != values.shape or keys.shape[2] != d:
+        raise RuntimeError("keys and values must be [N, Hkv, %d]" % d)
+    if keys.shape[1] == 0 or h == 0 or h % keys.shape[1]:
+        raise RuntimeError("%d query heads cannot share %d key heads" % (h, keys.shape[1]))
+    if query_ends.shape != key_ends.shape:
+        raise RuntimeError("query_ends and key_ends must have one entry per cloud each")
+    if d == 0 or d > 256:
+        raise RuntimeError("head size %d outside [1, 256]" % d)
+    scale = 1.0 / d ** 0.5 if scale is None else float(scale)
+    if os.environ.get("PCCNN_VALIDATE_NEIGHBORS", "0") == "1" and not torch.cuda.is_current_stream_capturing():
+        validate_ends(query_ends, m, "query_ends")
+        validate_ends(key_ends, keys.shape[0], "key_ends")
+    shape = (m, keys.shape[0], query_ends.shape[0], h, keys.shape[1], d, int(queries.dtype == torch.bfloat16))
+    inputs = (_p(queries), _head_strides(queries), _p(keys), _head_strides(keys), _p(values), _head_strides(values), _p(query_ends),
+              _p(key_ends), scale)
+    return (queries, keys, values, query_ends, key_ends), shape, inputs
+
+
+def validate_ends(ends, num_rows, name="ends"):
+    """Raises RuntimeError where the end offsets of packed clouds decrease or leave [0, num_rows].  Synchronises.  Runs in
+    front of cross_attention and cross_attention_grads (outside of a graph's capture) when the environment variable
+    PCCNN_VALIDATE_NEIGHBORS is set to 1."""
+    ends = _need(ends, "ends", torch.int32, 1)
+    host = ends.tolist()
+    for b, e in enumerate(host):
+        if e < (host[b - 1] if b else 0):
+            raise RuntimeError("%s: end offsets decrease (at cloud %d, value %d)" % (name, b, e))
+        if e > num_rows:
+            raise RuntimeError("%s: end offset beyond the %d rows (at cloud %d, value %d)" % (name, num_rows, b, e))
+
+
+def cross_attention(queries, keys, values, query_ends, key_ends, scale=None):
+    """Attention of every cloud's queries to the same cloud's keys -> [out [M, H, D], lse [H, M] float32].
+
+    queries [M, H, D], keys and values [N, Hkv, D] with H a multiple of Hkv (query head h reads key head h // (H // Hkv));
+    query_ends and key_ends [B] int32 are the clouds' end offsets in the packed rows; out = softmax(scale q k^T) v, scale
+    defaults to 1 / sqrt(D).  A query without keys (an empty cloud, a row behind the last cloud) gets zeros and an lse of
+    minus infinity.  Head sizes up to 256."""
+    keep, shape, inputs = _attention_args(queries, keys, values, query_ends, key_ends, scale)
+    m, n, _, h, _, d, _ = shape
+    out = torch.empty((m, h, d), dtype=queries.dtype, device=queries.device)
+    lse = torch.empty((h, m), dtype=torch.float32, device=queries.device)
+    with _on(queries.device):
+        ws = _workspace(_lib.pccnn_cross_attention_workspace_bytes(*shape), queries.device)
+        _capi.check(_lib.pccnn_cross_attention(*shape, *inputs, _p(out), _p(lse), ws.data_ptr(), ws.numel(), _stream()),
+                    "cross_attention")
+    return [out, lse]
+
+
+def cross_attention_grads(queries, keys, values, query_ends, key_ends, out, lse, in_grads, scale=None):
+    """[dQueries [M, H, D], dKeys [N, Hkv, D], dValues [N, Hkv, D]] of cross_attention from its outputs `out` and `lse`.
+    Heads that share keys are added up; every sum is taken in a fixed order."""
+    keep, shape, inputs = _attention_args(queries, keys, values, query_ends, key_ends, scale)
+    queries, keys = keep[0], keep[1]
+    in_grads = _feature_rows(in_grads, "in_grads", 3, queries.dtype)
+    out = _need(out, "out", queries.dtype, 3)
+    lse = _need(lse, "lse", torch.float32, 2)
+    _same_device(queries=queries, out=out, lse=lse, in_grads=in_grads)
+    m, n, _, h, _, d, _ = shape
+    if tuple(in_grads.shape) != (m, h, d) or tuple(out.shape) != (m, h, d) or tuple(lse.shape) != (h, m):
+        raise RuntimeError("out and in_grads must be [M, H, D] as queries and lse [H, M]")
+    d_q = torch.empty((m, h, d), dtype=queries.dtype, device=queries.device)
+    d_k, d_v = (torch.empty(tuple(keys.shape), dtype=queries.dtype, device=queries.device) for _ in range(2))
+    with _on(queries.device):
+        ws = _workspace(_lib.pccnn_cross_attention_grads_workspace_bytes(*shape), queries.device)
+        _capi.check(_lib.pccnn_cross_attention_grads(*shape, *inputs, _p(out), _p(lse), _p(in_grads), _head_strides(in_grads),
+                                                     _p(d_q), _p(d_k), _p(d_v), ws.data_ptr(), ws.numel(), _stream()),
+                    "cross_attention_grads")
+    return [d_q, d_k, d_v]

@@ -37,6 +37,16 @@ class Pointcloud(object):
         with torch.no_grad():
             return torch.bincount(self.batch_ids_.to(torch.int64), minlength=self.batch_size_host()).to(torch.int32)
 
+    def get_batch_ends(self, p_batch_size=None):
+        """End offset of every cloud in the packed rows, int32 [batch size] (p_batch_size: at least that many, the further
+        ones empty); the rows have to be grouped by ascending batch id, which is checked (one host synchronisation)."""
+        with torch.no_grad():
+            ids = self.batch_ids_.to(torch.int64)
+            if ids.numel() > 1 and bool((ids[1:] < ids[:-1]).any()):
+                raise RuntimeError("the points are not grouped by ascending batch id")
+            size = self.batch_size_host() if p_batch_size is None else max(int(p_batch_size), self.batch_size_host())
+            return torch.cumsum(torch.bincount(ids, minlength=size), 0).to(torch.int32)
+
     def compute_pdf(self, p_badnwidth):
         """KDE of every point with the given per-axis bandwidth; neighbors are searched within
         4 bandwidths and capped at 300 per point (pccnn_lib/pc/Pointcloud.py:81-109)."""
