@@ -12,13 +12,13 @@
 #include "attention.cuh"
 #include "common.cuh"
 #include "features.cuh"
+#include "status.cuh"
 
 namespace pccnn {
 
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kMaxHeadSize = 256;
-constexpr int kMaxSplits = 64;
 
 // ---- layout of a block: LPK lanes of a warp share a streamed row (V elements each, NC times), 32 / LPK rows per warp ----
 template <class T, int V, int NC>
@@ -466,6 +466,14 @@ static int key_grad_splits(const AttentionCall& a) {
     return choose_splits(a.num_keys * a.kv_heads, mean_rows(a.num_queries, a.clouds));
 }
 
+int join_splits(const AttentionCall& a, int splits, const float* part, const float2* stat, void* out, float* lse, cudaStream_t s) {
+    const unsigned blocks = (unsigned)((a.num_queries * a.heads + 7) / 8);
+    if (a.is_bf16) attention_join_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(a.num_queries, a.heads, a.size, splits, part, stat, (__nv_bfloat16*)out, lse);
+    else attention_join_kernel<float><<<blocks, 256, 0, s>>>(a.num_queries, a.heads, a.size, splits, part, stat, (float*)out, lse);
+    PCCNN_LAUNCH_CHECK();
+    return PCCNN_OK;
+}
+
 template <class T, int V, int NC>
 static int launch_rows(const AttentionCall& a, const RowLayout& l, void* out, float* lse, char* ws, cudaStream_t s) {
     const int splits = forward_splits(a);
@@ -475,12 +483,7 @@ static int launch_rows(const AttentionCall& a, const RowLayout& l, void* out, fl
     if (a.heads > a.kv_heads) attention_row_kernel<T, V, NC, 4><<<grid, kRowThreads, 0, s>>>(a, l.lanes, splits, (T*)out, lse, part, stat);
     else attention_row_kernel<T, V, NC, 1><<<grid, kRowThreads, 0, s>>>(a, l.lanes, splits, (T*)out, lse, part, stat);
     PCCNN_LAUNCH_CHECK();
-    if (splits > 1) {
-        attention_join_kernel<T><<<(unsigned)((a.num_queries * a.heads + 7) / 8), 256, 0, s>>>(a.num_queries, a.heads, a.size, splits, part,
-                                                                                             stat, (T*)out, lse);
-        PCCNN_LAUNCH_CHECK();
-    }
-    return PCCNN_OK;
+    return splits > 1 ? join_splits(a, splits, part, stat, out, lse, s) : PCCNN_OK;
 }
 
 template <class T>
@@ -567,9 +570,9 @@ size_t pccnn_cross_attention_workspace_bytes(int64_t num_queries, int64_t num_ke
     const AttentionCall a = describe(num_queries, num_keys, clouds, heads, kv_heads, size, is_bf16, nullptr, nullptr, nullptr, nullptr,
                                      nullptr, nullptr, nullptr, nullptr, 1.f);
     const int splits = forward_splits(a);
-    if (splits == 1) return 256;
-    const size_t rows = (size_t)splits * num_queries * heads;
-    return align_up(rows * sizeof(float2)) + align_up(rows * size * 4);
+    const size_t rows = splits > 1 ? (size_t)splits * num_queries * heads : 0;
+    const size_t by_rows = align_up(rows * sizeof(float2)) + align_up(rows * size * 4) + 256, by_tiles = tc_shape(a) ? tc_forward_workspace(a) : 0;
+    return by_rows > by_tiles ? by_rows : by_tiles;
 }
 
 int pccnn_cross_attention(int64_t num_queries, int64_t num_keys, int clouds, int heads, int kv_heads, int size, int is_bf16,
@@ -587,6 +590,8 @@ int pccnn_cross_attention(int64_t num_queries, int64_t num_keys, int clouds, int
         set_error("cross_attention: workspace of %zu bytes, need %zu", workspace_bytes, need);
         return PCCNN_ERR_WORKSPACE;
     }
+    if (int rc = take_sticky_status("cross_attention")) return rc;  // an earlier call's tensor-core kernel gave up
+    if (num_keys > 0 && tc_shape(a) && tc_layout(a, nullptr) && aligned16(out)) return tc_forward(a, out, out_lse, (char*)workspace, (cudaStream_t)stream);
     const ForwardRows f{a, row_layout(a, nullptr), out, out_lse, (char*)workspace, (cudaStream_t)stream};
     return is_bf16 ? dispatch_rows<__nv_bfloat16>(f.l, f) : dispatch_rows<float>(f.l, f);
 }

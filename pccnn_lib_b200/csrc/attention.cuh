@@ -21,6 +21,18 @@ struct AttentionCall {
     float scale;
 };
 
+constexpr int kMaxSplits = 64;
+
+// Tensor-core kernels (attention_tc.cu).  Whether a call may use them goes by its shape (tc_shape: the workspace does not
+// depend on anything else) and then by the layout of its tensors (tc_layout).
+bool tc_shape(const AttentionCall& a);
+bool tc_layout(const AttentionCall& a, const HeadRows* grads);
+size_t tc_forward_workspace(const AttentionCall& a);
+int tc_forward(const AttentionCall& a, void* out, float* lse, char* ws, cudaStream_t s);
+
+// Joins the splits of every query: part_out [splits, queries, heads, size] relative to part_stat's (maximum in log2 units, sum).
+int join_splits(const AttentionCall& a, int splits, const float* part_out, const float2* part_stat, void* out, float* lse, cudaStream_t s);
+
 #ifdef __CUDACC__
 
 constexpr float kLog2e = 1.4426950408889634f;

@@ -1,0 +1,565 @@
+// Tensor-core kernels of cross attention on packed clouds (tcgen05, sm_100a).
+//
+// Operands are bf16 tiles of `rows x 64 features` in shared memory (128-byte swizzle, one block per 64 features), brought in
+// by TMA.  32-bit features come as three bf16 planes, x = h + m + l with h = bf16(x), m = bf16(x - h), l = bf16(x - h - m):
+// 24 bits, and a product is the six plane products h h + h m + m h + m m + h l + l h in one fp32 accumulator (the dropped
+// ones are below 2^-24 of it).
+//
+// A tile that ends inside a cloud is not loaded by TMA but row by row, with zeros behind the cloud's last row: the rows that
+// follow belong to another cloud and may hold infinities, which would reach this one as 0 * inf.
+//
+// Roles of the ten warps of a CTA: two groups of four warps do the element-wise work (one row of a 128-row tile per thread,
+// which is one lane of tensor memory), warp 8 loads, one thread of warp 9 issues the products.  The element-wise groups work
+// on different units in turn, so one of them computes while the tensor cores run the products of the other.
+// Every wait is bounded: a role whose wait runs out sets a flag that ends the other roles' waits, the CTA waits for its
+// copies and products in flight, frees its tensor memory and records the failure in the pinned status word.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "attention.cuh"
+#include "common.cuh"
+#include "features.cuh"
+#include "tc_ptx.cuh"
+
+namespace pccnn {
+
+constexpr int kTcThreads = 320;
+constexpr int kTcRows = 128;  // rows of the tile whose products have them as the M dimension
+constexpr int kTcMaxStages = 8;
+
+// bf16 rows [planes][rows, heads, size] for the loads that TMA does not do.
+struct TcRows {
+    const __nv_bfloat16* data;
+    int64_t row, head, plane;
+};
+
+struct TcControl {
+    uint32_t poll_limit;
+    int withhold_from;  // test hook: the loader stops in front of this streamed tile (-1: off)
+    int* sticky;        // pinned status word
+    int status;         // value to record: origin in the upper bits
+};
+
+struct TcShared {
+    uint64_t fixed_full, full[kTcMaxStages], empty[kTcMaxStages], s_full[2], e_ready[2], all_done, drained;
+    uint32_t tmem;
+    int failed;
+};
+
+// Bounded wait that also ends when another role of the CTA has failed.
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, uint32_t limit, volatile int* failed) {
+    for (uint32_t left = limit; left > 0;) {
+        const uint32_t now = left < 1024 ? left : 1024;
+        if (mbar_wait(bar, parity, now)) return true;
+        if (*failed) return false;
+        left -= now;
+    }
+    return false;
+}
+// The same for a whole warp, with one answer for all its lanes.
+__device__ __forceinline__ bool tc_wait_warp(uint64_t* bar, uint32_t parity, uint32_t limit, volatile int* failed) {
+    return __all_sync(kFullMask, tc_wait(bar, parity, limit, failed));
+}
+
+// The cloud of block `slot` of a grid with rows / ROWS + clouds + 1 blocks: cloud b's blocks start at
+// begin(b) / ROWS + b, which leaves room for all of them without a prefix sum.  Cloud `clouds` is the rest of the rows.
+// All lanes of a warp search together.  Returns false for a block without rows.
+template <int ROWS>
+__device__ __forceinline__ bool tc_block_rows(const int32_t* __restrict__ ends, int clouds, int64_t n, int64_t slot, int& cloud,
+                                              int64_t& row0, int64_t& row_end) {
+    int lo = 0, hi = clouds + 1;  // the answer lies in [lo, hi)
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, b = lo + (int)(threadIdx.x & 31) * step;
+        const bool before = b < hi && cloud_begin(ends, b, n) / ROWS + b <= slot;
+        const int count = __popc(__ballot_sync(kFullMask, before));  // lane 0's is always true for a valid range
+        const int at = lo + (count > 0 ? count - 1 : 0) * step;
+        hi = min(hi, at + step);
+        lo = at;
+    }
+    cloud = lo;
+    const int64_t begin = cloud_begin(ends, lo, n);
+    row_end = cloud_end(ends, lo, clouds, n);
+    row0 = begin + (slot - (begin / ROWS + lo)) * ROWS;
+    return row0 >= begin && row0 < row_end;
+}
+
+// ---- loads ------------------------------------------------------------------------------------------------------
+// R rows from row0 of `head` into the tile at dst ([plane][64 features][R rows]); `valid` of them belong to the cloud.
+// Called by a whole warp; completes one phase of `bar`.
+template <int R, int NP, int GR>
+__device__ __forceinline__ void tc_load_tile(uint8_t* dst, const CUtensorMap* map, const TcRows& src, int64_t plane_rows, int head,
+                                             int64_t row0, int valid, int size, uint64_t* bar) {
+    const int lane = threadIdx.x & 31;
+    if (valid >= R) {
+        if (lane == 0) {
+            mbar_expect_tx(bar, NP * GR * R * 128);
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+#pragma unroll
+                for (int g = 0; g < GR; ++g)
+                    tma_load_3d(dst + (p * GR + g) * R * 128, map, bar, g * 64, head, (int)(p * plane_rows + row0));
+        }
+    } else {
+        const int chunks = size >> 3;
+#pragma unroll 1
+        for (int pg = 0; pg < NP * GR; ++pg) {
+            const int p = pg / GR, g = pg % GR;
+            const __nv_bfloat16* from = src.data + p * src.plane + row0 * src.row + head * src.head + g * 64;
+#pragma unroll 8
+            for (int i = lane; i < R * 8; i += 32) {
+                const int r = i >> 3, c = i & 7;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (r < valid && g * 8 + c < chunks) v = *reinterpret_cast<const uint4*>(from + r * src.row + c * 8);
+                *reinterpret_cast<uint4*>(dst + pg * R * 128 + sw128_offset(r, c)) = v;
+            }
+        }
+        fence_smem_to_async_proxy();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+    }
+    __syncwarp();
+}
+
+// ---- products (one thread) ----------------------------------------------------------------------------------------
+// The plane pairs of a product, smallest first; one pair (0, 0) for bf16 features.
+template <int NP> struct TcPairs;
+template <> struct TcPairs<1> {
+    static constexpr int kCount = 1;
+    __device__ static constexpr int a(int) { return 0; }
+    __device__ static constexpr int b(int) { return 0; }
+};
+template <> struct TcPairs<3> {
+    static constexpr int kCount = 6;
+    __device__ static constexpr int a(int i) { return i == 0 ? 1 : i == 1 ? 2 : i == 2 ? 0 : i == 3 ? 1 : 0; }
+    __device__ static constexpr int b(int i) { return i == 0 ? 1 : i == 1 ? 0 : i == 2 ? 2 : i == 3 ? 0 : i == 4 ? 1 : 0; }
+};
+
+// fp32 accumulate, bf16 x bf16, M = 128, N = n; b_mn: B's rows in memory are the K dimension.
+__device__ __forceinline__ uint32_t tc_idesc(int n, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTcRows >> 4) << 24);
+}
+
+// D[128, RB] = A[128, features] B[RB, features]^T, both tiles in shared memory.
+template <int NP, int GR, int RB>
+__device__ __forceinline__ void tc_rows_by_rows(uint32_t d, uint32_t a, uint32_t b, int steps) {
+    const uint32_t idesc = tc_idesc(RB, false);
+#pragma unroll
+    for (int i = 0; i < TcPairs<NP>::kCount; ++i) {
+        const uint32_t pa = a + TcPairs<NP>::a(i) * GR * kTcRows * 128, pb = b + TcPairs<NP>::b(i) * GR * RB * 128;
+#pragma unroll 1
+        for (int k = 0; k < steps; ++k)  // 16 features = 32 bytes further inside the swizzled row
+            tc_mma_bf16(d, umma_desc_k_sw128(pa + (k >> 2) * kTcRows * 128) + 2 * (k & 3),
+                        umma_desc_k_sw128(pb + (k >> 2) * RB * 128) + 2 * (k & 3), idesc, (i > 0 || k > 0) ? 1u : 0u);
+    }
+}
+
+// D[128, n] (+)= E[128, RB] B[RB, n]: E in tensor memory (planes of RB / 2 columns), B's tile in shared memory; `steps` blocks
+// of 16 rows of B.
+template <int NP, int GR, int RB>
+__device__ __forceinline__ void tc_weights_by_rows(uint32_t d, uint32_t e, uint32_t b, int n, int steps, bool accumulate) {
+    const uint32_t idesc = tc_idesc(n, true);
+#pragma unroll
+    for (int i = 0; i < TcPairs<NP>::kCount; ++i) {
+        const uint32_t pe = e + TcPairs<NP>::a(i) * (RB / 2), pb = b + TcPairs<NP>::b(i) * GR * RB * 128;
+#pragma unroll 1
+        for (int k = 0; k < steps; ++k)
+            tc_mma_bf16_ts(d, pe + k * 8, umma_desc_mn_sw128(pb + k * 2048, RB * 128), idesc, (accumulate || i > 0 || k > 0) ? 1u : 0u);
+    }
+}
+
+// ---- element-wise ------------------------------------------------------------------------------------------------
+// 32 values of this thread's row as bf16 planes into tensor memory, 16 columns of each plane.
+template <int NP, int PLANE_COLS>
+__device__ __forceinline__ void tc_store_weights(uint32_t dst, const float (&p)[32]) {
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = pack_bf16(p[2 * i], p[2 * i + 1]);
+    tc_st_32x16(dst, w);
+    if constexpr (NP == 3) {
+        float r[32];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            r[2 * i] = p[2 * i] - __uint_as_float(w[i] << 16);
+            r[2 * i + 1] = p[2 * i + 1] - __uint_as_float(w[i] & 0xffff0000u);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = pack_bf16(r[2 * i], r[2 * i + 1]);
+        tc_st_32x16(dst + PLANE_COLS, w);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            w[i] = pack_bf16(r[2 * i] - __uint_as_float(w[i] << 16), r[2 * i + 1] - __uint_as_float(w[i] & 0xffff0000u));
+        tc_st_32x16(dst + 2 * PLANE_COLS, w);
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void tc_write16(T* __restrict__ dst, int c, int size, const float (&x)[16]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if (c + 8 * h >= size) break;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = x[8 * h + i];
+        store_vec<T, 8>(dst + c + 8 * h, v);
+    }
+}
+
+// ---- set-up and teardown -----------------------------------------------------------------------------------------
+template <int COLUMNS>
+__device__ __forceinline__ uint32_t tc_begin(TcShared* sh, int stages) {
+    if (threadIdx.x == 0) {
+        mbar_init(&sh->fixed_full, 1);
+        for (int i = 0; i < stages; ++i) {
+            mbar_init(&sh->full[i], 1);
+            mbar_init(&sh->empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh->s_full[i], 1);
+            mbar_init(&sh->e_ready[i], 128);
+        }
+        mbar_init(&sh->all_done, 1);
+        mbar_init(&sh->drained, 1);
+        sh->failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (threadIdx.x < 32) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem)), "r"(COLUMNS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    return sh->tmem;
+}
+template <int COLUMNS>
+__device__ __forceinline__ void tc_end(uint32_t tmem) {
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x < 32)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(COLUMNS) : "memory");
+}
+__device__ __forceinline__ void tc_fail(TcShared* sh, const TcControl& ctl, int code) {
+    *(volatile int*)&sh->failed = 1;
+    atomicCAS_system(ctl.sticky, 0, ctl.status | code);
+}
+// After a failure: copies that nobody has waited for must land before the CTA retires.
+__device__ __forceinline__ void tc_drain_loads(TcShared* sh, int issued, int stages, uint32_t limit) {
+    mbar_wait(&sh->fixed_full, 0, limit);
+    for (int i = issued > stages ? issued - stages : 0; i < issued; ++i) mbar_wait(&sh->full[i % stages], (i / stages) & 1, limit);
+}
+
+// ---- forward ------------------------------------------------------------------------------------------------------
+// Block = up to QT x 128 queries of one cloud and head x one split of the keys.  Units: with two query tiles unit u is
+// (keys u / 2, tile u % 2); with one, unit u is key tile u, and the two element-wise groups take every other one, each with an
+// accumulator, running maximum and sum of its own that are joined at the end.
+// The accumulator is scaled only when the maximum has grown by more than 2^8 since it was last scaled: the probabilities
+// stay below 2^8, and the final division is by a sum relative to the same reference.
+template <int GR, int BN, int NP, int QT>
+struct TcForward {
+    static constexpr int kQ = QT * NP * GR * kTcRows * 128;
+    static constexpr int kSlot = NP * GR * BN * 128;
+    static constexpr int kFit = (200 * 1024 - kQ) / kSlot;
+    static constexpr int kStages = kFit > 6 ? 6 : kFit;
+    static constexpr int kBuffer = NP == 1 ? BN : (BN * 3 / 2 > BN ? BN * 3 / 2 : BN);  // logits, then the planes of the probabilities
+    static constexpr int kBytes = kQ + kStages * kSlot + 1024 + 512;
+    static_assert(QT == 1 || NP == 1, "two query tiles are loaded as one plane");
+    static_assert(kStages >= 2 && 2 * kBuffer + 2 * GR * 64 <= 512, "does not fit");
+    static_assert(kTcRows * GR * 64 * 4 + 2 * kTcRows * 4 <= kQ + kStages * kSlot, "no room to join the two groups");
+};
+
+template <int GR, int BN, int NP, int QT, class T>
+__global__ void __launch_bounds__(kTcThreads, 1)
+attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                    const __grid_constant__ CUtensorMap map_v, AttentionCall a, TcRows rows_q, TcRows rows_k, TcRows rows_v, int splits,
+                    T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part_out, float2* __restrict__ part_stat,
+                    TcControl ctl) {
+    using Cfg = TcForward<GR, BN, NP, QT>;
+    constexpr int kStages = Cfg::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* ring = smem + Cfg::kQ;
+    TcShared* sh = (TcShared*)(ring + kStages * Cfg::kSlot);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int h = blockIdx.y, kv = h / (a.heads / a.kv_heads), split = blockIdx.z;
+    int cloud;
+    int64_t row0, row_end, begin = 0, end = 0;
+    if (!tc_block_rows<QT * kTcRows>(a.query_ends, a.clouds, a.num_queries, blockIdx.x, cloud, row0, row_end)) return;
+    const int rows_here = (int)min((int64_t)(QT * kTcRows), row_end - row0);
+    if (cloud < a.clouds) {
+        begin = cloud_begin(a.key_ends, cloud, a.num_keys);
+        end = cloud_end(a.key_ends, cloud, a.clouds, a.num_keys);
+    }
+    {  // this split's keys, in whole tiles
+        const int64_t tiles = (end - begin + BN - 1) / BN, per = (tiles + splits - 1) / splits;
+        const int64_t lo = begin + split * per * BN;
+        end = min(end, lo + per * BN);
+        begin = min(lo, end);
+    }
+    const int64_t stat0 = ((int64_t)split * a.num_queries + row0) * a.heads + h;
+    if (begin == end) {  // the same for the whole block
+        for (int r = threadIdx.x; r < rows_here; r += kTcThreads) {
+            if (splits > 1) {
+                part_stat[stat0 + (int64_t)r * a.heads] = make_float2(-INFINITY, 0.f);
+            } else {
+                lse[(int64_t)h * a.num_queries + row0 + r] = -INFINITY;
+                const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                for (int c = 0; c < a.size; c += 8) store_vec<T, 8>(out + ((row0 + r) * a.heads + h) * a.size + c, zero);
+            }
+        }
+        return;
+    }
+    const uint32_t tmem = tc_begin<512>(sh, kStages);
+    const int tiles = (int)((end - begin + BN - 1) / BN), q_tiles = rows_here > kTcRows ? 2 : 1, units = tiles * q_tiles;
+    const int last_valid = (int)(end - begin) - (tiles - 1) * BN;
+    const int steps = (a.size + 15) >> 4, n_out = steps * 16;
+    const uint32_t acc = tmem + 2 * Cfg::kBuffer;  // accumulator of group w: acc + w * GR * 64
+    volatile int* failed = &sh->failed;
+    const uint32_t limit = ctl.poll_limit;
+
+    int issued = 0;  // streamed tiles that the loader has started
+    if (warp == 8) {
+        // ---- loader: the tiles in the order in which the products use them
+        bool ok = true;
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            // both tiles complete the one phase of fixed_full, which the products wait for
+            const int valid = rows_here - t * kTcRows;
+            if (t < q_tiles && q_tiles == 1) tc_load_tile<kTcRows, NP, GR>(smem, &map_q, rows_q, a.num_queries, h, row0, valid, a.size, &sh->fixed_full);
+        }
+        if (QT == 2 && q_tiles == 2) {
+            // the first tile is whole; the second may end inside the cloud
+            const int valid = rows_here - kTcRows;
+            if (valid < kTcRows) {
+                // written by the warp first, so that the one arrival (with the first tile's bytes) covers it
+                const int chunks = a.size >> 3;
+#pragma unroll 1
+                for (int g = 0; g < GR; ++g) {
+                    const __nv_bfloat16* from = rows_q.data + (row0 + kTcRows) * rows_q.row + h * rows_q.head + g * 64;
+#pragma unroll 8
+                    for (int i = lane; i < kTcRows * 8; i += 32) {
+                        const int r = i >> 3, c = i & 7;
+                        uint4 v = make_uint4(0, 0, 0, 0);
+                        if (r < valid && g * 8 + c < chunks) v = *reinterpret_cast<const uint4*>(from + r * rows_q.row + c * 8);
+                        *reinterpret_cast<uint4*>(smem + (GR + g) * kTcRows * 128 + sw128_offset(r, c)) = v;
+                    }
+                }
+                fence_smem_to_async_proxy();
+                __syncwarp();
+            }
+            if (lane == 0) {
+                mbar_expect_tx(&sh->fixed_full, (valid < kTcRows ? 1 : 2) * GR * kTcRows * 128);
+                for (int t = 0; t < (valid < kTcRows ? 1 : 2); ++t)
+#pragma unroll
+                    for (int g = 0; g < GR; ++g)
+                        tma_load_3d(smem + (t * GR + g) * kTcRows * 128, &map_q, &sh->fixed_full, g * 64, h, (int)(row0 + t * kTcRows));
+            }
+            __syncwarp();
+        }
+        // one query tile: K0 K1 V0 K2 V1 ... ; two: K0 V0 K1 V1 ...
+        const int loads = 2 * tiles;
+        for (; issued < loads; ++issued) {
+            const int it = issued;
+            if (ctl.withhold_from >= 0 && it >= ctl.withhold_from) ok = false;
+            const int s = it % kStages;
+            if (ok && it >= kStages) ok = tc_wait_warp(&sh->empty[s], (it / kStages - 1) & 1, limit, failed);
+            if (!ok) break;
+            bool is_value;
+            int j;
+            if (q_tiles == 2 || tiles == 1) {
+                is_value = it & 1;
+                j = it >> 1;
+            } else if (it == 0) {
+                is_value = false;
+                j = 0;
+            } else if (it == loads - 1) {
+                is_value = true;
+                j = tiles - 1;
+            } else {
+                is_value = !(it & 1);
+                j = is_value ? it / 2 - 1 : it / 2 + 1;
+            }
+            const int valid = j == tiles - 1 ? last_valid : BN;
+            if (is_value) tc_load_tile<BN, NP, GR>(ring + s * Cfg::kSlot, &map_v, rows_v, a.num_keys, kv, begin + (int64_t)j * BN, valid, a.size, &sh->full[s]);
+            else tc_load_tile<BN, NP, GR>(ring + s * Cfg::kSlot, &map_k, rows_k, a.num_keys, kv, begin + (int64_t)j * BN, valid, a.size, &sh->full[s]);
+        }
+        if (!ok && lane == 0) tc_fail(sh, ctl, 1);
+    } else if (warp == 9 && lane == 0) {
+        // ---- products: logits of units 0 and 1, then (output of unit u, logits of unit u + 2)
+        int used = 0, key_slot = 0, value_slot = 0;
+        auto take = [&](int& slot) {  // the next tile of the ring
+            slot = used % kStages;
+            const bool good = tc_wait(&sh->full[slot], (used / kStages) & 1, limit, failed);
+            ++used;
+            tc_fence_after();
+            return good;
+        };
+        auto logits = [&](int u) {
+            const bool first = q_tiles == 1 || !(u & 1), last = q_tiles == 1 || (u & 1);
+            if (first && !take(key_slot)) return false;
+            const int t = q_tiles == 2 ? u & 1 : 0;
+            tc_rows_by_rows<NP, GR, BN>(tmem + (u & 1) * Cfg::kBuffer, smem_u32(smem + t * NP * GR * kTcRows * 128),
+                                        smem_u32(ring + key_slot * Cfg::kSlot), steps);
+            if (last) tc_commit(&sh->empty[key_slot]);
+            tc_commit(&sh->s_full[u & 1]);
+            return true;
+        };
+        auto weigh = [&](int u) {
+            const bool first = q_tiles == 1 || !(u & 1), last = q_tiles == 1 || (u & 1);
+            if (first && !take(value_slot)) return false;
+            if (!tc_wait(&sh->e_ready[u & 1], (u >> 1) & 1, limit, failed)) return false;
+            tc_fence_after();
+            const int j = q_tiles == 2 ? u >> 1 : u, valid = j == tiles - 1 ? last_valid : BN;
+            tc_weights_by_rows<NP, GR, BN>(acc + (u & 1) * GR * 64, tmem + (u & 1) * Cfg::kBuffer, smem_u32(ring + value_slot * Cfg::kSlot),
+                                           n_out, (valid + 15) >> 4, u >= 2);
+            if (last) tc_commit(&sh->empty[value_slot]);
+            return true;
+        };
+        bool ok = tc_wait(&sh->fixed_full, 0, limit, failed);
+        tc_fence_after();
+        ok = ok && logits(0) && (units < 2 || logits(1));
+        for (int u = 0; u < units && ok; ++u) ok = weigh(u) && (u + 2 >= units || logits(u + 2));
+        if (ok) {
+            tc_commit(&sh->all_done);
+        } else {
+            tc_fail(sh, ctl, 2);
+            tc_commit(&sh->drained);  // tensor memory may only be released once the products in flight have finished
+            mbar_wait(&sh->drained, 0, limit);
+        }
+    }
+
+    const int group = warp >> 2, row = threadIdx.x & 127;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of tensor memory, in the address's upper half
+    const float c2 = a.scale * kLog2e;
+    float base = -INFINITY, total = 0.f;  // reference of the exponents (log2 units) and sum of the probabilities
+    bool ok = true;
+    if (warp < 8) {
+        // ---- element-wise: logits to probabilities
+        const uint32_t buf = tmem + lanes + group * Cfg::kBuffer, my_acc = acc + lanes + group * GR * 64;
+        for (int u = group; u < units; u += 2) {
+            if (!(ok = tc_wait_warp(&sh->s_full[group], (u >> 1) & 1, limit, failed))) break;
+            tc_fence_after();
+            const int j = q_tiles == 2 ? u >> 1 : u, valid = j == tiles - 1 ? last_valid : BN;
+            uint32_t s[BN / 32][32];
+#pragma unroll
+            for (int i = 0; i < BN / 32; ++i) tc_ld_32x32(buf + 32 * i, s[i]);
+            if (valid < BN) {  // columns behind the cloud repeat the first one, which changes no maximum
+#pragma unroll
+                for (int i = 0; i < BN; ++i)
+                    if (i >= valid) s[i / 32][i % 32] = s[0][0];
+            }
+            float m[4];
+            if (c2 >= 0.f) {
+#pragma unroll
+                for (int i = 0; i < BN; ++i) m[i & 3] = i < 4 ? __uint_as_float(s[0][i]) : fmaxf(m[i & 3], __uint_as_float(s[i / 32][i % 32]));
+                m[0] = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < BN; ++i) m[i & 3] = i < 4 ? __uint_as_float(s[0][i]) : fminf(m[i & 3], __uint_as_float(s[i / 32][i % 32]));
+                m[0] = fminf(fminf(m[0], m[1]), fminf(m[2], m[3]));
+            }
+            const float top = m[0] * c2;
+            if (__any_sync(kFullMask, !(top <= base + 8.f))) {
+                const float now = fmaxf(base, top), fade = exp2_fast(base - (now == -INFINITY ? 0.f : now));
+                base = now;
+                total *= fade;
+                if (u >= 2) {
+#pragma unroll 1
+                    for (int c = 0; c < n_out; c += 16) {
+                        uint32_t r[16];
+                        tc_ld_32x16(my_acc + c, r);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * fade);
+                        tc_st_32x16(my_acc + c, r);
+                    }
+                }
+            }
+            const float from = base == -INFINITY ? 0.f : base;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < BN / 32; ++i) {
+                float p[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) p[e] = exp2_fast(fmaf(__uint_as_float(s[i][e]), c2, -from));
+                if (valid < BN) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (i * 32 + e >= valid) p[e] = 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < 32; ++e) sum[e & 3] += p[e];
+                // rounded to bf16 (NP = 1) only as the weights of the values; their sum is taken before
+                tc_store_weights<NP, BN / 2>(buf + 16 * i, p);
+            }
+            total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(&sh->e_ready[group]);
+        }
+        if (ok && group < units) {
+            ok = tc_wait_warp(&sh->all_done, 0, limit, failed);
+            tc_fence_after();
+        }
+        if (!ok && lane == 0) tc_fail(sh, ctl, 3);
+    }
+    __syncwarp();  // the thread that issued the products rejoins its warp
+    __syncthreads();
+    const bool good = !*failed;
+    if (!good && warp == 8) tc_drain_loads(sh, issued, kStages, limit);
+    // ---- joining the two groups of a single query tile, through the shared memory of the tiles
+    float* swap_acc = (float*)smem;                    // [features][128 rows]
+    float* swap_stat = swap_acc + kTcRows * GR * 64;   // [2][128]
+    if (good && warp >= 4 && warp < 8 && q_tiles == 1) {
+        if (units > 1) {
+#pragma unroll 1
+            for (int c = 0; c < n_out; c += 16) {
+                uint32_t r[16];
+                tc_ld_32x16(acc + lanes + GR * 64 + c, r);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) swap_acc[(c + i) * kTcRows + row] = __uint_as_float(r[i]);
+            }
+        }
+        swap_stat[row] = base;
+        swap_stat[kTcRows + row] = total;
+    }
+    __syncthreads();
+    if (good && warp < 4 * q_tiles) {
+        const int64_t m = row0 + group * kTcRows + row;
+        const bool live = m < row_end;
+        float own = 1.f, other = 0.f;
+        if (q_tiles == 1 && units > 1) {
+            const float b1 = swap_stat[row], now = fmaxf(base, b1), from = now == -INFINITY ? 0.f : now;
+            own = exp2_fast(base - from);
+            other = exp2_fast(b1 - from);
+            total = total * own + swap_stat[kTcRows + row] * other;
+            base = now;
+        }
+        const float inv = splits > 1 ? 1.f : total == 0.f ? 0.f : 1.f / total;
+        const int64_t at = m * a.heads + h;
+        if (live) {
+            if (splits > 1) part_stat[stat0 + ((int64_t)group * kTcRows + row) * a.heads] = make_float2(base, total);
+            else lse[(int64_t)h * a.num_queries + m] = total == 0.f ? -INFINITY : (base + log2f(total)) * kLn2;
+        }
+        const int64_t slot = (int64_t)split * a.num_queries * a.heads + at;
+#pragma unroll 1
+        for (int c = 0; c < n_out; c += 16) {
+            uint32_t r[16];
+            tc_ld_32x16(acc + lanes + group * GR * 64 + c, r);
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                x[i] = __uint_as_float(r[i]);
+                if (q_tiles == 1 && units > 1) x[i] = x[i] * own + swap_acc[(c + i) * kTcRows + row] * other;
+                x[i] *= inv;
+            }
+            if (live) {
+                if (splits > 1) tc_write16<float>(part_out + slot * a.size, c, a.size, x);
+                else tc_write16<T>(out + at * a.size, c, a.size, x);
+            }
+        }
+    }
+    tc_end<512>(tmem);
+}
+
+}  // namespace pccnn

@@ -597,6 +597,8 @@ transpose_bf16_kernel(int rows, int cols, const __nv_bfloat16* __restrict__ src,
 // ---- host side ------------------------------------------------------------------------------
 static uint32_t g_host_poll_limit = 1u << 21;  // host mirror of d_poll_limit for kernels of other translation units
 uint32_t tensor_core_poll_limit() { return g_host_poll_limit; }
+static int g_host_withhold_from = -1;  // host mirror of d_withhold_from, likewise
+int tensor_core_withhold_from() { return g_host_withhold_from; }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -636,6 +638,29 @@ static int make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t ld
     if (r != CUDA_SUCCESS) {
         set_error("cuTensorMapEncodeTiled failed with code %d (rows %lld, ld %lld, box %d)", (int)r, (long long)rows,
                   (long long)ld, box_rows);
+        return PCCNN_ERR_CUDA;
+    }
+    return PCCNN_OK;
+}
+
+// bf16 tensor [rows, heads, size] with the given row and head strides (elements, multiples of 8), box = box_rows x 1 x 64,
+// 128-byte swizzle; features beyond `size` read as zeros.
+int make_heads_map(CUtensorMap* map, const void* base, int64_t rows, int heads, int size, int64_t row_stride, int64_t head_stride,
+                   int box_rows) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) {
+        set_error("cuTensorMapEncodeTiled is not available from the driver");
+        return PCCNN_ERR_CUDA;
+    }
+    const cuuint64_t dims[3] = {(cuuint64_t)size, (cuuint64_t)heads, (cuuint64_t)rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)row_stride * 2};
+    const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows}, ones[3] = {1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, ones,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled failed (%d) for %lld x %d heads of %d, strides %lld, %lld", (int)r, (long long)rows, heads, size,
+                  (long long)row_stride, (long long)head_stride);
         return PCCNN_ERR_CUDA;
     }
     return PCCNN_OK;
@@ -771,6 +796,7 @@ int pccnn_gemm_set_test_hooks(int poll_limit, int withhold_from) {
     const uint32_t limit = poll_limit > 0 ? (uint32_t)poll_limit : (1u << 21);
     g_host_poll_limit = limit;
     const int withhold = withhold_from >= 0 ? withhold_from : -1;
+    g_host_withhold_from = withhold;
     PCCNN_CUDA(cudaMemcpyToSymbol(d_poll_limit, &limit, sizeof(limit)));
     PCCNN_CUDA(cudaMemcpyToSymbol(d_withhold_from, &withhold, sizeof(withhold)));
     return PCCNN_OK;

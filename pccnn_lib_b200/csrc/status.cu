@@ -52,11 +52,22 @@ int publish_status(const int* status_dev, int origin, cudaStream_t s) {
     return PCCNN_OK;
 }
 
+int* sticky_status_device() {
+    int* sticky = sticky_status_word();
+    int* dev = nullptr;
+    if (!sticky || cudaHostGetDevicePointer((void**)&dev, sticky, 0) != cudaSuccess) {
+        set_error("no pinned status word: %s", cudaGetErrorString(g_status_err));
+        return nullptr;
+    }
+    return dev;
+}
+
 static const char* origin_name(int origin) {
     switch (origin) {
         case kOriginConvForward: return "convolution forward";
         case kOriginConvBackward: return "convolution backward";
         case kOriginWeightVar: return "weight-variance operator";
+        case kOriginAttention: return "cross attention";
         default: return "kernel";
     }
 }
