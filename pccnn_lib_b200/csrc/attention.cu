@@ -486,9 +486,10 @@ static int launch_rows(const AttentionCall& a, const RowLayout& l, void* out, fl
     return splits > 1 ? join_splits(a, splits, part, stat, out, lse, s) : PCCNN_OK;
 }
 
-template <class T>
-static int add_splits(int64_t count, int splits, const float* part, void* out, cudaStream_t s) {
-    add_splits_kernel<T><<<grid_for(count, 256, 8), 256, 0, s>>>(count, splits, part, (T*)out);
+int add_splits(int is_bf16, int64_t count, int splits, const float* part, void* out, cudaStream_t s) {
+    const unsigned blocks = grid_for(count, 256, 8);
+    if (is_bf16) add_splits_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(count, splits, part, (__nv_bfloat16*)out);
+    else add_splits_kernel<float><<<blocks, 256, 0, s>>>(count, splits, part, (float*)out);
     PCCNN_LAUNCH_CHECK();
     return PCCNN_OK;
 }
@@ -503,7 +504,7 @@ static int launch_grad_rows(const AttentionCall& a, const HeadRows& grads, const
             a, grads, l.lanes, splits, lse, delta, (T*)dq, part);
         PCCNN_LAUNCH_CHECK();
         if (splits > 1)
-            if (int rc = add_splits<T>(a.num_queries * a.heads * a.size, splits, part, dq, s)) return rc;
+            if (int rc = add_splits(a.is_bf16, a.num_queries * a.heads * a.size, splits, part, dq, s)) return rc;
     }
     if (a.num_keys > 0) {
         const int splits = key_grad_splits(a);
@@ -512,8 +513,8 @@ static int launch_grad_rows(const AttentionCall& a, const HeadRows& grads, const
             a, grads, l.lanes, splits, lse, delta, (T*)dk, (T*)dv, part, part + splits * count);
         PCCNN_LAUNCH_CHECK();
         if (splits > 1) {
-            if (int rc = add_splits<T>(count, splits, part, dk, s)) return rc;
-            if (int rc = add_splits<T>(count, splits, part + splits * count, dv, s)) return rc;
+            if (int rc = add_splits(a.is_bf16, count, splits, part, dk, s)) return rc;
+            if (int rc = add_splits(a.is_bf16, count, splits, part + splits * count, dv, s)) return rc;
         }
     }
     return PCCNN_OK;
@@ -603,7 +604,8 @@ size_t pccnn_cross_attention_grads_workspace_bytes(int64_t num_queries, int64_t 
                                      nullptr, nullptr, nullptr, nullptr, 1.f);
     const size_t sq = query_grad_splits(a), sk = key_grad_splits(a);
     const size_t pq = sq > 1 ? sq * num_queries * heads * size * 4 : 0, pk = sk > 1 ? 2 * sk * num_keys * kv_heads * size * 4 : 0;
-    return align_up((size_t)num_queries * heads * 4 + 256) + align_up(pq > pk ? pq : pk);
+    const size_t by_rows = align_up(pq > pk ? pq : pk), by_tiles = tc_grads_shape(a) ? tc_grads_workspace(a) : 0;
+    return align_up((size_t)num_queries * heads * 4 + 256) + (by_rows > by_tiles ? by_rows : by_tiles);
 }
 
 int pccnn_cross_attention_grads(int64_t num_queries, int64_t num_keys, int clouds, int heads, int kv_heads, int size, int is_bf16,
@@ -624,6 +626,7 @@ int pccnn_cross_attention_grads(int64_t num_queries, int64_t num_keys, int cloud
         return PCCNN_ERR_WORKSPACE;
     }
     cudaStream_t s = (cudaStream_t)stream;
+    if (int rc = take_sticky_status("cross_attention_grads")) return rc;
     const HeadRows grads{in_grads, grad_strides_host[0], grad_strides_host[1]};
     float* delta = (float*)workspace;
     char* rest = (char*)workspace + align_up((size_t)num_queries * heads * 4 + 256);
@@ -633,6 +636,9 @@ int pccnn_cross_attention_grads(int64_t num_queries, int64_t num_keys, int cloud
         else attention_delta_kernel<float><<<blocks, 256, 0, s>>>(num_queries, heads, size, (const float*)out, grads, delta);
         PCCNN_LAUNCH_CHECK();
     }
+    if (num_queries > 0 && num_keys > 0 && tc_grads_shape(a) && tc_layout(a, &grads) && aligned16(out_query_grads) && aligned16(out_key_grads) &&
+        aligned16(out_value_grads))
+        return tc_grads(a, grads, lse, delta, out_query_grads, out_key_grads, out_value_grads, rest, s);
     const BackwardRows b{a, grads, row_layout(a, &grads), lse, delta, out_query_grads, out_key_grads, out_value_grads, rest, s};
     return is_bf16 ? dispatch_rows<__nv_bfloat16>(b.l, b) : dispatch_rows<float>(b.l, b);
 }

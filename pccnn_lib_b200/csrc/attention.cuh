@@ -30,6 +30,13 @@ bool tc_layout(const AttentionCall& a, const HeadRows* grads);
 size_t tc_forward_workspace(const AttentionCall& a);
 int tc_forward(const AttentionCall& a, void* out, float* lse, char* ws, cudaStream_t s);
 
+bool tc_grads_shape(const AttentionCall& a);
+size_t tc_grads_workspace(const AttentionCall& a);
+int tc_grads(const AttentionCall& a, const HeadRows& grads, const float* lse, const float* delta, void* dq, void* dk, void* dv, char* ws,
+             cudaStream_t s);
+
+// out = the sum of the splits' parts [splits, count].
+int add_splits(int is_bf16, int64_t count, int splits, const float* part, void* out, cudaStream_t s);
 // Joins the splits of every query: part_out [splits, queries, heads, size] relative to part_stat's (maximum in log2 units, sum).
 int join_splits(const AttentionCall& a, int splits, const float* part_out, const float2* part_stat, void* out, float* lse, cudaStream_t s);
 

@@ -159,4 +159,74 @@ int tc_forward(const AttentionCall& a, void* out, float* lse, char* ws, cudaStre
     return a.size <= 64 ? launch_forward<1, 64, 3, 1, float>(a, out, lse, ws, s) : launch_forward<2, 64, 3, 1, float>(a, out, lse, ws, s);
 }
 
+// ---- backward -----------------------------------------------------------------------------------------------------
+// The tiles that stay in shared memory: 32-bit heads of more than 64 features need 192 KB for them alone and take the row kernels.
+// The streamed tiles of all heads that share a key head are counted in 32 bits.
+bool tc_grads_shape(const AttentionCall& a) {
+    return tc_shape(a) && (a.is_bf16 || a.size <= 64) && (a.num_queries / 64 + 1) * (a.heads / a.kv_heads) < 0x7fffffffLL;
+}
+
+static int tc_grad_splits(const AttentionCall& a, bool keys) {
+    const int64_t rows = keys ? a.num_keys : a.num_queries, streamed = keys ? a.num_queries : a.num_keys;
+    const int clouds = a.clouds > 0 ? a.clouds : 1;
+    const int64_t blocks = ((rows + kTcRows - 1) / kTcRows + clouds / 2) * (keys ? a.kv_heads : a.heads);
+    return tc_splits(blocks, streamed / clouds * (keys ? a.heads / a.kv_heads : 1), 64);
+}
+
+size_t tc_grads_workspace(const AttentionCall& a) {
+    const bool planes = !a.is_bf16;
+    const size_t sq = tc_grad_splits(a, false), sk = tc_grad_splits(a, true);
+    const size_t pq = sq > 1 ? sq * a.num_queries * a.heads * a.size * 4 : 0, pk = sk > 1 ? 2 * sk * a.num_keys * a.kv_heads * a.size * 4 : 0;
+    return 2 * operand_bytes(a.num_queries, a.heads, a.size, planes) + 2 * operand_bytes(a.num_keys, a.kv_heads, a.size, planes) +
+           align_up(pq > pk ? pq : pk) + 256;
+}
+
+template <bool KEYS, int GR, int NP, class T>
+static int launch_grads(const AttentionCall& a, const TcOperand& f1, const TcOperand& f2, const TcOperand& y1, const TcOperand& y2,
+                        const float* lse, const float* delta, void* out1, void* out2, char* ws, cudaStream_t s) {
+    using Cfg = TcBackward<KEYS, GR, NP>;
+    static std::atomic<uint64_t> done{0};
+    const auto kernel = attention_tc_grads_kernel<KEYS, GR, NP, T>;
+    if (int rc = allow_shared(kernel, Cfg::kBytes, done)) return rc;
+    TcControl ctl;
+    if (int rc = tc_control(ctl)) return rc;
+    CUtensorMap m[4];
+    if (int rc = operand_map(&m[0], f1, a.size, NP == 3, kTcRows)) return rc;
+    if (int rc = operand_map(&m[1], f2, a.size, NP == 3, kTcRows)) return rc;
+    if (int rc = operand_map(&m[2], y1, a.size, NP == 3, Cfg::kBN)) return rc;
+    if (int rc = operand_map(&m[3], y2, a.size, NP == 3, Cfg::kBN)) return rc;
+    const int64_t rows = KEYS ? a.num_keys : a.num_queries;
+    const int heads = KEYS ? a.kv_heads : a.heads, splits = tc_grad_splits(a, KEYS);
+    const int64_t count = rows * heads * a.size;
+    float* part = (float*)ws;
+    const dim3 grid((unsigned)tc_blocks(rows, kTcRows, a.clouds), (unsigned)heads, (unsigned)splits);
+    kernel<<<grid, kTcThreads, Cfg::kBytes, s>>>(m[0], m[1], m[2], m[3], a, f1.rows, f2.rows, y1.rows, y2.rows, splits, lse, delta, (T*)out1,
+                                                 (T*)out2, part, part + splits * count, ctl);
+    PCCNN_LAUNCH_CHECK();
+    if (splits > 1) {
+        if (int rc = add_splits(a.is_bf16, count, splits, part, out1, s)) return rc;
+        if (KEYS) return add_splits(a.is_bf16, count, splits, part + splits * count, out2, s);
+    }
+    return PCCNN_OK;
+}
+
+template <int GR, int NP, class T>
+static int launch_both_grads(const AttentionCall& a, const HeadRows& grads, const float* lse, const float* delta, void* dq, void* dk, void* dv,
+                             char* ws, cudaStream_t s) {
+    TcOperand q, k, v, g;
+    if (int rc = tc_operand(q, a.q, a.num_queries, a.heads, a.size, NP == 3, ws, s)) return rc;
+    if (int rc = tc_operand(g, grads, a.num_queries, a.heads, a.size, NP == 3, ws, s)) return rc;
+    if (int rc = tc_operand(k, a.k, a.num_keys, a.kv_heads, a.size, NP == 3, ws, s)) return rc;
+    if (int rc = tc_operand(v, a.v, a.num_keys, a.kv_heads, a.size, NP == 3, ws, s)) return rc;
+    if (int rc = launch_grads<false, GR, NP, T>(a, q, g, k, v, lse, delta, dq, nullptr, ws, s)) return rc;
+    return launch_grads<true, GR, NP, T>(a, k, v, q, g, lse, delta, dk, dv, ws, s);
+}
+
+int tc_grads(const AttentionCall& a, const HeadRows& grads, const float* lse, const float* delta, void* dq, void* dk, void* dv, char* ws,
+             cudaStream_t s) {
+    if (!a.is_bf16) return launch_both_grads<1, 3, float>(a, grads, lse, delta, dq, dk, dv, ws, s);
+    return a.size <= 64 ? launch_both_grads<1, 1, __nv_bfloat16>(a, grads, lse, delta, dq, dk, dv, ws, s)
+                        : launch_both_grads<2, 1, __nv_bfloat16>(a, grads, lse, delta, dq, dk, dv, ws, s);
+}
+
 }  // namespace pccnn

@@ -42,7 +42,8 @@ struct TcControl {
 };
 
 struct TcShared {
-    uint64_t fixed_full, full[kTcMaxStages], empty[kTcMaxStages], s_full[2], e_ready[2], all_done, drained;
+    uint64_t fixed_full, fixed_full2, full[kTcMaxStages], full2[kTcMaxStages], empty[kTcMaxStages], s_full[2], e_ready[2], all_done,
+        drained;
     uint32_t tmem;
     int failed;
 };
@@ -210,8 +211,10 @@ template <int COLUMNS>
 __device__ __forceinline__ uint32_t tc_begin(TcShared* sh, int stages) {
     if (threadIdx.x == 0) {
         mbar_init(&sh->fixed_full, 1);
+        mbar_init(&sh->fixed_full2, 1);
         for (int i = 0; i < stages; ++i) {
             mbar_init(&sh->full[i], 1);
+            mbar_init(&sh->full2[i], 1);
             mbar_init(&sh->empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -556,6 +559,247 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             if (live) {
                 if (splits > 1) tc_write16<float>(part_out + slot * a.size, c, a.size, x);
                 else tc_write16<T>(out + at * a.size, c, a.size, x);
+            }
+        }
+    }
+    tc_end<512>(tmem);
+}
+
+
+// ---- backward -----------------------------------------------------------------------------------------------------
+// KEYS = false: block = 128 queries of one cloud and head; it keeps Q and dO and streams K and V:
+//   s = Q K^T, t = dO V^T, e = exp(scale s - lse) (t - delta),  dQ += e K.
+// KEYS = true: block = 128 keys of one cloud and key head; it keeps K and V and streams Q and dO of every head that shares them:
+//   s = K Q^T, t = V dO^T, p = exp(scale s - lse), e = p (t - delta),  dK += e Q,  dV += p dO.
+// Two kernels, each recomputing the logits, instead of one that adds dQ with atomics: every sum is taken in a fixed order.
+template <bool KEYS, int GR, int NP>
+struct TcBackward {
+    static constexpr int kBN = 64;
+    static constexpr int kFixed = NP * GR * kTcRows * 128;   // one of the two tiles that stay
+    static constexpr int kTile = NP * GR * kBN * 128;        // one of the two tiles of a slot
+    static constexpr int kFit = (200 * 1024 - 2 * kFixed) / (2 * kTile);
+    static constexpr int kStages = kFit > 5 ? 5 : kFit;
+    static constexpr int kPlane = kBN / 2;
+    static constexpr int kBuffer = NP == 3 && KEYS ? 2 * NP * kPlane : 2 * kBN;  // s and t; then the planes of e, and those of p
+    static constexpr int kWeights = NP * kPlane;                                 // p's columns behind e's
+    static constexpr int kAcc = GR * 64;
+    static constexpr int kBytes = 2 * kFixed + kStages * (2 * kTile + 2 * kBN * 4) + 1024 + 512;
+    static_assert(kStages >= 2 && 2 * kBuffer + (KEYS ? 2 : 1) * kAcc <= 512 && kBytes <= 227 * 1024, "does not fit");
+};
+
+template <bool KEYS, int GR, int NP, class T>
+__global__ void __launch_bounds__(kTcThreads, 1)
+attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __grid_constant__ CUtensorMap map_f2,
+                          const __grid_constant__ CUtensorMap map_y1, const __grid_constant__ CUtensorMap map_y2, AttentionCall a,
+                          TcRows rows_f1, TcRows rows_f2, TcRows rows_y1, TcRows rows_y2, int splits, const float* __restrict__ lse,
+                          const float* __restrict__ delta, T* __restrict__ out1, T* __restrict__ out2, float* __restrict__ part1,
+                          float* __restrict__ part2, TcControl ctl) {
+    using Cfg = TcBackward<KEYS, GR, NP>;
+    constexpr int kStages = Cfg::kStages, BN = Cfg::kBN;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* ring = smem + 2 * Cfg::kFixed;
+    float* column_stats = (float*)(ring + kStages * 2 * Cfg::kTile);  // [stages][lse in log2 units, delta][BN]
+    TcShared* sh = (TcShared*)(column_stats + kStages * 2 * BN);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int head = blockIdx.y, split = blockIdx.z, share = a.heads / a.kv_heads;
+    const int64_t num_rows = KEYS ? a.num_keys : a.num_queries, num_stream = KEYS ? a.num_queries : a.num_keys;
+    const int32_t* row_ends = KEYS ? a.key_ends : a.query_ends;
+    const int32_t* stream_ends = KEYS ? a.query_ends : a.key_ends;
+    const int out_heads = KEYS ? a.kv_heads : a.heads;
+    int cloud;
+    int64_t row0, row_end, begin = 0, end = 0;
+    if (!tc_block_rows<kTcRows>(row_ends, a.clouds, num_rows, blockIdx.x, cloud, row0, row_end)) return;
+    const int rows_here = (int)min((int64_t)kTcRows, row_end - row0);
+    if (cloud < a.clouds) {
+        begin = cloud_begin(stream_ends, cloud, num_stream);
+        end = cloud_end(stream_ends, cloud, a.clouds, num_stream);
+    }
+    {
+        const int64_t tiles = (end - begin + BN - 1) / BN, per = (tiles + splits - 1) / splits;
+        const int64_t lo = begin + split * per * BN;
+        end = min(end, lo + per * BN);
+        begin = min(lo, end);
+    }
+    const int64_t out0 = (row0 * out_heads + head) * a.size, shift = (int64_t)split * num_rows * out_heads * a.size;
+    if (begin == end) {
+        const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        for (int r = threadIdx.x; r < rows_here; r += kTcThreads)
+            for (int c = 0; c < a.size; c += 8) {
+                const int64_t at = out0 + (int64_t)r * out_heads * a.size + c;
+                if (splits > 1) {
+                    store_vec<float, 8>(part1 + shift + at, zero);
+                    if (KEYS) store_vec<float, 8>(part2 + shift + at, zero);
+                } else {
+                    store_vec<T, 8>(out1 + at, zero);
+                    if (KEYS) store_vec<T, 8>(out2 + at, zero);
+                }
+            }
+        return;
+    }
+    const uint32_t tmem = tc_begin<512>(sh, kStages);
+    const int tiles = (int)((end - begin + BN - 1) / BN), units = tiles * (KEYS ? share : 1);
+    const int last_valid = (int)(end - begin) - (tiles - 1) * BN;
+    const int steps = (a.size + 15) >> 4, n_out = steps * 16;
+    const uint32_t acc = tmem + 2 * Cfg::kBuffer;
+    volatile int* failed = &sh->failed;
+    const uint32_t limit = ctl.poll_limit;
+    const float c2 = a.scale * kLog2e;
+
+    int issued = 0;
+    if (warp == 8) {
+        // ---- loader: a barrier for each of the two tiles that stay, and for each tile of a slot
+        bool ok = true;
+        tc_load_tile<kTcRows, NP, GR>(smem, &map_f1, rows_f1, num_rows, head, row0, rows_here, a.size, &sh->fixed_full);
+        tc_load_tile<kTcRows, NP, GR>(smem + Cfg::kFixed, &map_f2, rows_f2, num_rows, head, row0, rows_here, a.size, &sh->fixed_full2);
+        for (; issued < units; ++issued) {
+            if (ctl.withhold_from >= 0 && issued >= ctl.withhold_from) ok = false;
+            const int s = issued % kStages;
+            if (ok && issued >= kStages) ok = tc_wait_warp(&sh->empty[s], (issued / kStages - 1) & 1, limit, failed);
+            if (!ok) break;
+            const int j = issued % tiles, h = KEYS ? head * share + issued / tiles : head / share;
+            const int valid = j == tiles - 1 ? last_valid : BN;
+            const int64_t from = begin + (int64_t)j * BN;
+            uint8_t* slot = ring + s * 2 * Cfg::kTile;
+            if (KEYS) {  // the columns' statistics; an absent query has probability 2^-inf
+                float* stats = column_stats + s * 2 * BN;
+#pragma unroll
+                for (int i = lane; i < BN; i += 32) {
+                    const float l = i < valid ? lse[(int64_t)h * num_stream + from + i] : -INFINITY;
+                    stats[i] = l == -INFINITY ? INFINITY : l * kLog2e;
+                    stats[BN + i] = i < valid ? delta[(int64_t)h * num_stream + from + i] : 0.f;
+                }
+                __syncwarp();
+            }
+            tc_load_tile<BN, NP, GR>(slot, &map_y1, rows_y1, num_stream, h, from, valid, a.size, &sh->full[s]);
+            tc_load_tile<BN, NP, GR>(slot + Cfg::kTile, &map_y2, rows_y2, num_stream, h, from, valid, a.size, &sh->full2[s]);
+        }
+        if (!ok && lane == 0) tc_fail(sh, ctl, 1);
+    } else if (warp == 9 && lane == 0) {
+        // ---- products: logits of units 0 and 1, then (sums of unit u, logits of unit u + 2)
+        auto logits = [&](int u) {
+            const int s = u % kStages;
+            if (!tc_wait(&sh->full[s], (u / kStages) & 1, limit, failed)) return false;
+            if (!tc_wait(&sh->full2[s], (u / kStages) & 1, limit, failed)) return false;
+            tc_fence_after();
+            const uint32_t buf = tmem + (u & 1) * Cfg::kBuffer, slot = smem_u32(ring + s * 2 * Cfg::kTile);
+            tc_rows_by_rows<NP, GR, BN>(buf, smem_u32(smem), slot, steps);
+            tc_rows_by_rows<NP, GR, BN>(buf + BN, smem_u32(smem + Cfg::kFixed), slot + Cfg::kTile, steps);
+            tc_commit(&sh->s_full[u & 1]);
+            return true;
+        };
+        auto weigh = [&](int u) {
+            if (!tc_wait(&sh->e_ready[u & 1], (u >> 1) & 1, limit, failed)) return false;
+            tc_fence_after();
+            const int s = u % kStages, valid = u % tiles == tiles - 1 ? last_valid : BN;
+            const uint32_t buf = tmem + (u & 1) * Cfg::kBuffer, slot = smem_u32(ring + s * 2 * Cfg::kTile);
+            tc_weights_by_rows<NP, GR, BN>(acc, buf, slot, n_out, (valid + 15) >> 4, u > 0);
+            if (KEYS) tc_weights_by_rows<NP, GR, BN>(acc + Cfg::kAcc, buf + Cfg::kWeights, slot + Cfg::kTile, n_out, (valid + 15) >> 4, u > 0);
+            tc_commit(&sh->empty[s]);
+            return true;
+        };
+        bool ok = tc_wait(&sh->fixed_full, 0, limit, failed) && tc_wait(&sh->fixed_full2, 0, limit, failed);
+        tc_fence_after();
+        ok = ok && logits(0) && (units < 2 || logits(1));
+        for (int u = 0; u < units && ok; ++u) ok = weigh(u) && (u + 2 >= units || logits(u + 2));
+        if (ok) {
+            tc_commit(&sh->all_done);
+        } else {
+            tc_fail(sh, ctl, 2);
+            tc_commit(&sh->drained);  // tensor memory may only be released once the products in flight have finished
+            mbar_wait(&sh->drained, 0, limit);
+        }
+    }
+
+    const int group = warp >> 2, row = threadIdx.x & 127;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    if (warp < 8) {
+        // ---- element-wise
+        bool ok = true;
+        const uint32_t buf = tmem + lanes + group * Cfg::kBuffer;
+        float row_base = INFINITY, row_delta = 0.f;  // KEYS = false: of this thread's query (an absent one: probability 0)
+        if (!KEYS && row < rows_here) {
+            const float l = lse[(int64_t)head * num_rows + row0 + row];
+            row_base = l == -INFINITY ? INFINITY : l * kLog2e;
+            row_delta = delta[(int64_t)head * num_rows + row0 + row];
+        }
+        for (int u = group; u < units; u += 2) {
+            ok = tc_wait_warp(&sh->s_full[group], (u >> 1) & 1, limit, failed);
+            if (KEYS && ok) ok = tc_wait_warp(&sh->full[u % kStages], (u / kStages) & 1, limit, failed);  // the statistics are visible
+            if (!ok) break;
+            tc_fence_after();
+            const int valid = u % tiles == tiles - 1 ? last_valid : BN;
+            const float* stats = column_stats + (u % kStages) * 2 * BN;
+            uint32_t s[BN / 32][32], t[BN / 32][32];
+#pragma unroll
+            for (int i = 0; i < BN / 32; ++i) {
+                tc_ld_32x32(buf + 32 * i, s[i]);
+                tc_ld_32x32(buf + BN + 32 * i, t[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < BN / 32; ++i) {
+                float p[32], e[32];
+#pragma unroll
+                for (int c = 0; c < 32; c += 4) {
+                    float4 base = make_float4(row_base, row_base, row_base, row_base), d = make_float4(row_delta, row_delta, row_delta, row_delta);
+                    if (KEYS) {
+                        base = *reinterpret_cast<const float4*>(stats + i * 32 + c);
+                        d = *reinterpret_cast<const float4*>(stats + BN + i * 32 + c);
+                    }
+                    p[c] = exp2_fast(fmaf(__uint_as_float(s[i][c]), c2, -base.x));
+                    p[c + 1] = exp2_fast(fmaf(__uint_as_float(s[i][c + 1]), c2, -base.y));
+                    p[c + 2] = exp2_fast(fmaf(__uint_as_float(s[i][c + 2]), c2, -base.z));
+                    p[c + 3] = exp2_fast(fmaf(__uint_as_float(s[i][c + 3]), c2, -base.w));
+                    e[c] = p[c] * (__uint_as_float(t[i][c]) - d.x);
+                    e[c + 1] = p[c + 1] * (__uint_as_float(t[i][c + 1]) - d.y);
+                    e[c + 2] = p[c + 2] * (__uint_as_float(t[i][c + 2]) - d.z);
+                    e[c + 3] = p[c + 3] * (__uint_as_float(t[i][c + 3]) - d.w);
+                }
+                if (!KEYS && valid < BN) {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (i * 32 + c >= valid) e[c] = 0.f;  // a key behind the cloud: its probability may overflow
+                }
+                // rounded to bf16 (NP = 1) as the weights of the last two products, as the probabilities of the forward pass
+                tc_store_weights<NP, Cfg::kPlane>(buf + 16 * i, e);
+                if (KEYS) tc_store_weights<NP, Cfg::kPlane>(buf + Cfg::kWeights + 16 * i, p);
+            }
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(&sh->e_ready[group]);
+        }
+        if (ok) {
+            ok = tc_wait_warp(&sh->all_done, 0, limit, failed);
+            tc_fence_after();
+        }
+        if (!ok && lane == 0) tc_fail(sh, ctl, 3);
+    }
+    __syncwarp();  // the thread that issued the products rejoins its warp
+    __syncthreads();
+    const bool good = !*failed;
+    if (!good && warp == 8) {
+        mbar_wait(&sh->fixed_full2, 0, limit);
+        for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i) mbar_wait(&sh->full2[i % kStages], (i / kStages) & 1, limit);
+        tc_drain_loads(sh, issued, kStages, limit);
+    }
+    if (good && warp < 8) {
+        // KEYS: the first group writes dK, the second dV.  Otherwise the groups share the columns of dQ.
+        const float factor = KEYS && group == 1 ? 1.f : a.scale;
+        const int64_t at = out0 + (int64_t)row * out_heads * a.size;
+        T* out = KEYS && group == 1 ? out2 : out1;
+        float* part = KEYS && group == 1 ? part2 : part1;
+        const uint32_t from = acc + lanes + (KEYS ? group * Cfg::kAcc : 0);
+#pragma unroll 1
+        for (int c = KEYS ? 0 : group * 16; c < n_out; c += KEYS ? 16 : 32) {
+            uint32_t r[16];
+            tc_ld_32x16(from + c, r);
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(r[i]) * factor;
+            if (row < rows_here) {
+                if (splits > 1) tc_write16<float>(part + shift + at, c, a.size, x);
+                else tc_write16<T>(out + at, c, a.size, x);
             }
         }
     }
