@@ -43,7 +43,7 @@ struct TcControl {
 
 struct TcShared {
     uint64_t fixed_full, fixed_full2, full[kTcMaxStages], full2[kTcMaxStages], empty[kTcMaxStages], s_full[2], e_ready[2], all_done,
-        drained;
+        drained, round_done, acc_free;
     uint32_t tmem;
     int failed;
 };
@@ -194,6 +194,20 @@ __device__ __forceinline__ void tc_store_weights(uint32_t dst, const float (&p)[
     }
 }
 
+// sum[c] += column c of this thread's row, for the first n of N columns (n is a multiple of 16).
+template <int N>
+__device__ __forceinline__ void tc_add_columns(uint32_t from, int n, float (&sum)[N]) {
+#pragma unroll
+    for (int c = 0; c < N; c += 16) {
+        if (c < n) {
+            uint32_t r[16];
+            tc_ld_32x16(from + c, r);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[c + i] += __uint_as_float(r[i]);
+        }
+    }
+}
+
 template <class T>
 __device__ __forceinline__ void tc_write16(T* __restrict__ dst, int c, int size, const float (&x)[16]) {
 #pragma unroll
@@ -223,6 +237,8 @@ __device__ __forceinline__ uint32_t tc_begin(TcShared* sh, int stages) {
         }
         mbar_init(&sh->all_done, 1);
         mbar_init(&sh->drained, 1);
+        mbar_init(&sh->round_done, 1);
+        mbar_init(&sh->acc_free, 256);
         sh->failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -256,6 +272,9 @@ __device__ __forceinline__ void tc_drain_loads(TcShared* sh, int issued, int sta
 // Block = up to QT x 128 queries of one cloud and head x one split of the keys.  Units: with two query tiles unit u is
 // (keys u / 2, tile u % 2); with one, unit u is key tile u, and the two element-wise groups take every other one, each with an
 // accumulator, running maximum and sum of its own that are joined at the end.
+// The tensor cores truncate when they add to an accumulator (measured on 32-bit heads of 64, 1000 keys: 3.7e-6 of the output with
+// one accumulator for all keys), which bf16 weights hide and 32-bit features do not: for those every unit starts its
+// accumulator anew and the thread of a row adds the units up in registers, rounding to nearest.
 // The accumulator is scaled only when the maximum has grown by more than 2^8 since it was last scaled: the probabilities
 // stay below 2^8, and the final division is by a sum relative to the same reference.
 template <int GR, int BN, int NP, int QT>
@@ -415,7 +434,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             tc_fence_after();
             const int j = q_tiles == 2 ? u >> 1 : u, valid = j == tiles - 1 ? last_valid : BN;
             tc_weights_by_rows<NP, GR, BN>(acc + (u & 1) * GR * 64, tmem + (u & 1) * Cfg::kBuffer, smem_u32(ring + value_slot * Cfg::kSlot),
-                                           n_out, (valid + 15) >> 4, u >= 2);
+                                           n_out, (valid + 15) >> 4, NP == 1 && u >= 2);
             if (last) tc_commit(&sh->empty[value_slot]);
             return true;
         };
@@ -436,6 +455,9 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of tensor memory, in the address's upper half
     const float c2 = a.scale * kLog2e;
     float base = -INFINITY, total = 0.f;  // reference of the exponents (log2 units) and sum of the probabilities
+    float kept[NP == 3 ? GR * 64 : 1];    // the output of all units but the last, for 32-bit features
+#pragma unroll
+    for (int c = 0; c < (NP == 3 ? GR * 64 : 1); ++c) kept[c] = 0.f;
     bool ok = true;
     if (warp < 8) {
         // ---- element-wise: logits to probabilities
@@ -463,11 +485,17 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 m[0] = fminf(fminf(m[0], m[1]), fminf(m[2], m[3]));
             }
             const float top = m[0] * c2;
+            if constexpr (NP == 3) {
+                if (u >= 2) tc_add_columns<GR * 64>(my_acc, n_out, kept);
+            }
             if (__any_sync(kFullMask, !(top <= base + 8.f))) {
                 const float now = fmaxf(base, top), fade = exp2_fast(base - (now == -INFINITY ? 0.f : now));
                 base = now;
                 total *= fade;
-                if (u >= 2) {
+                if constexpr (NP == 3) {
+#pragma unroll
+                    for (int c = 0; c < GR * 64; ++c) kept[c] *= fade;
+                } else if (u >= 2) {
 #pragma unroll 1
                     for (int c = 0; c < n_out; c += 16) {
                         uint32_t r[16];
@@ -505,11 +533,30 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             tc_fence_after();
         }
         if (!ok && lane == 0) tc_fail(sh, ctl, 3);
+        if constexpr (NP == 3) {
+            if (ok && group < units) tc_add_columns<GR * 64>(my_acc, n_out, kept);
+        }
     }
     __syncwarp();  // the thread that issued the products rejoins its warp
     __syncthreads();
     const bool good = !*failed;
     if (!good && warp == 8) tc_drain_loads(sh, issued, kStages, limit);
+    // 16 columns of this thread's accumulator from column c
+    auto result = [&](int c, float (&x)[16]) {
+        if constexpr (NP == 3) {
+#pragma unroll
+            for (int k = 0; k < GR * 64; k += 16)
+                if (c == k) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = kept[k + i];
+                }
+        } else {
+            uint32_t r[16];
+            tc_ld_32x16(acc + lanes + group * GR * 64 + c, r);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(r[i]);
+        }
+    };
     // ---- joining the two groups of a single query tile, through the shared memory of the tiles
     float* swap_acc = (float*)smem;                    // [features][128 rows]
     float* swap_stat = swap_acc + kTcRows * GR * 64;   // [2][128]
@@ -517,10 +564,10 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         if (units > 1) {
 #pragma unroll 1
             for (int c = 0; c < n_out; c += 16) {
-                uint32_t r[16];
-                tc_ld_32x16(acc + lanes + GR * 64 + c, r);
+                float x[16];
+                result(c, x);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) swap_acc[(c + i) * kTcRows + row] = __uint_as_float(r[i]);
+                for (int i = 0; i < 16; ++i) swap_acc[(c + i) * kTcRows + row] = x[i];
             }
         }
         swap_stat[row] = base;
@@ -547,12 +594,10 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         const int64_t slot = (int64_t)split * a.num_queries * a.heads + at;
 #pragma unroll 1
         for (int c = 0; c < n_out; c += 16) {
-            uint32_t r[16];
-            tc_ld_32x16(acc + lanes + group * GR * 64 + c, r);
             float x[16];
+            result(c, x);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                x[i] = __uint_as_float(r[i]);
                 if (q_tiles == 1 && units > 1) x[i] = x[i] * own + swap_acc[(c + i) * kTcRows + row] * other;
                 x[i] *= inv;
             }
@@ -571,6 +616,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 //   s = Q K^T, t = dO V^T, e = exp(scale s - lse) (t - delta),  dQ += e K.
 // KEYS = true: block = 128 keys of one cloud and key head; it keeps K and V and streams Q and dO of every head that shares them:
 //   s = K Q^T, t = V dO^T, p = exp(scale s - lse), e = p (t - delta),  dK += e Q,  dV += p dO.
+// For 32-bit features the accumulators are emptied into registers every kRound units (see the forward kernel on truncation).
 // Two kernels, each recomputing the logits, instead of one that adds dQ with atomics: every sum is taken in a fixed order.
 template <bool KEYS, int GR, int NP>
 struct TcBackward {
@@ -583,6 +629,8 @@ struct TcBackward {
     static constexpr int kBuffer = NP == 3 && KEYS ? 2 * NP * kPlane : 2 * kBN;  // s and t; then the planes of e, and those of p
     static constexpr int kWeights = NP * kPlane;                                 // p's columns behind e's
     static constexpr int kAcc = GR * 64;
+    static constexpr int kRound = 2;                                             // even: both groups have units in a round
+    static constexpr int kKept = NP == 3 ? (KEYS ? kAcc : kAcc / 2) : 1;         // columns that a thread adds up in registers
     static constexpr int kBytes = 2 * kFixed + kStages * (2 * kTile + 2 * kBN * 4) + 1024 + 512;
     static_assert(kStages >= 2 && 2 * kBuffer + (KEYS ? 2 : 1) * kAcc <= 512 && kBytes <= 227 * 1024, "does not fit");
 };
@@ -691,12 +739,15 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
         };
         auto weigh = [&](int u) {
             if (!tc_wait(&sh->e_ready[u & 1], (u >> 1) & 1, limit, failed)) return false;
+            const bool fresh = u == 0 || (NP == 3 && u % Cfg::kRound == 0);
+            if (u > 0 && fresh && !tc_wait(&sh->acc_free, (u / Cfg::kRound - 1) & 1, limit, failed)) return false;
             tc_fence_after();
             const int s = u % kStages, valid = u % tiles == tiles - 1 ? last_valid : BN;
             const uint32_t buf = tmem + (u & 1) * Cfg::kBuffer, slot = smem_u32(ring + s * 2 * Cfg::kTile);
-            tc_weights_by_rows<NP, GR, BN>(acc, buf, slot, n_out, (valid + 15) >> 4, u > 0);
-            if (KEYS) tc_weights_by_rows<NP, GR, BN>(acc + Cfg::kAcc, buf + Cfg::kWeights, slot + Cfg::kTile, n_out, (valid + 15) >> 4, u > 0);
+            tc_weights_by_rows<NP, GR, BN>(acc, buf, slot, n_out, (valid + 15) >> 4, !fresh);
+            if (KEYS) tc_weights_by_rows<NP, GR, BN>(acc + Cfg::kAcc, buf + Cfg::kWeights, slot + Cfg::kTile, n_out, (valid + 15) >> 4, !fresh);
             tc_commit(&sh->empty[s]);
+            if (NP == 3 && (u + 1) % Cfg::kRound == 0 && u + 1 < units) tc_commit(&sh->round_done);
             return true;
         };
         bool ok = tc_wait(&sh->fixed_full, 0, limit, failed) && tc_wait(&sh->fixed_full2, 0, limit, failed);
@@ -714,10 +765,28 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
 
     const int group = warp >> 2, row = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+    float kept[Cfg::kKept];
+#pragma unroll
+    for (int c = 0; c < Cfg::kKept; ++c) kept[c] = 0.f;
+    // KEYS: the first group holds dK, the second dV.  Otherwise each group holds half the columns of dQ.
+    const uint32_t my_acc = acc + lanes + group * (KEYS ? Cfg::kAcc : Cfg::kAcc / 2);
+    const int my_columns = KEYS ? n_out : min(max(n_out - group * (Cfg::kAcc / 2), 0), Cfg::kAcc / 2);
     if (warp < 8) {
         // ---- element-wise
         bool ok = true;
         const uint32_t buf = tmem + lanes + group * Cfg::kBuffer;
+        int emptied = 0;
+        auto empty_until = [&](int round) {  // the accumulators of the rounds before `round` into registers
+            if constexpr (NP == 3) {
+                for (; emptied < round && ok; ++emptied) {
+                    if (!(ok = tc_wait_warp(&sh->round_done, emptied & 1, limit, failed))) break;
+                    tc_fence_after();
+                    tc_add_columns<Cfg::kKept>(my_acc, my_columns, kept);
+                    tc_fence_before();
+                    mbar_arrive(&sh->acc_free);
+                }
+            }
+        };
         float row_base = INFINITY, row_delta = 0.f;  // KEYS = false: of this thread's query (an absent one: probability 0)
         if (!KEYS && row < rows_here) {
             const float l = lse[(int64_t)head * num_rows + row0 + row];
@@ -725,7 +794,8 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
             row_delta = delta[(int64_t)head * num_rows + row0 + row];
         }
         for (int u = group; u < units; u += 2) {
-            ok = tc_wait_warp(&sh->s_full[group], (u >> 1) & 1, limit, failed);
+            empty_until(u / Cfg::kRound);
+            ok = ok && tc_wait_warp(&sh->s_full[group], (u >> 1) & 1, limit, failed);
             if (KEYS && ok) ok = tc_wait_warp(&sh->full[u % kStages], (u / kStages) & 1, limit, failed);  // the statistics are visible
             if (!ok) break;
             tc_fence_after();
@@ -769,9 +839,13 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
             tc_fence_before();
             mbar_arrive(&sh->e_ready[group]);
         }
+        empty_until((units - 1) / Cfg::kRound);
         if (ok) {
             ok = tc_wait_warp(&sh->all_done, 0, limit, failed);
             tc_fence_after();
+        }
+        if constexpr (NP == 3) {
+            if (ok) tc_add_columns<Cfg::kKept>(my_acc, my_columns, kept);
         }
         if (!ok && lane == 0) tc_fail(sh, ctl, 3);
     }
@@ -784,22 +858,27 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
         tc_drain_loads(sh, issued, kStages, limit);
     }
     if (good && warp < 8) {
-        // KEYS: the first group writes dK, the second dV.  Otherwise the groups share the columns of dQ.
         const float factor = KEYS && group == 1 ? 1.f : a.scale;
         const int64_t at = out0 + (int64_t)row * out_heads * a.size;
         T* out = KEYS && group == 1 ? out2 : out1;
         float* part = KEYS && group == 1 ? part2 : part1;
-        const uint32_t from = acc + lanes + (KEYS ? group * Cfg::kAcc : 0);
-#pragma unroll 1
-        for (int c = KEYS ? 0 : group * 16; c < n_out; c += KEYS ? 16 : 32) {
-            uint32_t r[16];
-            tc_ld_32x16(from + c, r);
-            float x[16];
+        const int column0 = KEYS ? 0 : group * (Cfg::kAcc / 2);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(r[i]) * factor;
+        for (int c = 0; c < (KEYS ? Cfg::kAcc : Cfg::kAcc / 2); c += 16) {
+            if (c >= my_columns) break;
+            float x[16];
+            if constexpr (NP == 3) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = kept[c + i] * factor;
+            } else {
+                uint32_t r[16];
+                tc_ld_32x16(my_acc + c, r);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(r[i]) * factor;
+            }
             if (row < rows_here) {
-                if (splits > 1) tc_write16<float>(part + shift + at, c, a.size, x);
-                else tc_write16<T>(out + at, c, a.size, x);
+                if (splits > 1) tc_write16<float>(part + shift + at, column0 + c, a.size, x);
+                else tc_write16<T>(out + at, column0 + c, a.size, x);
             }
         }
     }
