@@ -9,7 +9,7 @@
 // follow belong to another cloud and may hold infinities, which would reach this one as 0 * inf.
 //
 // Roles of the ten warps of a CTA: two groups of four warps do the element-wise work (one row of a 128-row tile per thread,
-// which is one lane of tensor memory), warp 8 loads, one thread of warp 9 issues the products.  The element-wise groups work
+// which is one lane of tensor memory), warp 8 loads, an elected lane of warp 9 issues the products.  The element-wise groups work
 // on different units in turn, so one of them computes while the tensor cores run the products of the other.
 // Every wait is bounded: a role whose wait runs out sets a flag that ends the other roles' waits, the CTA waits for its
 // copies and products in flight, frees its tensor memory and records the failure in the pinned status word.
@@ -122,7 +122,14 @@ __device__ __forceinline__ void tc_load_tile(uint8_t* dst, const CUtensorMap* ma
     __syncwarp();
 }
 
-// ---- products (one thread) ----------------------------------------------------------------------------------------
+// One lane of a converged warp, always the same one.
+__device__ __forceinline__ bool tc_elect() {
+    uint32_t yes;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(yes));
+    return yes != 0;
+}
+
+// ---- products (one elected thread of a converged warp) ----------------------------------------------------------------------------------------
 // The plane pairs of a product, smallest first; one pair (0, 0) for bf16 features.
 template <int NP> struct TcPairs;
 template <> struct TcPairs<1> {
@@ -141,17 +148,22 @@ __device__ __forceinline__ uint32_t tc_idesc(int n, bool b_mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTcRows >> 4) << 24);
 }
 
-// D[128, RB] = A[128, features] B[RB, features]^T, both tiles in shared memory.
+// One thread issues all products, and until it has issued those of a unit the rows of that unit wait: the loops are unrolled
+// and a descriptor is its tile's first one plus a constant (measured with descriptors built in the loop: 3500 of the 5700
+// cycles of a unit were spent waiting for the next logits).
+// D[128, RB] = A[128, features] B[RB, features]^T, both tiles in shared memory; `steps` blocks of 16 features.
 template <int NP, int GR, int RB>
 __device__ __forceinline__ void tc_rows_by_rows(uint32_t d, uint32_t a, uint32_t b, int steps) {
     const uint32_t idesc = tc_idesc(RB, false);
+    const uint64_t da = umma_desc_k_sw128(a), db = umma_desc_k_sw128(b);
 #pragma unroll
     for (int i = 0; i < TcPairs<NP>::kCount; ++i) {
-        const uint32_t pa = a + TcPairs<NP>::a(i) * GR * kTcRows * 128, pb = b + TcPairs<NP>::b(i) * GR * RB * 128;
-#pragma unroll 1
-        for (int k = 0; k < steps; ++k)  // 16 features = 32 bytes further inside the swizzled row
-            tc_mma_bf16(d, umma_desc_k_sw128(pa + (k >> 2) * kTcRows * 128) + 2 * (k & 3),
-                        umma_desc_k_sw128(pb + (k >> 2) * RB * 128) + 2 * (k & 3), idesc, (i > 0 || k > 0) ? 1u : 0u);
+#pragma unroll
+        for (int k = 0; k < GR * 4; ++k) {  // 16 features = 32 bytes further inside the swizzled row; addresses in 16-byte units
+            const int at_a = (TcPairs<NP>::a(i) * GR + (k >> 2)) * kTcRows * 8 + 2 * (k & 3);
+            const int at_b = (TcPairs<NP>::b(i) * GR + (k >> 2)) * RB * 8 + 2 * (k & 3);
+            if (k < steps) tc_mma_bf16(d, da + at_a, db + at_b, idesc, (i > 0 || k > 0) ? 1u : 0u);
+        }
     }
 }
 
@@ -160,12 +172,14 @@ __device__ __forceinline__ void tc_rows_by_rows(uint32_t d, uint32_t a, uint32_t
 template <int NP, int GR, int RB>
 __device__ __forceinline__ void tc_weights_by_rows(uint32_t d, uint32_t e, uint32_t b, int n, int steps, bool accumulate) {
     const uint32_t idesc = tc_idesc(n, true);
+    const uint64_t db = umma_desc_mn_sw128(b, RB * 128);
 #pragma unroll
     for (int i = 0; i < TcPairs<NP>::kCount; ++i) {
-        const uint32_t pe = e + TcPairs<NP>::a(i) * (RB / 2), pb = b + TcPairs<NP>::b(i) * GR * RB * 128;
-#pragma unroll 1
-        for (int k = 0; k < steps; ++k)
-            tc_mma_bf16_ts(d, pe + k * 8, umma_desc_mn_sw128(pb + k * 2048, RB * 128), idesc, (accumulate || i > 0 || k > 0) ? 1u : 0u);
+#pragma unroll
+        for (int k = 0; k < RB / 16; ++k)
+            if (k < steps)
+                tc_mma_bf16_ts(d, e + TcPairs<NP>::a(i) * (RB / 2) + k * 8, db + TcPairs<NP>::b(i) * GR * RB * 8 + k * 128, idesc,
+                               (accumulate || i > 0 || k > 0) ? 1u : 0u);
     }
 }
 
@@ -261,6 +275,20 @@ __device__ __forceinline__ void tc_end(uint32_t tmem) {
 __device__ __forceinline__ void tc_fail(TcShared* sh, const TcControl& ctl, int code) {
     *(volatile int*)&sh->failed = 1;
     atomicCAS_system(ctl.sticky, 0, ctl.status | code);
+}
+// The end of the warp that issues the products: all of them have finished when all_done completes; after a failure it waits for
+// those in flight, since tensor memory may only be released after them.
+__device__ __forceinline__ void tc_finish_products(TcShared* sh, const TcControl& ctl, bool ok, bool leader) {
+    if (leader) {
+        if (ok) {
+            tc_commit(&sh->all_done);
+        } else {
+            tc_fail(sh, ctl, 2);
+            tc_commit(&sh->drained);
+            mbar_wait(&sh->drained, 0, ctl.poll_limit);
+        }
+    }
+    __syncwarp();
 }
 // After a failure: copies that nobody has waited for must land before the CTA retires.
 __device__ __forceinline__ void tc_drain_loads(TcShared* sh, int issued, int stages, uint32_t limit) {
@@ -407,12 +435,13 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             else tc_load_tile<BN, NP, GR>(ring + s * Cfg::kSlot, &map_k, rows_k, a.num_keys, kv, begin + (int64_t)j * BN, valid, a.size, &sh->full[s]);
         }
         if (!ok && lane == 0) tc_fail(sh, ctl, 1);
-    } else if (warp == 9 && lane == 0) {
+    } else if (warp == 9) {
         // ---- products: logits of units 0 and 1, then (output of unit u, logits of unit u + 2)
+        const bool leader = tc_elect();
         int used = 0, key_slot = 0, value_slot = 0;
         auto take = [&](int& slot) {  // the next tile of the ring
             slot = used % kStages;
-            const bool good = tc_wait(&sh->full[slot], (used / kStages) & 1, limit, failed);
+            const bool good = tc_wait_warp(&sh->full[slot], (used / kStages) & 1, limit, failed);
             ++used;
             tc_fence_after();
             return good;
@@ -421,34 +450,34 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const bool first = q_tiles == 1 || !(u & 1), last = q_tiles == 1 || (u & 1);
             if (first && !take(key_slot)) return false;
             const int t = q_tiles == 2 ? u & 1 : 0;
-            tc_rows_by_rows<NP, GR, BN>(tmem + (u & 1) * Cfg::kBuffer, smem_u32(smem + t * NP * GR * kTcRows * 128),
-                                        smem_u32(ring + key_slot * Cfg::kSlot), steps);
-            if (last) tc_commit(&sh->empty[key_slot]);
-            tc_commit(&sh->s_full[u & 1]);
+            if (leader) {
+                tc_rows_by_rows<NP, GR, BN>(tmem + (u & 1) * Cfg::kBuffer, smem_u32(smem + t * NP * GR * kTcRows * 128),
+                                            smem_u32(ring + key_slot * Cfg::kSlot), steps);
+                if (last) tc_commit(&sh->empty[key_slot]);
+                tc_commit(&sh->s_full[u & 1]);
+            }
+            __syncwarp();
             return true;
         };
         auto weigh = [&](int u) {
             const bool first = q_tiles == 1 || !(u & 1), last = q_tiles == 1 || (u & 1);
             if (first && !take(value_slot)) return false;
-            if (!tc_wait(&sh->e_ready[u & 1], (u >> 1) & 1, limit, failed)) return false;
+            if (!tc_wait_warp(&sh->e_ready[u & 1], (u >> 1) & 1, limit, failed)) return false;
             tc_fence_after();
             const int j = q_tiles == 2 ? u >> 1 : u, valid = j == tiles - 1 ? last_valid : BN;
-            tc_weights_by_rows<NP, GR, BN>(acc + (u & 1) * GR * 64, tmem + (u & 1) * Cfg::kBuffer, smem_u32(ring + value_slot * Cfg::kSlot),
-                                           n_out, (valid + 15) >> 4, NP == 1 && u >= 2);
-            if (last) tc_commit(&sh->empty[value_slot]);
+            if (leader) {
+                tc_weights_by_rows<NP, GR, BN>(acc + (u & 1) * GR * 64, tmem + (u & 1) * Cfg::kBuffer,
+                                               smem_u32(ring + value_slot * Cfg::kSlot), n_out, (valid + 15) >> 4, NP == 1 && u >= 2);
+                if (last) tc_commit(&sh->empty[value_slot]);
+            }
+            __syncwarp();
             return true;
         };
-        bool ok = tc_wait(&sh->fixed_full, 0, limit, failed);
+        bool ok = tc_wait_warp(&sh->fixed_full, 0, limit, failed);
         tc_fence_after();
         ok = ok && logits(0) && (units < 2 || logits(1));
         for (int u = 0; u < units && ok; ++u) ok = weigh(u) && (u + 2 >= units || logits(u + 2));
-        if (ok) {
-            tc_commit(&sh->all_done);
-        } else {
-            tc_fail(sh, ctl, 2);
-            tc_commit(&sh->drained);  // tensor memory may only be released once the products in flight have finished
-            mbar_wait(&sh->drained, 0, limit);
-        }
+        tc_finish_products(sh, ctl, ok, leader);
     }
 
     const int group = warp >> 2, row = threadIdx.x & 127;
@@ -537,7 +566,6 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             if (ok && group < units) tc_add_columns<GR * 64>(my_acc, n_out, kept);
         }
     }
-    __syncwarp();  // the thread that issued the products rejoins its warp
     __syncthreads();
     const bool good = !*failed;
     if (!good && warp == 8) tc_drain_loads(sh, issued, kStages, limit);
@@ -724,43 +752,45 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
             tc_load_tile<BN, NP, GR>(slot + Cfg::kTile, &map_y2, rows_y2, num_stream, h, from, valid, a.size, &sh->full2[s]);
         }
         if (!ok && lane == 0) tc_fail(sh, ctl, 1);
-    } else if (warp == 9 && lane == 0) {
+    } else if (warp == 9) {
+        const bool leader = tc_elect();
         // ---- products: logits of units 0 and 1, then (sums of unit u, logits of unit u + 2)
         auto logits = [&](int u) {
             const int s = u % kStages;
-            if (!tc_wait(&sh->full[s], (u / kStages) & 1, limit, failed)) return false;
-            if (!tc_wait(&sh->full2[s], (u / kStages) & 1, limit, failed)) return false;
+            if (!tc_wait_warp(&sh->full[s], (u / kStages) & 1, limit, failed)) return false;
+            if (!tc_wait_warp(&sh->full2[s], (u / kStages) & 1, limit, failed)) return false;
             tc_fence_after();
             const uint32_t buf = tmem + (u & 1) * Cfg::kBuffer, slot = smem_u32(ring + s * 2 * Cfg::kTile);
-            tc_rows_by_rows<NP, GR, BN>(buf, smem_u32(smem), slot, steps);
-            tc_rows_by_rows<NP, GR, BN>(buf + BN, smem_u32(smem + Cfg::kFixed), slot + Cfg::kTile, steps);
-            tc_commit(&sh->s_full[u & 1]);
+            if (leader) {
+                tc_rows_by_rows<NP, GR, BN>(buf, smem_u32(smem), slot, steps);
+                tc_rows_by_rows<NP, GR, BN>(buf + BN, smem_u32(smem + Cfg::kFixed), slot + Cfg::kTile, steps);
+                tc_commit(&sh->s_full[u & 1]);
+            }
+            __syncwarp();
             return true;
         };
         auto weigh = [&](int u) {
-            if (!tc_wait(&sh->e_ready[u & 1], (u >> 1) & 1, limit, failed)) return false;
+            if (!tc_wait_warp(&sh->e_ready[u & 1], (u >> 1) & 1, limit, failed)) return false;
             const bool fresh = u == 0 || (NP == 3 && u % Cfg::kRound == 0);
-            if (u > 0 && fresh && !tc_wait(&sh->acc_free, (u / Cfg::kRound - 1) & 1, limit, failed)) return false;
+            if (u > 0 && fresh && !tc_wait_warp(&sh->acc_free, (u / Cfg::kRound - 1) & 1, limit, failed)) return false;
             tc_fence_after();
             const int s = u % kStages, valid = u % tiles == tiles - 1 ? last_valid : BN;
             const uint32_t buf = tmem + (u & 1) * Cfg::kBuffer, slot = smem_u32(ring + s * 2 * Cfg::kTile);
-            tc_weights_by_rows<NP, GR, BN>(acc, buf, slot, n_out, (valid + 15) >> 4, !fresh);
-            if (KEYS) tc_weights_by_rows<NP, GR, BN>(acc + Cfg::kAcc, buf + Cfg::kWeights, slot + Cfg::kTile, n_out, (valid + 15) >> 4, !fresh);
-            tc_commit(&sh->empty[s]);
-            if (NP == 3 && (u + 1) % Cfg::kRound == 0 && u + 1 < units) tc_commit(&sh->round_done);
+            if (leader) {
+                tc_weights_by_rows<NP, GR, BN>(acc, buf, slot, n_out, (valid + 15) >> 4, !fresh);
+                if (KEYS)
+                    tc_weights_by_rows<NP, GR, BN>(acc + Cfg::kAcc, buf + Cfg::kWeights, slot + Cfg::kTile, n_out, (valid + 15) >> 4, !fresh);
+                tc_commit(&sh->empty[s]);
+                if (NP == 3 && (u + 1) % Cfg::kRound == 0 && u + 1 < units) tc_commit(&sh->round_done);
+            }
+            __syncwarp();
             return true;
         };
-        bool ok = tc_wait(&sh->fixed_full, 0, limit, failed) && tc_wait(&sh->fixed_full2, 0, limit, failed);
+        bool ok = tc_wait_warp(&sh->fixed_full, 0, limit, failed) && tc_wait_warp(&sh->fixed_full2, 0, limit, failed);
         tc_fence_after();
         ok = ok && logits(0) && (units < 2 || logits(1));
         for (int u = 0; u < units && ok; ++u) ok = weigh(u) && (u + 2 >= units || logits(u + 2));
-        if (ok) {
-            tc_commit(&sh->all_done);
-        } else {
-            tc_fail(sh, ctl, 2);
-            tc_commit(&sh->drained);  // tensor memory may only be released once the products in flight have finished
-            mbar_wait(&sh->drained, 0, limit);
-        }
+        tc_finish_products(sh, ctl, ok, leader);
     }
 
     const int group = warp >> 2, row = threadIdx.x & 127;
@@ -849,7 +879,6 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
         }
         if (!ok && lane == 0) tc_fail(sh, ctl, 3);
     }
-    __syncwarp();  // the thread that issued the products rejoins its warp
     __syncthreads();
     const bool good = !*failed;
     if (!good && warp == 8) {
