@@ -48,19 +48,26 @@ struct TcShared {
     int failed;
 };
 
-// Bounded wait that also ends when another role of the CTA has failed.
-__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, uint32_t limit, volatile int* failed) {
-    for (uint32_t left = limit; left > 0;) {
-        const uint32_t now = left < 1024 ? left : 1024;
-        if (mbar_wait(bar, parity, now)) return true;
-        if (*failed) return false;
-        left -= now;
+// Bounded wait of a converged warp, with one answer for all its lanes; it also ends when another role of the CTA has failed.
+// The phase has usually completed already, so the first poll is all that costs (a loop of single lanes took 350 cycles).
+__device__ __forceinline__ bool tc_poll(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return __all_sync(kFullMask, done != 0);
+}
+__device__ __forceinline__ bool tc_wait_warp(uint64_t* bar, uint32_t parity, uint32_t limit, volatile int* failed) {
+    const uint32_t addr = smem_u32(bar);
+    if (tc_poll(addr, parity)) return true;
+#pragma unroll 1
+    for (uint32_t n = 1; n < limit; ++n) {
+        if (tc_poll(addr, parity)) return true;
+        if ((n & 255) == 0 && __any_sync(kFullMask, *failed)) return false;
     }
     return false;
-}
-// The same for a whole warp, with one answer for all its lanes.
-__device__ __forceinline__ bool tc_wait_warp(uint64_t* bar, uint32_t parity, uint32_t limit, volatile int* failed) {
-    return __all_sync(kFullMask, tc_wait(bar, parity, limit, failed));
 }
 
 // The cloud of block `slot` of a grid with rows / ROWS + clouds + 1 blocks: cloud b's blocks start at
