@@ -155,8 +155,8 @@ static int launch_forward(const AttentionCall& a, void* out, float* lse, char* w
 
 int tc_forward(const AttentionCall& a, void* out, float* lse, char* ws, cudaStream_t s) {
     if (a.is_bf16)
-        return a.size <= 64 ? launch_forward<1, 128, 1, 2, __nv_bfloat16>(a, out, lse, ws, s) : launch_forward<2, 128, 1, 2, __nv_bfloat16>(a, out, lse, ws, s);
-    return a.size <= 64 ? launch_forward<1, 64, 3, 1, float>(a, out, lse, ws, s) : launch_forward<2, 64, 3, 1, float>(a, out, lse, ws, s);
+        return a.size <= 64 ? launch_forward<1, 128, 1, 2, __nv_bfloat16>(a, out, lse, ws, s) : launch_forward<2, 64, 1, 2, __nv_bfloat16>(a, out, lse, ws, s);
+    return a.size <= 64 ? launch_forward<1, 64, 3, 1, float>(a, out, lse, ws, s) : launch_forward<2, 32, 3, 1, float>(a, out, lse, ws, s);
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------

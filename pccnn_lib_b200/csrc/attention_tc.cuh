@@ -42,8 +42,8 @@ struct TcControl {
 };
 
 struct TcShared {
-    uint64_t fixed_full, fixed_full2, full[kTcMaxStages], full2[kTcMaxStages], empty[kTcMaxStages], s_full[2], e_ready[2], all_done,
-        drained, round_done, acc_free;
+    uint64_t fixed_full, fixed_full2, full[kTcMaxStages], full2[kTcMaxStages], empty[kTcMaxStages], s_full[2], s_free[2], e_ready[2],
+        e_done[2], all_done, drained, round_done, acc_free;
     uint32_t tmem;
     int failed;
 };
@@ -254,7 +254,9 @@ __device__ __forceinline__ uint32_t tc_begin(TcShared* sh, int stages) {
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh->s_full[i], 1);
+            mbar_init(&sh->s_free[i], 128);
             mbar_init(&sh->e_ready[i], 128);
+            mbar_init(&sh->e_done[i], 1);
         }
         mbar_init(&sh->all_done, 1);
         mbar_init(&sh->drained, 1);
@@ -312,16 +314,20 @@ __device__ __forceinline__ void tc_drain_loads(TcShared* sh, int issued, int sta
 // accumulator anew and the thread of a row adds the units up in registers, rounding to nearest.
 // The accumulator is scaled only when the maximum has grown by more than 2^8 since it was last scaled: the probabilities
 // stay below 2^8, and the final division is by a sum relative to the same reference.
+// The logits and the probabilities have columns of their own: once the rows have been read into registers the logits of the
+// group's next unit can be computed, while this unit's probabilities are still being made.
 template <int GR, int BN, int NP, int QT>
 struct TcForward {
     static constexpr int kQ = QT * NP * GR * kTcRows * 128;
     static constexpr int kSlot = NP * GR * BN * 128;
     static constexpr int kFit = (200 * 1024 - kQ) / kSlot;
-    static constexpr int kStages = kFit > 6 ? 6 : kFit;
-    static constexpr int kBuffer = NP == 1 ? BN : (BN * 3 / 2 > BN ? BN * 3 / 2 : BN);  // logits, then the planes of the probabilities
+    static constexpr int kStages = kFit > kTcMaxStages ? kTcMaxStages : kFit;
+    static constexpr int kWeights = 2 * BN;             // columns of the probabilities, behind the logits of both groups
+    static constexpr int kWeightCols = NP * (BN / 2);   // of one group
+    static constexpr int kAcc = kWeights + 2 * kWeightCols;
     static constexpr int kBytes = kQ + kStages * kSlot + 1024 + 512;
     static_assert(QT == 1 || NP == 1, "two query tiles are loaded as one plane");
-    static_assert(kStages >= 2 && 2 * kBuffer + 2 * GR * 64 <= 512, "does not fit");
+    static_assert(kStages >= 4 && kAcc + 2 * GR * 64 <= 512, "does not fit");
     static_assert(kTcRows * GR * 64 * 4 + 2 * kTcRows * 4 <= kQ + kStages * kSlot, "no room to join the two groups");
 };
 
@@ -371,7 +377,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const int tiles = (int)((end - begin + BN - 1) / BN), q_tiles = rows_here > kTcRows ? 2 : 1, units = tiles * q_tiles;
     const int last_valid = (int)(end - begin) - (tiles - 1) * BN;
     const int steps = (a.size + 15) >> 4, n_out = steps * 16;
-    const uint32_t acc = tmem + 2 * Cfg::kBuffer;  // accumulator of group w: acc + w * GR * 64
+    const uint32_t acc = tmem + Cfg::kAcc;  // accumulator of group w: acc + w * GR * 64
     volatile int* failed = &sh->failed;
     const uint32_t limit = ctl.poll_limit;
 
@@ -414,36 +420,24 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             }
             __syncwarp();
         }
-        // one query tile: K0 K1 V0 K2 V1 ... ; two: K0 V0 K1 V1 ...
-        const int loads = 2 * tiles;
+        // the logits run ahead by two units: K0 K1 V0 K2 V1 ... for two query tiles, K0 K1 K2 V0 K3 V1 ... for one
+        const int loads = 2 * tiles, ahead = min(tiles, q_tiles == 2 ? 1 : 2);
         for (; issued < loads; ++issued) {
             const int it = issued;
             if (ctl.withhold_from >= 0 && it >= ctl.withhold_from) ok = false;
             const int s = it % kStages;
             if (ok && it >= kStages) ok = tc_wait_warp(&sh->empty[s], (it / kStages - 1) & 1, limit, failed);
             if (!ok) break;
-            bool is_value;
-            int j;
-            if (q_tiles == 2 || tiles == 1) {
-                is_value = it & 1;
-                j = it >> 1;
-            } else if (it == 0) {
-                is_value = false;
-                j = 0;
-            } else if (it == loads - 1) {
-                is_value = true;
-                j = tiles - 1;
-            } else {
-                is_value = !(it & 1);
-                j = is_value ? it / 2 - 1 : it / 2 + 1;
-            }
+            const int pair = (it - ahead) >> 1;
+            const bool rest = it >= ahead && pair >= tiles - ahead, is_value = rest || (it >= ahead && ((it - ahead) & 1));
+            const int j = it < ahead ? it : rest ? it - tiles : is_value ? pair : ahead + pair;
             const int valid = j == tiles - 1 ? last_valid : BN;
             if (is_value) tc_load_tile<BN, NP, GR>(ring + s * Cfg::kSlot, &map_v, rows_v, a.num_keys, kv, begin + (int64_t)j * BN, valid, a.size, &sh->full[s]);
             else tc_load_tile<BN, NP, GR>(ring + s * Cfg::kSlot, &map_k, rows_k, a.num_keys, kv, begin + (int64_t)j * BN, valid, a.size, &sh->full[s]);
         }
         if (!ok && lane == 0) tc_fail(sh, ctl, 1);
     } else if (warp == 9) {
-        // ---- products: logits of units 0 and 1, then (output of unit u, logits of unit u + 2)
+        // ---- products: logits of units 0 and 1, then (logits of unit u + 2, output of unit u)
         const bool leader = tc_elect();
         int used = 0, key_slot = 0, value_slot = 0;
         auto take = [&](int& slot) {  // the next tile of the ring
@@ -456,9 +450,13 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         auto logits = [&](int u) {
             const bool first = q_tiles == 1 || !(u & 1), last = q_tiles == 1 || (u & 1);
             if (first && !take(key_slot)) return false;
+            if (u >= 2) {  // the rows of unit u - 2 have been read
+                if (!tc_wait_warp(&sh->s_free[u & 1], ((u >> 1) - 1) & 1, limit, failed)) return false;
+                tc_fence_after();
+            }
             const int t = q_tiles == 2 ? u & 1 : 0;
             if (leader) {
-                tc_rows_by_rows<NP, GR, BN>(tmem + (u & 1) * Cfg::kBuffer, smem_u32(smem + t * NP * GR * kTcRows * 128),
+                tc_rows_by_rows<NP, GR, BN>(tmem + (u & 1) * BN, smem_u32(smem + t * NP * GR * kTcRows * 128),
                                             smem_u32(ring + key_slot * Cfg::kSlot), steps);
                 if (last) tc_commit(&sh->empty[key_slot]);
                 tc_commit(&sh->s_full[u & 1]);
@@ -473,9 +471,10 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             tc_fence_after();
             const int j = q_tiles == 2 ? u >> 1 : u, valid = j == tiles - 1 ? last_valid : BN;
             if (leader) {
-                tc_weights_by_rows<NP, GR, BN>(acc + (u & 1) * GR * 64, tmem + (u & 1) * Cfg::kBuffer,
+                tc_weights_by_rows<NP, GR, BN>(acc + (u & 1) * GR * 64, tmem + Cfg::kWeights + (u & 1) * Cfg::kWeightCols,
                                                smem_u32(ring + value_slot * Cfg::kSlot), n_out, (valid + 15) >> 4, NP == 1 && u >= 2);
                 if (last) tc_commit(&sh->empty[value_slot]);
+                tc_commit(&sh->e_done[u & 1]);
             }
             __syncwarp();
             return true;
@@ -483,7 +482,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         bool ok = tc_wait_warp(&sh->fixed_full, 0, limit, failed);
         tc_fence_after();
         ok = ok && logits(0) && (units < 2 || logits(1));
-        for (int u = 0; u < units && ok; ++u) ok = weigh(u) && (u + 2 >= units || logits(u + 2));
+        for (int u = 0; u < units && ok; ++u) ok = (u + 2 >= units || logits(u + 2)) && weigh(u);
         tc_finish_products(sh, ctl, ok, leader);
     }
 
@@ -497,7 +496,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     bool ok = true;
     if (warp < 8) {
         // ---- element-wise: logits to probabilities
-        const uint32_t buf = tmem + lanes + group * Cfg::kBuffer, my_acc = acc + lanes + group * GR * 64;
+        const uint32_t buf = tmem + lanes + group * BN, my_acc = acc + lanes + group * GR * 64;
+        const uint32_t weights = tmem + lanes + Cfg::kWeights + group * Cfg::kWeightCols;
         for (int u = group; u < units; u += 2) {
             if (!(ok = tc_wait_warp(&sh->s_full[group], (u >> 1) & 1, limit, failed))) break;
             tc_fence_after();
@@ -505,6 +505,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             uint32_t s[BN / 32][32];
 #pragma unroll
             for (int i = 0; i < BN / 32; ++i) tc_ld_32x32(buf + 32 * i, s[i]);
+            tc_fence_before();
+            mbar_arrive(&sh->s_free[group]);
             if (valid < BN) {  // columns behind the cloud repeat the first one, which changes no maximum
 #pragma unroll
                 for (int i = 0; i < BN; ++i)
@@ -521,6 +523,10 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 m[0] = fminf(fminf(m[0], m[1]), fminf(m[2], m[3]));
             }
             const float top = m[0] * c2;
+            if (u >= 2) {  // the group's last unit has been added: its accumulator and its columns of probabilities are free
+                if (!(ok = tc_wait_warp(&sh->e_done[group], ((u >> 1) - 1) & 1, limit, failed))) break;
+                tc_fence_after();
+            }
             if constexpr (NP == 3) {
                 if (u >= 2) tc_add_columns<GR * 64>(my_acc, n_out, kept);
             }
@@ -557,7 +563,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
                 for (int e = 0; e < 32; ++e) sum[e & 3] += p[e];
                 // rounded to bf16 (NP = 1) only as the weights of the values; their sum is taken before
-                tc_store_weights<NP, BN / 2>(buf + 16 * i, p);
+                tc_store_weights<NP, BN / 2>(weights + 16 * i, p);
             }
             total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tc_wait_st();
@@ -655,19 +661,22 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 // Two kernels, each recomputing the logits, instead of one that adds dQ with atomics: every sum is taken in a fixed order.
 template <bool KEYS, int GR, int NP>
 struct TcBackward {
-    static constexpr int kBN = 64;
+    // streamed rows of a unit: as many as leave columns for s, t, the weights and the accumulators, and three slots of the ring (a
+    // slot is held until its unit has been added, and the logits run ahead by two units)
+    static constexpr int kBN = NP == 3 || (KEYS && GR == 2) ? 32 : 64;
     static constexpr int kFixed = NP * GR * kTcRows * 128;   // one of the two tiles that stay
     static constexpr int kTile = NP * GR * kBN * 128;        // one of the two tiles of a slot
     static constexpr int kFit = (200 * 1024 - 2 * kFixed) / (2 * kTile);
-    static constexpr int kStages = kFit > 5 ? 5 : kFit;
+    static constexpr int kStages = kFit > kTcMaxStages ? kTcMaxStages : kFit;
     static constexpr int kPlane = kBN / 2;
-    static constexpr int kBuffer = NP == 3 && KEYS ? 2 * NP * kPlane : 2 * kBN;  // s and t; then the planes of e, and those of p
-    static constexpr int kWeights = NP * kPlane;                                 // p's columns behind e's
+    static constexpr int kWeights = 4 * kBN;                                     // columns of the weights, behind s and t of both groups
+    static constexpr int kWeightCols = (KEYS ? 2 : 1) * NP * kPlane;             // of one group: e, then p
+    static constexpr int kAccStart = kWeights + 2 * kWeightCols;
     static constexpr int kAcc = GR * 64;
-    static constexpr int kRound = 2;                                             // even: both groups have units in a round
+    static constexpr int kRound = 4;                                             // even: both groups have units in a round
     static constexpr int kKept = NP == 3 ? (KEYS ? kAcc : kAcc / 2) : 1;         // columns that a thread adds up in registers
     static constexpr int kBytes = 2 * kFixed + kStages * (2 * kTile + 2 * kBN * 4) + 1024 + 512;
-    static_assert(kStages >= 2 && 2 * kBuffer + (KEYS ? 2 : 1) * kAcc <= 512 && kBytes <= 227 * 1024, "does not fit");
+    static_assert(kStages >= 3 && kAccStart + (KEYS ? 2 : 1) * kAcc <= 512 && kBytes <= 227 * 1024, "does not fit");
 };
 
 template <bool KEYS, int GR, int NP, class T>
@@ -725,7 +734,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
     const int tiles = (int)((end - begin + BN - 1) / BN), units = tiles * (KEYS ? share : 1);
     const int last_valid = (int)(end - begin) - (tiles - 1) * BN;
     const int steps = (a.size + 15) >> 4, n_out = steps * 16;
-    const uint32_t acc = tmem + 2 * Cfg::kBuffer;
+    const uint32_t acc = tmem + Cfg::kAccStart;
     volatile int* failed = &sh->failed;
     const uint32_t limit = ctl.poll_limit;
     const float c2 = a.scale * kLog2e;
@@ -761,13 +770,14 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
         if (!ok && lane == 0) tc_fail(sh, ctl, 1);
     } else if (warp == 9) {
         const bool leader = tc_elect();
-        // ---- products: logits of units 0 and 1, then (sums of unit u, logits of unit u + 2)
+        // ---- products: logits of units 0 and 1, then (logits of unit u + 2, sums of unit u)
         auto logits = [&](int u) {
             const int s = u % kStages;
             if (!tc_wait_warp(&sh->full[s], (u / kStages) & 1, limit, failed)) return false;
             if (!tc_wait_warp(&sh->full2[s], (u / kStages) & 1, limit, failed)) return false;
+            if (u >= 2 && !tc_wait_warp(&sh->s_free[u & 1], ((u >> 1) - 1) & 1, limit, failed)) return false;
             tc_fence_after();
-            const uint32_t buf = tmem + (u & 1) * Cfg::kBuffer, slot = smem_u32(ring + s * 2 * Cfg::kTile);
+            const uint32_t buf = tmem + (u & 1) * 2 * BN, slot = smem_u32(ring + s * 2 * Cfg::kTile);
             if (leader) {
                 tc_rows_by_rows<NP, GR, BN>(buf, smem_u32(smem), slot, steps);
                 tc_rows_by_rows<NP, GR, BN>(buf + BN, smem_u32(smem + Cfg::kFixed), slot + Cfg::kTile, steps);
@@ -782,12 +792,14 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
             if (u > 0 && fresh && !tc_wait_warp(&sh->acc_free, (u / Cfg::kRound - 1) & 1, limit, failed)) return false;
             tc_fence_after();
             const int s = u % kStages, valid = u % tiles == tiles - 1 ? last_valid : BN;
-            const uint32_t buf = tmem + (u & 1) * Cfg::kBuffer, slot = smem_u32(ring + s * 2 * Cfg::kTile);
+            const uint32_t weights = tmem + Cfg::kWeights + (u & 1) * Cfg::kWeightCols, slot = smem_u32(ring + s * 2 * Cfg::kTile);
             if (leader) {
-                tc_weights_by_rows<NP, GR, BN>(acc, buf, slot, n_out, (valid + 15) >> 4, !fresh);
+                tc_weights_by_rows<NP, GR, BN>(acc, weights, slot, n_out, (valid + 15) >> 4, !fresh);
                 if (KEYS)
-                    tc_weights_by_rows<NP, GR, BN>(acc + Cfg::kAcc, buf + Cfg::kWeights, slot + Cfg::kTile, n_out, (valid + 15) >> 4, !fresh);
+                    tc_weights_by_rows<NP, GR, BN>(acc + Cfg::kAcc, weights + NP * Cfg::kPlane, slot + Cfg::kTile, n_out, (valid + 15) >> 4,
+                                                   !fresh);
                 tc_commit(&sh->empty[s]);
+                tc_commit(&sh->e_done[u & 1]);
                 if (NP == 3 && (u + 1) % Cfg::kRound == 0 && u + 1 < units) tc_commit(&sh->round_done);
             }
             __syncwarp();
@@ -796,7 +808,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
         bool ok = tc_wait_warp(&sh->fixed_full, 0, limit, failed) && tc_wait_warp(&sh->fixed_full2, 0, limit, failed);
         tc_fence_after();
         ok = ok && logits(0) && (units < 2 || logits(1));
-        for (int u = 0; u < units && ok; ++u) ok = weigh(u) && (u + 2 >= units || logits(u + 2));
+        for (int u = 0; u < units && ok; ++u) ok = (u + 2 >= units || logits(u + 2)) && weigh(u);
         tc_finish_products(sh, ctl, ok, leader);
     }
 
@@ -811,7 +823,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
     if (warp < 8) {
         // ---- element-wise
         bool ok = true;
-        const uint32_t buf = tmem + lanes + group * Cfg::kBuffer;
+        const uint32_t buf = tmem + lanes + group * 2 * BN, weights = tmem + lanes + Cfg::kWeights + group * Cfg::kWeightCols;
         int emptied = 0;
         auto empty_until = [&](int round) {  // the accumulators of the rounds before `round` into registers
             if constexpr (NP == 3) {
@@ -844,6 +856,12 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                 tc_ld_32x32(buf + 32 * i, s[i]);
                 tc_ld_32x32(buf + BN + 32 * i, t[i]);
             }
+            tc_fence_before();
+            mbar_arrive(&sh->s_free[group]);
+            if (u >= 2) {  // the group's last unit has been added: its columns of weights are free
+                if (!(ok = tc_wait_warp(&sh->e_done[group], ((u >> 1) - 1) & 1, limit, failed))) break;
+                tc_fence_after();
+            }
 #pragma unroll
             for (int i = 0; i < BN / 32; ++i) {
                 float p[32], e[32];
@@ -869,8 +887,8 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                         if (i * 32 + c >= valid) e[c] = 0.f;  // a key behind the cloud: its probability may overflow
                 }
                 // rounded to bf16 (NP = 1) as the weights of the last two products, as the probabilities of the forward pass
-                tc_store_weights<NP, Cfg::kPlane>(buf + 16 * i, e);
-                if (KEYS) tc_store_weights<NP, Cfg::kPlane>(buf + Cfg::kWeights + 16 * i, p);
+                tc_store_weights<NP, Cfg::kPlane>(weights + 16 * i, e);
+                if (KEYS) tc_store_weights<NP, Cfg::kPlane>(weights + NP * Cfg::kPlane + 16 * i, p);
             }
             tc_wait_st();
             tc_fence_before();
