@@ -140,15 +140,17 @@ static int launch_forward(const AttentionCall& a, void* out, float* lse, char* w
     if (int rc = tc_operand(q, a.q, a.num_queries, a.heads, a.size, NP == 3, ws, s)) return rc;
     if (int rc = tc_operand(k, a.k, a.num_keys, a.kv_heads, a.size, NP == 3, ws, s)) return rc;
     if (int rc = tc_operand(v, a.v, a.num_keys, a.kv_heads, a.size, NP == 3, ws, s)) return rc;
-    CUtensorMap map_q, map_k, map_v;
+    CUtensorMap map_q, map_k, map_v, map_k8, map_v8;
     if (int rc = operand_map(&map_q, q, a.size, NP == 3, kTcRows)) return rc;
     if (int rc = operand_map(&map_k, k, a.size, NP == 3, BN)) return rc;
     if (int rc = operand_map(&map_v, v, a.size, NP == 3, BN)) return rc;
+    if (int rc = operand_map(&map_k8, k, a.size, NP == 3, 8)) return rc;
+    if (int rc = operand_map(&map_v8, v, a.size, NP == 3, 8)) return rc;
     const int splits = tc_forward_splits(a);
     float2* stat = (float2*)ws;
     float* part = (float*)(ws + align_up((size_t)splits * a.num_queries * a.heads * sizeof(float2)));
     const dim3 grid((unsigned)tc_blocks(a.num_queries, QT * kTcRows, a.clouds), (unsigned)a.heads, (unsigned)splits);
-    kernel<<<grid, kTcThreads, Cfg::kBytes, s>>>(map_q, map_k, map_v, a, q.rows, k.rows, v.rows, splits, (T*)out, lse, part, stat, ctl);
+    kernel<<<grid, kTcThreads, Cfg::kBytes, s>>>(map_q, map_k, map_v, map_k8, map_v8, a, k.rows, v.rows, splits, (T*)out, lse, part, stat, ctl);
     PCCNN_LAUNCH_CHECK();
     return splits > 1 ? join_splits(a, splits, part, stat, out, lse, s) : PCCNN_OK;
 }
@@ -190,17 +192,19 @@ static int launch_grads(const AttentionCall& a, const TcOperand& f1, const TcOpe
     if (int rc = allow_shared(kernel, Cfg::kBytes, done)) return rc;
     TcControl ctl;
     if (int rc = tc_control(ctl)) return rc;
-    CUtensorMap m[4];
+    CUtensorMap m[6];
     if (int rc = operand_map(&m[0], f1, a.size, NP == 3, kTcRows)) return rc;
     if (int rc = operand_map(&m[1], f2, a.size, NP == 3, kTcRows)) return rc;
     if (int rc = operand_map(&m[2], y1, a.size, NP == 3, Cfg::kBN)) return rc;
     if (int rc = operand_map(&m[3], y2, a.size, NP == 3, Cfg::kBN)) return rc;
+    if (int rc = operand_map(&m[4], y1, a.size, NP == 3, 8)) return rc;
+    if (int rc = operand_map(&m[5], y2, a.size, NP == 3, 8)) return rc;
     const int64_t rows = KEYS ? a.num_keys : a.num_queries;
     const int heads = KEYS ? a.kv_heads : a.heads, splits = tc_grad_splits(a, KEYS);
     const int64_t count = rows * heads * a.size;
     float* part = (float*)ws;
     const dim3 grid((unsigned)tc_blocks(rows, kTcRows, a.clouds), (unsigned)heads, (unsigned)splits);
-    kernel<<<grid, kTcThreads, Cfg::kBytes, s>>>(m[0], m[1], m[2], m[3], a, f1.rows, f2.rows, y1.rows, y2.rows, splits, lse, delta, (T*)out1,
+    kernel<<<grid, kTcThreads, Cfg::kBytes, s>>>(m[0], m[1], m[2], m[3], m[4], m[5], a, y1.rows, y2.rows, splits, lse, delta, (T*)out1,
                                                  (T*)out2, part, part + splits * count, ctl);
     PCCNN_LAUNCH_CHECK();
     if (splits > 1) {

@@ -5,8 +5,8 @@
 // 24 bits, and a product is the six plane products h h + h m + m h + m m + h l + l h in one fp32 accumulator (the dropped
 // ones are below 2^-24 of it).
 //
-// A tile that ends inside a cloud is not loaded by TMA but row by row, with zeros behind the cloud's last row: the rows that
-// follow belong to another cloud and may hold infinities, which would reach this one as 0 * inf.
+// A streamed tile in which the cloud ends gets zeros behind the cloud's last row: the rows that follow belong to another cloud
+// and may hold infinities, which would reach this one as 0 * inf.
 //
 // Roles of the ten warps of a CTA: two groups of four warps do the element-wise work (one row of a 128-row tile per thread,
 // which is one lane of tensor memory), warp 8 loads, an elected lane of warp 9 issues the products.  The element-wise groups work
@@ -70,6 +70,13 @@ __device__ __forceinline__ bool tc_wait_warp(uint64_t* bar, uint32_t parity, uin
     return false;
 }
 
+// One arrival for a warp, behind the tensor-memory accesses of all its lanes.
+__device__ __forceinline__ void tc_arrive_warp(uint64_t* bar) {
+    tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
 // The cloud of block `slot` of a grid with rows / ROWS + clouds + 1 blocks: cloud b's blocks start at
 // begin(b) / ROWS + b, which leaves room for all of them without a prefix sum.  Cloud `clouds` is the rest of the rows.
 // All lanes of a warp search together.  Returns false for a block without rows.
@@ -93,29 +100,35 @@ __device__ __forceinline__ bool tc_block_rows(const int32_t* __restrict__ ends, 
 }
 
 // ---- loads ------------------------------------------------------------------------------------------------------
-// R rows from row0 of `head` into the tile at dst ([plane][64 features][R rows]); `valid` of them belong to the cloud.
-// Called by a whole warp; completes one phase of `bar`.
+// R rows from row0 of `head` into the tile at dst ([plane][64 features][R rows]), by one thread; completes `bytes` of `bar`.
 template <int R, int NP, int GR>
-__device__ __forceinline__ void tc_load_tile(uint8_t* dst, const CUtensorMap* map, const TcRows& src, int64_t plane_rows, int head,
-                                             int64_t row0, int valid, int size, uint64_t* bar) {
+__device__ __forceinline__ void tc_load_whole(uint8_t* dst, const CUtensorMap* map, int64_t plane_rows, int head, int64_t row0, uint64_t* bar) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int g = 0; g < GR; ++g) tma_load_3d(dst + (p * GR + g) * R * 128, map, bar, g * 64, head, (int)(p * plane_rows + row0));
+}
+
+// The same for a streamed tile of which only the first `valid` rows belong to the cloud, with zeros behind them.  Called by a
+// whole warp; completes one phase of `bar`.  A tile that ends inside the cloud takes boxes of eight rows (map8) as far as they
+// go and at most seven rows through registers.
+template <int R, int NP, int GR>
+__device__ __forceinline__ void tc_load_tile(uint8_t* dst, const CUtensorMap* map, const CUtensorMap* map8, const TcRows& src,
+                                             int64_t plane_rows, int head, int64_t row0, int valid, int size, uint64_t* bar) {
     const int lane = threadIdx.x & 31;
     if (valid >= R) {
         if (lane == 0) {
             mbar_expect_tx(bar, NP * GR * R * 128);
-#pragma unroll
-            for (int p = 0; p < NP; ++p)
-#pragma unroll
-                for (int g = 0; g < GR; ++g)
-                    tma_load_3d(dst + (p * GR + g) * R * 128, map, bar, g * 64, head, (int)(p * plane_rows + row0));
+            tc_load_whole<R, NP, GR>(dst, map, plane_rows, head, row0, bar);
         }
     } else {
-        const int chunks = size >> 3;
+        const int chunks = size >> 3, boxed = valid & ~7;
 #pragma unroll 1
         for (int pg = 0; pg < NP * GR; ++pg) {
             const int p = pg / GR, g = pg % GR;
             const __nv_bfloat16* from = src.data + p * src.plane + row0 * src.row + head * src.head + g * 64;
-#pragma unroll 8
-            for (int i = lane; i < R * 8; i += 32) {
+#pragma unroll 4
+            for (int i = boxed * 8 + lane; i < R * 8; i += 32) {
                 const int r = i >> 3, c = i & 7;
                 uint4 v = make_uint4(0, 0, 0, 0);
                 if (r < valid && g * 8 + c < chunks) v = *reinterpret_cast<const uint4*>(from + r * src.row + c * 8);
@@ -124,7 +137,12 @@ __device__ __forceinline__ void tc_load_tile(uint8_t* dst, const CUtensorMap* ma
         }
         fence_smem_to_async_proxy();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar);
+        if (lane == 0) {
+            mbar_expect_tx(bar, NP * GR * boxed * 128);
+            for (int pg = 0; pg < NP * GR; ++pg)
+                for (int r = 0; r < boxed; r += 8)
+                    tma_load_3d(dst + pg * R * 128 + r * 128, map8, bar, (pg % GR) * 64, head, (int)((pg / GR) * plane_rows + row0 + r));
+        }
     }
     __syncwarp();
 }
@@ -254,14 +272,14 @@ __device__ __forceinline__ uint32_t tc_begin(TcShared* sh, int stages) {
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh->s_full[i], 1);
-            mbar_init(&sh->s_free[i], 128);
-            mbar_init(&sh->e_ready[i], 128);
+            mbar_init(&sh->s_free[i], 4);  // the four warps of a group
+            mbar_init(&sh->e_ready[i], 4);
             mbar_init(&sh->e_done[i], 1);
         }
         mbar_init(&sh->all_done, 1);
         mbar_init(&sh->drained, 1);
         mbar_init(&sh->round_done, 1);
-        mbar_init(&sh->acc_free, 256);
+        mbar_init(&sh->acc_free, 8);
         sh->failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -334,7 +352,8 @@ struct TcForward {
 template <int GR, int BN, int NP, int QT, class T>
 __global__ void __launch_bounds__(kTcThreads, 1)
 attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                    const __grid_constant__ CUtensorMap map_v, AttentionCall a, TcRows rows_q, TcRows rows_k, TcRows rows_v, int splits,
+                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_k8,
+                    const __grid_constant__ CUtensorMap map_v8, AttentionCall a, TcRows rows_k, TcRows rows_v, int splits,
                     T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part_out, float2* __restrict__ part_stat,
                     TcControl ctl) {
     using Cfg = TcForward<GR, BN, NP, QT>;
@@ -385,41 +404,13 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     if (warp == 8) {
         // ---- loader: the tiles in the order in which the products use them
         bool ok = true;
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            // both tiles complete the one phase of fixed_full, which the products wait for
-            const int valid = rows_here - t * kTcRows;
-            if (t < q_tiles && q_tiles == 1) tc_load_tile<kTcRows, NP, GR>(smem, &map_q, rows_q, a.num_queries, h, row0, valid, a.size, &sh->fixed_full);
+        // rows behind the cloud's last query are other clouds' (or zeros): each of them only reaches its own row of the products
+        if (lane == 0) {
+            mbar_expect_tx(&sh->fixed_full, q_tiles * NP * GR * kTcRows * 128);
+            for (int t = 0; t < q_tiles; ++t)
+                tc_load_whole<kTcRows, NP, GR>(smem + t * NP * GR * kTcRows * 128, &map_q, a.num_queries, h, row0 + t * kTcRows, &sh->fixed_full);
         }
-        if (QT == 2 && q_tiles == 2) {
-            // the first tile is whole; the second may end inside the cloud
-            const int valid = rows_here - kTcRows;
-            if (valid < kTcRows) {
-                // written by the warp first, so that the one arrival (with the first tile's bytes) covers it
-                const int chunks = a.size >> 3;
-#pragma unroll 1
-                for (int g = 0; g < GR; ++g) {
-                    const __nv_bfloat16* from = rows_q.data + (row0 + kTcRows) * rows_q.row + h * rows_q.head + g * 64;
-#pragma unroll 8
-                    for (int i = lane; i < kTcRows * 8; i += 32) {
-                        const int r = i >> 3, c = i & 7;
-                        uint4 v = make_uint4(0, 0, 0, 0);
-                        if (r < valid && g * 8 + c < chunks) v = *reinterpret_cast<const uint4*>(from + r * rows_q.row + c * 8);
-                        *reinterpret_cast<uint4*>(smem + (GR + g) * kTcRows * 128 + sw128_offset(r, c)) = v;
-                    }
-                }
-                fence_smem_to_async_proxy();
-                __syncwarp();
-            }
-            if (lane == 0) {
-                mbar_expect_tx(&sh->fixed_full, (valid < kTcRows ? 1 : 2) * GR * kTcRows * 128);
-                for (int t = 0; t < (valid < kTcRows ? 1 : 2); ++t)
-#pragma unroll
-                    for (int g = 0; g < GR; ++g)
-                        tma_load_3d(smem + (t * GR + g) * kTcRows * 128, &map_q, &sh->fixed_full, g * 64, h, (int)(row0 + t * kTcRows));
-            }
-            __syncwarp();
-        }
+        __syncwarp();
         // the logits run ahead by two units: K0 K1 V0 K2 V1 ... for two query tiles, K0 K1 K2 V0 K3 V1 ... for one
         const int loads = 2 * tiles, ahead = min(tiles, q_tiles == 2 ? 1 : 2);
         for (; issued < loads; ++issued) {
@@ -432,8 +423,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const bool rest = it >= ahead && pair >= tiles - ahead, is_value = rest || (it >= ahead && ((it - ahead) & 1));
             const int j = it < ahead ? it : rest ? it - tiles : is_value ? pair : ahead + pair;
             const int valid = j == tiles - 1 ? last_valid : BN;
-            if (is_value) tc_load_tile<BN, NP, GR>(ring + s * Cfg::kSlot, &map_v, rows_v, a.num_keys, kv, begin + (int64_t)j * BN, valid, a.size, &sh->full[s]);
-            else tc_load_tile<BN, NP, GR>(ring + s * Cfg::kSlot, &map_k, rows_k, a.num_keys, kv, begin + (int64_t)j * BN, valid, a.size, &sh->full[s]);
+            if (is_value) tc_load_tile<BN, NP, GR>(ring + s * Cfg::kSlot, &map_v, &map_v8, rows_v, a.num_keys, kv, begin + (int64_t)j * BN, valid, a.size, &sh->full[s]);
+            else tc_load_tile<BN, NP, GR>(ring + s * Cfg::kSlot, &map_k, &map_k8, rows_k, a.num_keys, kv, begin + (int64_t)j * BN, valid, a.size, &sh->full[s]);
         }
         if (!ok && lane == 0) tc_fail(sh, ctl, 1);
     } else if (warp == 9) {
@@ -498,6 +489,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         // ---- element-wise: logits to probabilities
         const uint32_t buf = tmem + lanes + group * BN, my_acc = acc + lanes + group * GR * 64;
         const uint32_t weights = tmem + lanes + Cfg::kWeights + group * Cfg::kWeightCols;
+        const bool live = (q_tiles == 2 ? group * kTcRows : 0) + row < rows_here;  // a row behind the cloud may hold anything
         for (int u = group; u < units; u += 2) {
             if (!(ok = tc_wait_warp(&sh->s_full[group], (u >> 1) & 1, limit, failed))) break;
             tc_fence_after();
@@ -505,8 +497,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             uint32_t s[BN / 32][32];
 #pragma unroll
             for (int i = 0; i < BN / 32; ++i) tc_ld_32x32(buf + 32 * i, s[i]);
-            tc_fence_before();
-            mbar_arrive(&sh->s_free[group]);
+            tc_arrive_warp(&sh->s_free[group]);
             if (valid < BN) {  // columns behind the cloud repeat the first one, which changes no maximum
 #pragma unroll
                 for (int i = 0; i < BN; ++i)
@@ -530,7 +521,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             if constexpr (NP == 3) {
                 if (u >= 2) tc_add_columns<GR * 64>(my_acc, n_out, kept);
             }
-            if (__any_sync(kFullMask, !(top <= base + 8.f))) {
+            if (__any_sync(kFullMask, live && !(top <= base + 8.f))) {
                 const float now = fmaxf(base, top), fade = exp2_fast(base - (now == -INFINITY ? 0.f : now));
                 base = now;
                 total *= fade;
@@ -567,8 +558,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             }
             total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tc_wait_st();
-            tc_fence_before();
-            mbar_arrive(&sh->e_ready[group]);
+            tc_arrive_warp(&sh->e_ready[group]);
         }
         if (ok && group < units) {
             ok = tc_wait_warp(&sh->all_done, 0, limit, failed);
@@ -682,8 +672,9 @@ struct TcBackward {
 template <bool KEYS, int GR, int NP, class T>
 __global__ void __launch_bounds__(kTcThreads, 1)
 attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __grid_constant__ CUtensorMap map_f2,
-                          const __grid_constant__ CUtensorMap map_y1, const __grid_constant__ CUtensorMap map_y2, AttentionCall a,
-                          TcRows rows_f1, TcRows rows_f2, TcRows rows_y1, TcRows rows_y2, int splits, const float* __restrict__ lse,
+                          const __grid_constant__ CUtensorMap map_y1, const __grid_constant__ CUtensorMap map_y2,
+                          const __grid_constant__ CUtensorMap map_y18, const __grid_constant__ CUtensorMap map_y28, AttentionCall a,
+                          TcRows rows_y1, TcRows rows_y2, int splits, const float* __restrict__ lse,
                           const float* __restrict__ delta, T* __restrict__ out1, T* __restrict__ out2, float* __restrict__ part1,
                           float* __restrict__ part2, TcControl ctl) {
     using Cfg = TcBackward<KEYS, GR, NP>;
@@ -743,8 +734,13 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
     if (warp == 8) {
         // ---- loader: a barrier for each of the two tiles that stay, and for each tile of a slot
         bool ok = true;
-        tc_load_tile<kTcRows, NP, GR>(smem, &map_f1, rows_f1, num_rows, head, row0, rows_here, a.size, &sh->fixed_full);
-        tc_load_tile<kTcRows, NP, GR>(smem + Cfg::kFixed, &map_f2, rows_f2, num_rows, head, row0, rows_here, a.size, &sh->fixed_full2);
+        if (lane == 0) {  // rows behind the cloud's last one: see the forward kernel
+            mbar_expect_tx(&sh->fixed_full, Cfg::kFixed);
+            tc_load_whole<kTcRows, NP, GR>(smem, &map_f1, num_rows, head, row0, &sh->fixed_full);
+            mbar_expect_tx(&sh->fixed_full2, Cfg::kFixed);
+            tc_load_whole<kTcRows, NP, GR>(smem + Cfg::kFixed, &map_f2, num_rows, head, row0, &sh->fixed_full2);
+        }
+        __syncwarp();
         for (; issued < units; ++issued) {
             if (ctl.withhold_from >= 0 && issued >= ctl.withhold_from) ok = false;
             const int s = issued % kStages;
@@ -764,8 +760,8 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                 }
                 __syncwarp();
             }
-            tc_load_tile<BN, NP, GR>(slot, &map_y1, rows_y1, num_stream, h, from, valid, a.size, &sh->full[s]);
-            tc_load_tile<BN, NP, GR>(slot + Cfg::kTile, &map_y2, rows_y2, num_stream, h, from, valid, a.size, &sh->full2[s]);
+            tc_load_tile<BN, NP, GR>(slot, &map_y1, &map_y18, rows_y1, num_stream, h, from, valid, a.size, &sh->full[s]);
+            tc_load_tile<BN, NP, GR>(slot + Cfg::kTile, &map_y2, &map_y28, rows_y2, num_stream, h, from, valid, a.size, &sh->full2[s]);
         }
         if (!ok && lane == 0) tc_fail(sh, ctl, 1);
     } else if (warp == 9) {
@@ -831,8 +827,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                     if (!(ok = tc_wait_warp(&sh->round_done, emptied & 1, limit, failed))) break;
                     tc_fence_after();
                     tc_add_columns<Cfg::kKept>(my_acc, my_columns, kept);
-                    tc_fence_before();
-                    mbar_arrive(&sh->acc_free);
+                    tc_arrive_warp(&sh->acc_free);
                 }
             }
         };
@@ -856,8 +851,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                 tc_ld_32x32(buf + 32 * i, s[i]);
                 tc_ld_32x32(buf + BN + 32 * i, t[i]);
             }
-            tc_fence_before();
-            mbar_arrive(&sh->s_free[group]);
+            tc_arrive_warp(&sh->s_free[group]);
             if (u >= 2) {  // the group's last unit has been added: its columns of weights are free
                 if (!(ok = tc_wait_warp(&sh->e_done[group], ((u >> 1) - 1) & 1, limit, failed))) break;
                 tc_fence_after();
@@ -891,8 +885,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                 if (KEYS) tc_store_weights<NP, Cfg::kPlane>(weights + NP * Cfg::kPlane + 16 * i, p);
             }
             tc_wait_st();
-            tc_fence_before();
-            mbar_arrive(&sh->e_ready[group]);
+            tc_arrive_warp(&sh->e_ready[group]);
         }
         empty_until((units - 1) / Cfg::kRound);
         if (ok) {
