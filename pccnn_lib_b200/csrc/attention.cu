@@ -84,21 +84,54 @@ __device__ __forceinline__ void split_range(int64_t& begin, int64_t& end, int s,
     begin = lo < end ? lo : end;
 }
 
-// ---- forward: block = one query x GH heads that share keys x one split of the keys ------------------------------
+// ---- forward: block = one query x up to 8 key heads x one split of the keys -------------------------------------------
+// A warp serves one key head (and GH query heads that share it): with several key heads the warps of a block walk the same
+// rows side by side, so that a block reads whole rows; with fewer than eight the warps of a head take different keys.  A
+// lane has the next kUnroll keys and values in flight while it works on the last ones, as raw 16-byte vectors.
 // Without splits the output and lse are written; with splits the block leaves its unnormalised sum (relative to its own
 // maximum), the maximum and the sum of the probabilities.
+template <class T, int V> struct RawRow { uint4 v; };
+template <class T> struct RawRow<T, 1> { T v; };
+template <class T, int V>
+__device__ __forceinline__ void load_raw(RawRow<T, V>& r, const T* __restrict__ p) {
+    if constexpr (V == 1) r.v = *p;
+    else r.v = *reinterpret_cast<const uint4*>(p);
+}
+template <class T, int V>
+__device__ __forceinline__ void clear_raw(RawRow<T, V>& r) {
+    if constexpr (V == 1) r.v = from_float<T>(0.f);
+    else r.v = make_uint4(0, 0, 0, 0);
+}
+template <class T, int V>
+__device__ __forceinline__ void widen(const RawRow<T, V>& r, float (&x)[V]) {
+    if constexpr (V == 1) {
+        x[0] = to_float(r.v);
+    } else {
+        const uint32_t w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (V == 4) {
+                x[i] = __uint_as_float(w[i]);
+            } else {
+                x[2 * i] = __uint_as_float(w[i] << 16);
+                x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+    }
+}
+
 template <class T, int V, int NC, int GH>
 __global__ void __launch_bounds__(kRowThreads)
-attention_row_kernel(AttentionCall a, int lanes_per_row, int splits, T* __restrict__ out, float* __restrict__ lse,
+attention_row_kernel(AttentionCall a, int lanes_per_row, int warp_heads, int splits, T* __restrict__ out, float* __restrict__ lse,
                      float* __restrict__ part_out, float2* __restrict__ part_stat) {
     constexpr int kUnroll = NC * V * GH > 32 ? 2 : 4;
     __shared__ float scratch[kRowWarps * NC * 32 * V];
     __shared__ float stat[kRowWarps][2];
     const int64_t m = blockIdx.x;
     const int group = a.heads / a.kv_heads, parts = (group + GH - 1) / GH;
-    const int kv = blockIdx.y / parts, h0 = kv * group + (blockIdx.y % parts) * GH;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slices = kRowWarps / warp_heads, slice = warp / warp_heads;
+    const int kv = blockIdx.y / parts * warp_heads + warp % warp_heads, h0 = kv * group + (blockIdx.y % parts) * GH;
     const int heads_here = min(GH, (kv + 1) * group - h0), split = blockIdx.z;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int in_row = lane % lanes_per_row, sub = lane / lanes_per_row, per_warp = 32 / lanes_per_row;
 
     const int b = cloud_of_row(a.query_ends, a.clouds, m);
@@ -123,34 +156,49 @@ attention_row_kernel(AttentionCall a, int lanes_per_row, int splits, T* __restri
     }
     const T* keys = (const T*)a.k.data + kv * a.k.head;
     const T* values = (const T*)a.v.data + kv * a.v.head;
-    const int step = kRowWarps * per_warp;
-    for (int64_t first = begin + warp * per_warp; first < end; first += (int64_t)step * kUnroll) {  // the same for the warp's lanes
-        float s[GH][kUnroll], val[kUnroll][NC][V];
-        {
-            float key[kUnroll][NC][V];
+    const int step = slices * per_warp;
+    RawRow<T, V> key[kUnroll][NC], val[kUnroll][NC];
+    auto fetch = [&](int64_t first) {
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                const int64_t n = first + u * step + sub;
-                if (n < end) {
-                    load_row<T, V, NC>(keys + n * a.k.row, in_row, lanes_per_row, a.size, key[u]);
-                    load_row<T, V, NC>(values + n * a.v.row, in_row, lanes_per_row, a.size, val[u]);
+        for (int u = 0; u < kUnroll; ++u) {
+            const int64_t n = first + u * step + sub;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int d = (c * lanes_per_row + in_row) * V;
+                if (n < end && d < a.size) {
+                    load_raw<T, V>(key[u][c], keys + n * a.k.row + d);
+                    load_raw<T, V>(val[u][c], values + n * a.v.row + d);
                 } else {
-#pragma unroll
-                    for (int c = 0; c < NC; ++c)
-#pragma unroll
-                        for (int e = 0; e < V; ++e) key[u][c][e] = val[u][c][e] = 0.f;
+                    clear_raw<T, V>(key[u][c]);
+                    clear_raw<T, V>(val[u][c]);
                 }
             }
-#pragma unroll
-            for (int g = 0; g < GH; ++g)
-#pragma unroll
-                for (int u = 0; u < kUnroll; ++u) s[g][u] = sum_lanes(dot<V, NC>(q[g], key[u]), lanes_per_row) * c2;
         }
+    };
+    const int64_t start = begin + slice * per_warp;
+    if (start < end) fetch(start);
+    for (int64_t first = start; first < end; first += (int64_t)step * kUnroll) {  // the same for the warp's lanes
+        float s[GH][kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            float x[NC][V];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) widen<T, V>(key[u][c], x[c]);
+#pragma unroll
+            for (int g = 0; g < GH; ++g) s[g][u] = dot<V, NC>(q[g], x);
+        }
+        RawRow<T, V> now_val[kUnroll][NC];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) now_val[u][c] = val[u][c];
+        if (first + (int64_t)step * kUnroll < end) fetch(first + (int64_t)step * kUnroll);
 #pragma unroll
         for (int g = 0; g < GH; ++g) {
             float now = top[g];
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
+                s[g][u] = sum_lanes(s[g][u], lanes_per_row) * c2;
                 if (first + u * step + sub >= end) s[g][u] = -INFINITY;
                 now = fmaxf(now, s[g][u]);
             }
@@ -164,16 +212,24 @@ attention_row_kernel(AttentionCall a, int lanes_per_row, int splits, T* __restri
                 for (int e = 0; e < V; ++e) acc[g][c][e] *= fade;
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
-                const float p = exp2_fast(s[g][u] - from);
-                total[g] += p;
+                s[g][u] = exp2_fast(s[g][u] - from);
+                total[g] += s[g][u];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            float x[NC][V];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) widen<T, V>(now_val[u][c], x[c]);
+#pragma unroll
+            for (int g = 0; g < GH; ++g)
 #pragma unroll
                 for (int c = 0; c < NC; ++c)
 #pragma unroll
-                    for (int e = 0; e < V; ++e) acc[g][c][e] = fmaf(p, val[u][c][e], acc[g][c][e]);
-            }
+                    for (int e = 0; e < V; ++e) acc[g][c][e] = fmaf(s[g][u], x[c][e], acc[g][c][e]);
         }
     }
-    // join the row groups of the block
+    // join the row groups of a warp, then the warps of a head in ascending order
 #pragma unroll
     for (int g = 0; g < GH; ++g) {
         if (g >= heads_here) break;  // the same for the whole block
@@ -181,22 +237,31 @@ attention_row_kernel(AttentionCall a, int lanes_per_row, int splits, T* __restri
         for (int o = lanes_per_row; o < 32; o <<= 1) now = fmaxf(now, __shfl_xor_sync(kFullMask, now, o));
         if (lane == 0) stat[warp][0] = now;
         __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) now = fmaxf(now, stat[w][0]);
+        for (int w = warp % warp_heads; w < kRowWarps; w += warp_heads) now = fmaxf(now, stat[w][0]);
         const float from = now == -INFINITY ? 0.f : now;
         const float fade = exp2_fast(top[g] - from);
         float sum = total[g] * fade;
+        for (int o = lanes_per_row; o < 32; o <<= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+        if (lane == 0) stat[warp][1] = sum;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int e = 0; e < V; ++e) acc[g][c][e] *= fade;
-        for (int o = lanes_per_row; o < 32; o <<= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
-        if (lane == 0) stat[warp][1] = sum;
-        add_over_block<V, NC>(acc[g], lanes_per_row, scratch);  // synchronises, so `stat` is complete
-        if (warp == 0) {
-            sum = 0.f;
+            for (int e = 0; e < V; ++e) {
+                acc[g][c][e] *= fade;
+                for (int o = lanes_per_row; o < 32; o <<= 1) acc[g][c][e] += __shfl_xor_sync(kFullMask, acc[g][c][e], o);
+                if (slice > 0 && lane < lanes_per_row) scratch[((warp * NC + c) * 32 + lane) * V + e] = acc[g][c][e];
+            }
+        __syncthreads();
+        if (slice == 0) {
+            for (int w = warp + warp_heads; w < kRowWarps; w += warp_heads) {
+                sum += stat[w][1];
+                if (lane < lanes_per_row) {
 #pragma unroll
-            for (int w = 0; w < kRowWarps; ++w) sum += stat[w][1];
+                    for (int c = 0; c < NC; ++c)
+#pragma unroll
+                        for (int e = 0; e < V; ++e) acc[g][c][e] += scratch[((w * NC + c) * 32 + lane) * V + e];
+                }
+            }
             const int64_t at = m * a.heads + h0 + g;
             if (splits > 1) {
                 const int64_t slot = (int64_t)split * a.num_queries * a.heads + at;
@@ -439,9 +504,10 @@ static RowLayout row_layout(const AttentionCall& a, const HeadRows* grads) {
 }
 
 // How many blocks share the `streamed` rows of a cloud (on average) when there are `units` blocks without a split: enough to
-// give every SM about four blocks, as long as a block keeps at least 256 rows.
+// give every SM about twelve blocks (clouds differ in size, and the last blocks should be short), as long as a block keeps
+// at least 256 rows.
 static int choose_splits(int64_t units, int64_t streamed_per_cloud) {
-    const int64_t want = (int64_t)sm_count() * 4;
+    const int64_t want = (int64_t)sm_count() * 12;
     int64_t s = units > 0 ? (want + units - 1) / units : 1;
     const int64_t most = streamed_per_cloud / 256;
     if (s > most) s = most;
@@ -456,8 +522,14 @@ static int forward_parts(const AttentionCall& a) {
     return group >= 2 ? (group + 3) / 4 : 1;
 }
 
+// Key heads that a block of the forward kernel serves side by side, one (or several) warps each.
+static int warp_heads(const AttentionCall& a) {
+    int n = kRowWarps;
+    while (a.kv_heads % n) n /= 2;
+    return n;
+}
 static int forward_splits(const AttentionCall& a) {
-    return choose_splits(a.num_queries * a.kv_heads * forward_parts(a), mean_rows(a.num_keys, a.clouds));
+    return choose_splits(a.num_queries * (a.kv_heads / warp_heads(a)) * forward_parts(a), mean_rows(a.num_keys, a.clouds));
 }
 static int query_grad_splits(const AttentionCall& a) {
     return choose_splits(a.num_queries * a.heads, mean_rows(a.num_keys, a.clouds));
@@ -479,9 +551,12 @@ static int launch_rows(const AttentionCall& a, const RowLayout& l, void* out, fl
     const int splits = forward_splits(a);
     float2* stat = (float2*)ws;
     float* part = (float*)(ws + align_up((size_t)splits * a.num_queries * a.heads * sizeof(float2)));
-    const dim3 grid((unsigned)a.num_queries, (unsigned)(a.kv_heads * forward_parts(a)), (unsigned)splits);
-    if (a.heads > a.kv_heads) attention_row_kernel<T, V, NC, 4><<<grid, kRowThreads, 0, s>>>(a, l.lanes, splits, (T*)out, lse, part, stat);
-    else attention_row_kernel<T, V, NC, 1><<<grid, kRowThreads, 0, s>>>(a, l.lanes, splits, (T*)out, lse, part, stat);
+    const int side_by_side = warp_heads(a);
+    const dim3 grid((unsigned)a.num_queries, (unsigned)(a.kv_heads / side_by_side * forward_parts(a)), (unsigned)splits);
+    if (a.heads > a.kv_heads)
+        attention_row_kernel<T, V, NC, 4><<<grid, kRowThreads, 0, s>>>(a, l.lanes, side_by_side, splits, (T*)out, lse, part, stat);
+    else
+        attention_row_kernel<T, V, NC, 1><<<grid, kRowThreads, 0, s>>>(a, l.lanes, side_by_side, splits, (T*)out, lse, part, stat);
     PCCNN_LAUNCH_CHECK();
     return splits > 1 ? join_splits(a, splits, part, stat, out, lse, s) : PCCNN_OK;
 }

@@ -741,6 +741,18 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
             tc_load_whole<kTcRows, NP, GR>(smem + Cfg::kFixed, &map_f2, num_rows, head, row0, &sh->fixed_full2);
         }
         __syncwarp();
+        // KEYS: the columns' statistics of the next unit are on their way while the loader waits for its slot
+        float next_lse[BN / 32], next_delta[BN / 32];
+        auto fetch = [&](int u) {
+            const int64_t at = (int64_t)(head * share + u / tiles) * num_stream + begin + (int64_t)(u % tiles) * BN;
+#pragma unroll
+            for (int i = 0; i < BN / 32; ++i) {
+                const bool in = u < units && (u % tiles < tiles - 1 || i * 32 + lane < last_valid);
+                next_lse[i] = in ? lse[at + i * 32 + lane] : -INFINITY;
+                next_delta[i] = in ? delta[at + i * 32 + lane] : 0.f;
+            }
+        };
+        if (KEYS) fetch(0);
         for (; issued < units; ++issued) {
             if (ctl.withhold_from >= 0 && issued >= ctl.withhold_from) ok = false;
             const int s = issued % kStages;
@@ -750,15 +762,15 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
             const int valid = j == tiles - 1 ? last_valid : BN;
             const int64_t from = begin + (int64_t)j * BN;
             uint8_t* slot = ring + s * 2 * Cfg::kTile;
-            if (KEYS) {  // the columns' statistics; an absent query has probability 2^-inf
+            if (KEYS) {  // an absent query has probability 2^-inf
                 float* stats = column_stats + s * 2 * BN;
 #pragma unroll
-                for (int i = lane; i < BN; i += 32) {
-                    const float l = i < valid ? lse[(int64_t)h * num_stream + from + i] : -INFINITY;
-                    stats[i] = l == -INFINITY ? INFINITY : l * kLog2e;
-                    stats[BN + i] = i < valid ? delta[(int64_t)h * num_stream + from + i] : 0.f;
+                for (int i = 0; i < BN / 32; ++i) {
+                    stats[i * 32 + lane] = next_lse[i] == -INFINITY ? INFINITY : next_lse[i] * kLog2e;
+                    stats[BN + i * 32 + lane] = next_delta[i];
                 }
                 __syncwarp();
+                fetch(issued + 1);
             }
             tc_load_tile<BN, NP, GR>(slot, &map_y1, &map_y18, rows_y1, num_stream, h, from, valid, a.size, &sh->full[s]);
             tc_load_tile<BN, NP, GR>(slot + Cfg::kTile, &map_y2, &map_y28, rows_y2, num_stream, h, from, valid, a.size, &sh->full2[s]);
@@ -845,19 +857,16 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
             tc_fence_after();
             const int valid = u % tiles == tiles - 1 ? last_valid : BN;
             const float* stats = column_stats + (u % kStages) * 2 * BN;
-            uint32_t s[BN / 32][32], t[BN / 32][32];
 #pragma unroll
             for (int i = 0; i < BN / 32; ++i) {
-                tc_ld_32x32(buf + 32 * i, s[i]);
-                tc_ld_32x32(buf + BN + 32 * i, t[i]);
-            }
-            tc_arrive_warp(&sh->s_free[group]);
-            if (u >= 2) {  // the group's last unit has been added: its columns of weights are free
-                if (!(ok = tc_wait_warp(&sh->e_done[group], ((u >> 1) - 1) & 1, limit, failed))) break;
-                tc_fence_after();
-            }
-#pragma unroll
-            for (int i = 0; i < BN / 32; ++i) {
+                uint32_t s[32], t[32];
+                tc_ld_32x32(buf + 32 * i, s);
+                tc_ld_32x32(buf + BN + 32 * i, t);
+                if (i == BN / 32 - 1) tc_arrive_warp(&sh->s_free[group]);
+                if (i == 0 && u >= 2) {  // the group's last unit has been added: its columns of weights are free
+                    if (!(ok = tc_wait_warp(&sh->e_done[group], ((u >> 1) - 1) & 1, limit, failed))) break;
+                    tc_fence_after();
+                }
                 float p[32], e[32];
 #pragma unroll
                 for (int c = 0; c < 32; c += 4) {
@@ -866,14 +875,14 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                         base = *reinterpret_cast<const float4*>(stats + i * 32 + c);
                         d = *reinterpret_cast<const float4*>(stats + BN + i * 32 + c);
                     }
-                    p[c] = exp2_fast(fmaf(__uint_as_float(s[i][c]), c2, -base.x));
-                    p[c + 1] = exp2_fast(fmaf(__uint_as_float(s[i][c + 1]), c2, -base.y));
-                    p[c + 2] = exp2_fast(fmaf(__uint_as_float(s[i][c + 2]), c2, -base.z));
-                    p[c + 3] = exp2_fast(fmaf(__uint_as_float(s[i][c + 3]), c2, -base.w));
-                    e[c] = p[c] * (__uint_as_float(t[i][c]) - d.x);
-                    e[c + 1] = p[c + 1] * (__uint_as_float(t[i][c + 1]) - d.y);
-                    e[c + 2] = p[c + 2] * (__uint_as_float(t[i][c + 2]) - d.z);
-                    e[c + 3] = p[c + 3] * (__uint_as_float(t[i][c + 3]) - d.w);
+                    p[c] = exp2_fast(fmaf(__uint_as_float(s[c]), c2, -base.x));
+                    p[c + 1] = exp2_fast(fmaf(__uint_as_float(s[c + 1]), c2, -base.y));
+                    p[c + 2] = exp2_fast(fmaf(__uint_as_float(s[c + 2]), c2, -base.z));
+                    p[c + 3] = exp2_fast(fmaf(__uint_as_float(s[c + 3]), c2, -base.w));
+                    e[c] = p[c] * (__uint_as_float(t[c]) - d.x);
+                    e[c + 1] = p[c + 1] * (__uint_as_float(t[c + 1]) - d.y);
+                    e[c + 2] = p[c + 2] * (__uint_as_float(t[c + 2]) - d.z);
+                    e[c + 3] = p[c + 3] * (__uint_as_float(t[c + 3]) - d.w);
                 }
                 if (!KEYS && valid < BN) {
 #pragma unroll
@@ -884,6 +893,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                 tc_store_weights<NP, Cfg::kPlane>(weights + 16 * i, e);
                 if (KEYS) tc_store_weights<NP, Cfg::kPlane>(weights + NP * Cfg::kPlane + 16 * i, p);
             }
+            if (!ok) break;
             tc_wait_st();
             tc_arrive_warp(&sh->e_ready[group]);
         }

@@ -17,78 +17,111 @@ namespace pccnn {
 
 constexpr int kNormThreads = 256;
 
-// Sum over the TPR consecutive threads that share a row; every one of them gets it.  TPR = 256 uses shared memory
-// (one slot set per call site parity) and needs all threads of the block.
-template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float* slots) {
+// Sums of R rows over the TPR consecutive threads that share them; every one of them gets the sums.  TPR = 256 uses shared
+// memory and needs all threads of the block; consecutive calls alternate between the two halves of `slots`, so one barrier
+// per call is enough.
+template <int TPR, int R>
+__device__ __forceinline__ void row_sums(float (&v)[R], float (*slots)[kNormThreads / 32][R]) {
     constexpr int kLanes = TPR < 32 ? TPR : 32;
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
-    if (TPR > 32) {
-        __syncthreads();
-        if (lane_id() == 0) slots[threadIdx.x >> 5] = v;
-        __syncthreads();
-        v = 0.f;
+    for (int o = kLanes / 2; o > 0; o >>= 1) {
 #pragma unroll
-        for (int w = 0; w < kNormThreads / 32; ++w) v += slots[w];
+        for (int i = 0; i < R; ++i) v[i] += __shfl_xor_sync(kFullMask, v[i], o);
     }
-    return v;
+    if (TPR > 32) {
+        if (lane_id() == 0) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) (*slots)[threadIdx.x >> 5][i] = v[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            v[i] = 0.f;
+#pragma unroll
+            for (int w = 0; w < kNormThreads / 32; ++w) v[i] += (*slots)[w][i];
+        }
+    }
 }
 
-// One row per TPR threads, K vectors of V elements per thread.
-template <class T, int V, int TPR, int K>
+// R rows per TPR threads at once (their loads are in flight together), K vectors of V elements per thread and row.
+template <class T, int V, int TPR, int K, int R>
 __global__ void __launch_bounds__(kNormThreads)
 layer_norm_kernel(int64_t rows, int channels, const T* __restrict__ feats, int64_t ld, const float* __restrict__ weights,
                   const float* __restrict__ bias, float eps, T* __restrict__ out, float* __restrict__ out_mean,
                   float* __restrict__ out_rstd) {
-    __shared__ float slots[kNormThreads / 32];
+    __shared__ float slots[2][kNormThreads / 32][R];
     const int t = threadIdx.x % TPR;
-    const int64_t row = (int64_t)blockIdx.x * (kNormThreads / TPR) + threadIdx.x / TPR;
-    const bool live = row < rows;
-    const T* src = feats + (live ? row : 0) * ld;
-    float x[K][V];
-    float sum = 0.f;
+    const int64_t row0 = ((int64_t)blockIdx.x * (kNormThreads / TPR) + threadIdx.x / TPR) * R;
+    float x[R][K][V], mean[R], rstd[R];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int c = (k * TPR + t) * V;
-        if (live && c < channels) {
-            load_vec<T, V>(src + c, x[k]);
-        } else {
+    for (int i = 0; i < R; ++i) {
+        const T* src = feats + (row0 + i < rows ? row0 + i : 0) * ld;
 #pragma unroll
-            for (int e = 0; e < V; ++e) x[k][e] = 0.f;
-        }
+        for (int k = 0; k < K; ++k) {
+            const int c = (k * TPR + t) * V;
+            if (row0 + i < rows && c < channels) {
+                load_vec<T, V>(src + c, x[i][k]);
+            } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) sum += x[k][e];
-    }
-    const float mean = row_sum<TPR>(sum, slots) / (float)channels;
-    float sq = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const bool in = (k * TPR + t) * V < channels;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const float d = x[k][e] - mean;
-            sq += in ? d * d : 0.f;
+                for (int e = 0; e < V; ++e) x[i][k][e] = 0.f;
+            }
         }
     }
-    const float rstd = 1.f / sqrtf(row_sum<TPR>(sq, slots) / (float)channels + eps);
-    if (!live) return;
-    if (t == 0) {
-        out_mean[row] = mean;
-        out_rstd[row] = rstd;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        mean[i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int e = 0; e < V; ++e) mean[i] += x[i][k][e];
     }
-    T* dst = out + row * channels;
+    row_sums<TPR, R>(mean, &slots[0]);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        mean[i] /= (float)channels;
+        rstd[i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const bool in = (k * TPR + t) * V < channels;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float d = x[i][k][e] - mean[i];
+                rstd[i] += in ? d * d : 0.f;
+            }
+        }
+    }
+    row_sums<TPR, R>(rstd, &slots[1]);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        rstd[i] = 1.f / sqrtf(rstd[i] / (float)channels + eps);
+        if (t == 0 && row0 + i < rows) {
+            out_mean[row0 + i] = mean[i];
+            out_rstd[row0 + i] = rstd[i];
+        }
+    }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const int c = (k * TPR + t) * V;
         if (c >= channels) break;
-        float w[V], b[V], y[V];
+        float w[V], b[V];
         load_vec<float, V>(weights + c, w);
         load_vec<float, V>(bias + c, b);
 #pragma unroll
-        for (int e = 0; e < V; ++e) y[e] = (x[k][e] - mean) * rstd * w[e] + b[e];
-        store_vec<T, V>(dst + c, y);
+        for (int i = 0; i < R; ++i) {
+            if (row0 + i >= rows) break;
+            float y[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) y[e] = (x[i][k][e] - mean[i]) * rstd[i] * w[e] + b[e];
+            store_vec<T, V>(out + (row0 + i) * channels + c, y);
+        }
     }
+}
+
+// Sum over the block for the kernels of very wide rows.
+__device__ __forceinline__ float block_sum(float v, float (*slots)[kNormThreads / 32][1]) {
+    float s[1] = {v};
+    row_sums<kNormThreads, 1>(s, slots);
+    return s[0];
 }
 
 // Rows that do not fit the registers of a block: three passes over the row, which the first one leaves in the caches.
@@ -97,17 +130,17 @@ __global__ void __launch_bounds__(kNormThreads)
 layer_norm_wide_kernel(int channels, const T* __restrict__ feats, int64_t ld, const float* __restrict__ weights,
                        const float* __restrict__ bias, float eps, T* __restrict__ out, float* __restrict__ out_mean,
                        float* __restrict__ out_rstd) {
-    __shared__ float slots[kNormThreads / 32];
+    __shared__ float slots[2][kNormThreads / 32][1];
     const int64_t row = blockIdx.x;
     const T* src = feats + row * ld;
     float sum = 0.f, sq = 0.f;
     for (int c = threadIdx.x; c < channels; c += kNormThreads) sum += to_float(src[c]);
-    const float mean = row_sum<kNormThreads>(sum, slots) / (float)channels;
+    const float mean = block_sum(sum, &slots[0]) / (float)channels;
     for (int c = threadIdx.x; c < channels; c += kNormThreads) {
         const float d = to_float(src[c]) - mean;
         sq += d * d;
     }
-    const float rstd = 1.f / sqrtf(row_sum<kNormThreads>(sq, slots) / (float)channels + eps);
+    const float rstd = 1.f / sqrtf(block_sum(sq, &slots[1]) / (float)channels + eps);
     if (threadIdx.x == 0) {
         out_mean[row] = mean;
         out_rstd[row] = rstd;
@@ -116,16 +149,16 @@ layer_norm_wide_kernel(int channels, const T* __restrict__ feats, int64_t ld, co
         out[row * channels + c] = from_float<T>((to_float(src[c]) - mean) * rstd * weights[c] + bias[c]);
 }
 
-// Backward: the block's row groups walk the rows with a stride of the whole grid; column sums stay in registers and are
-// added over the groups of the block, in ascending order, at the end.
-template <class T, int V, int TPR, int K>
+// Backward: the block's row groups walk the rows, R at a time, with a stride of the whole grid; column sums stay in registers
+// and are added over the groups of the block, in ascending order, at the end.
+template <class T, int V, int TPR, int K, int R>
 __global__ void __launch_bounds__(kNormThreads)
 layer_norm_grads_kernel(int64_t rows, int channels, const T* __restrict__ feats, int64_t ld, const float* __restrict__ weights,
                         const float* __restrict__ mean, const float* __restrict__ rstd, const T* __restrict__ grads,
                         int64_t ld_g, T* __restrict__ out, float* __restrict__ partial) {
     constexpr int kGroups = kNormThreads / TPR;
     extern __shared__ float sums[];  // [2][channels], where several rows share a block (at most 1024 channels: 8 KB)
-    __shared__ float slots[kNormThreads / 32];
+    __shared__ float slots[2][kNormThreads / 32][2 * R];
     const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
     float w[K][V], dw[K][V], db[K][V];
 #pragma unroll
@@ -136,47 +169,59 @@ layer_norm_grads_kernel(int64_t rows, int channels, const T* __restrict__ feats,
         if (c < channels) load_vec<float, V>(weights + c, w[k]);
     }
     const float inv = 1.f / (float)channels;
-    for (int64_t base = (int64_t)blockIdx.x * kGroups; base < rows; base += (int64_t)gridDim.x * kGroups) {
-        const int64_t row = base + group;
-        const bool live = row < rows;  // every thread of the warp stays for the shuffles
-        const float mu = live ? mean[row] : 0.f, r = live ? rstd[row] : 0.f;
-        float x[K][V], g[K][V];
+    int turn = 0;
+    for (int64_t base = (int64_t)blockIdx.x * kGroups * R; base < rows; base += (int64_t)gridDim.x * kGroups * R, turn ^= 1) {
+        const int64_t row0 = base + group * R;
+        float x[R][K][V], g[R][K][V], mu[R], r[R], s[2 * R];
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = (k * TPR + t) * V;
-            if (live && c < channels) {
-                load_vec<T, V>(feats + row * ld + c, x[k]);
-                load_vec<T, V>(grads + row * ld_g + c, g[k]);
-            } else {
+        for (int i = 0; i < R; ++i) {
+            const int64_t row = row0 + i;
+            const bool live = row < rows;  // every thread of the warp stays for the shuffles
+            mu[i] = live ? mean[row] : 0.f;
+            r[i] = live ? rstd[row] : 0.f;
 #pragma unroll
-                for (int e = 0; e < V; ++e) x[k][e] = mu, g[k][e] = 0.f;
+            for (int k = 0; k < K; ++k) {
+                const int c = (k * TPR + t) * V;
+                if (live && c < channels) {
+                    load_vec<T, V>(feats + row * ld + c, x[i][k]);
+                    load_vec<T, V>(grads + row * ld_g + c, g[i][k]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) x[i][k][e] = mu[i], g[i][k][e] = 0.f;
+                }
             }
         }
-        float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
+        for (int i = 0; i < R; ++i) {
+            s[2 * i] = s[2 * i + 1] = 0.f;
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float hat = (x[k][e] - mu) * r;
-                dw[k][e] += g[k][e] * hat;
-                db[k][e] += g[k][e];
-                x[k][e] = hat;
-                g[k][e] *= w[k][e];
-                s1 += g[k][e];
-                s2 += g[k][e] * hat;
+            for (int k = 0; k < K; ++k) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float hat = (x[i][k][e] - mu[i]) * r[i];
+                    dw[k][e] += g[i][k][e] * hat;
+                    db[k][e] += g[i][k][e];
+                    x[i][k][e] = hat;
+                    g[i][k][e] *= w[k][e];
+                    s[2 * i] += g[i][k][e];
+                    s[2 * i + 1] += g[i][k][e] * hat;
+                }
             }
         }
-        s1 = row_sum<TPR>(s1, slots) * inv;
-        s2 = row_sum<TPR>(s2, slots) * inv;
-        if (!live) continue;
+        row_sums<TPR, 2 * R>(s, &slots[turn]);
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = (k * TPR + t) * V;
-            if (c >= channels) break;
-            float y[V];
+        for (int i = 0; i < R; ++i) {
+            if (row0 + i >= rows) break;
+            const float s1 = s[2 * i] * inv, s2 = s[2 * i + 1] * inv;
 #pragma unroll
-            for (int e = 0; e < V; ++e) y[e] = r * (g[k][e] - s1 - x[k][e] * s2);
-            store_vec<T, V>(out + row * channels + c, y);
+            for (int k = 0; k < K; ++k) {
+                const int c = (k * TPR + t) * V;
+                if (c >= channels) break;
+                float y[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) y[e] = r[i] * (g[i][k][e] - s1 - x[i][k][e] * s2);
+                store_vec<T, V>(out + (row0 + i) * channels + c, y);
+            }
         }
     }
     float* dst = partial + (int64_t)blockIdx.x * 2 * channels;
@@ -189,16 +234,16 @@ layer_norm_grads_kernel(int64_t rows, int channels, const T* __restrict__ feats,
             for (int e = 0; e < V; ++e) dst[c + e] = dw[k][e], dst[channels + c + e] = db[k][e];
         }
     } else {
-        for (int turn = 0; turn < kGroups; ++turn) {
-            if (group == turn) {
+        for (int g = 0; g < kGroups; ++g) {
+            if (group == g) {
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
                         const int c = (k * TPR + t) * V + e;
                         if (c < channels) {
-                            sums[c] = turn ? sums[c] + dw[k][e] : dw[k][e];
-                            sums[channels + c] = turn ? sums[channels + c] + db[k][e] : db[k][e];
+                            sums[c] = g ? sums[c] + dw[k][e] : dw[k][e];
+                            sums[channels + c] = g ? sums[channels + c] + db[k][e] : db[k][e];
                         }
                     }
                 }
@@ -215,7 +260,7 @@ __global__ void __launch_bounds__(kNormThreads)
 layer_norm_grads_wide_kernel(int64_t rows, int channels, const T* __restrict__ feats, int64_t ld,
                              const float* __restrict__ weights, const float* __restrict__ mean, const float* __restrict__ rstd,
                              const T* __restrict__ grads, int64_t ld_g, T* __restrict__ out, float* __restrict__ partial) {
-    __shared__ float slots[kNormThreads / 32];
+    __shared__ float slots[2][kNormThreads / 32][1];
     float* dw = partial + (int64_t)blockIdx.x * 2 * channels;
     float* db = dw + channels;
     for (int c = threadIdx.x; c < channels; c += kNormThreads) dw[c] = db[c] = 0.f;
@@ -230,8 +275,8 @@ layer_norm_grads_wide_kernel(int64_t rows, int channels, const T* __restrict__ f
             s1 += gr * weights[c];
             s2 += gr * weights[c] * hat;
         }
-        s1 = row_sum<kNormThreads>(s1, slots) / (float)channels;
-        s2 = row_sum<kNormThreads>(s2, slots) / (float)channels;
+        s1 = block_sum(s1, &slots[0]) / (float)channels;
+        s2 = block_sum(s2, &slots[1]) / (float)channels;
         for (int c = threadIdx.x; c < channels; c += kNormThreads) {
             const float hat = (to_float(x[c]) - mu) * r;
             out[row * channels + c] = from_float<T>(r * (to_float(g[c]) * weights[c] - s1 - hat * s2));
@@ -264,35 +309,38 @@ static int norm_blocks(int64_t rows, int rows_per_block) {
     return (int)(need < 1 ? 1 : need < cap ? need : cap);
 }
 
-// The vector width, threads per row and vectors per thread of a row: 16-byte vectors where every row starts on a 16-byte
-// boundary, single elements otherwise; as few threads per row as keep it to at most 8 vectors (16 single elements) each.
+// The vector width, threads per row, vectors per thread and rows at once: 16-byte vectors where every row starts on a 16-byte
+// boundary, single elements otherwise; few threads per row while that keeps it to a few vectors each, and then as many rows
+// at once as keep about four vectors (or sixteen single elements) of a thread in flight.
 template <class T, class Launch>
 static int dispatch_norm(int channels, bool vectors, const Launch& launch) {
     constexpr int kV = 16 / sizeof(T);
     if (vectors) {
         const int n = channels / kV;
-        if (n <= 8) return launch.template run<T, kV, 8, 1>();
-        if (n <= 16) return launch.template run<T, kV, 8, 2>();
-        if (n <= 32) return launch.template run<T, kV, 32, 1>();
-        if (n <= 64) return launch.template run<T, kV, 32, 2>();
-        if (n <= 128) return launch.template run<T, kV, 32, 4>();
-        if (n <= 1024) return launch.template run<T, kV, 256, 4>();
+        if (n <= 8) return launch.template run<T, kV, 8, 1, 4>();
+        if (n <= 16) return launch.template run<T, kV, 8, 2, 2>();
+        if (n <= 32) return launch.template run<T, kV, 32, 1, 4>();
+        if (n <= 64) return launch.template run<T, kV, 32, 2, 2>();
+        if (n <= 128) return launch.template run<T, kV, 32, 4, 1>();
+        if (n <= 256) return launch.template run<T, kV, 256, 1, 4>();
+        if (n <= 1024) return launch.template run<T, kV, 256, 4, 1>();
         return launch.template wide<T>();
     }
-    if (channels <= 32) return launch.template run<T, 1, 8, 4>();
-    if (channels <= 128) return launch.template run<T, 1, 32, 4>();
-    if (channels <= 512) return launch.template run<T, 1, 32, 16>();
-    if (channels <= 1024) return launch.template run<T, 1, 256, 4>();
-    if (channels <= 4096) return launch.template run<T, 1, 256, 16>();
+    if (channels <= 32) return launch.template run<T, 1, 8, 4, 4>();
+    if (channels <= 128) return launch.template run<T, 1, 32, 4, 4>();
+    if (channels <= 512) return launch.template run<T, 1, 32, 16, 1>();
+    if (channels <= 1024) return launch.template run<T, 1, 256, 4, 4>();
+    if (channels <= 4096) return launch.template run<T, 1, 256, 16, 1>();
     return launch.template wide<T>();
 }
 
 struct NormForward {
     int64_t rows; int channels; const void* feats; int64_t ld; const float *weights, *bias; float eps;
     void* out; float *mean, *rstd; cudaStream_t s;
-    template <class T, int V, int TPR, int K> int run() const {
-        const int64_t blocks = (rows + kNormThreads / TPR - 1) / (kNormThreads / TPR);
-        layer_norm_kernel<T, V, TPR, K><<<(unsigned)blocks, kNormThreads, 0, s>>>(rows, channels, (const T*)feats, ld, weights, bias,
+    template <class T, int V, int TPR, int K, int R> int run() const {
+        const int per_block = kNormThreads / TPR * R;
+        const int64_t blocks = (rows + per_block - 1) / per_block;
+        layer_norm_kernel<T, V, TPR, K, R><<<(unsigned)blocks, kNormThreads, 0, s>>>(rows, channels, (const T*)feats, ld, weights, bias,
                                                                                  eps, (T*)out, mean, rstd);
         PCCNN_LAUNCH_CHECK();
         return PCCNN_OK;
@@ -313,9 +361,9 @@ struct NormBackward {
         PCCNN_LAUNCH_CHECK();
         return PCCNN_OK;
     }
-    template <class T, int V, int TPR, int K> int run() const {
-        const int blocks = norm_blocks(rows, kNormThreads / TPR);
-        layer_norm_grads_kernel<T, V, TPR, K><<<blocks, kNormThreads, TPR < kNormThreads ? (size_t)2 * channels * 4 : 0, s>>>(
+    template <class T, int V, int TPR, int K, int R> int run() const {
+        const int blocks = norm_blocks(rows, kNormThreads / TPR * R);
+        layer_norm_grads_kernel<T, V, TPR, K, R><<<blocks, kNormThreads, TPR < kNormThreads ? (size_t)2 * channels * 4 : 0, s>>>(
             rows, channels, (const T*)feats, ld, weights, mean, rstd, (const T*)grads, ld_g, (T*)out, partial);
         PCCNN_LAUNCH_CHECK();
         return sums(blocks);

@@ -11,6 +11,8 @@
 // those lanes in a fixed order.
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "features.cuh"
 
@@ -42,72 +44,104 @@ __device__ __forceinline__ int axis_of(const RotaryAxes& axes, int pair) {
     return a;
 }
 
-// P pairs per access.  kGrads: `in` is the gradient, turned back, and the coordinates' gradient is taken from it and
-// `feats` when pt_grads is given.
-template <class T, int P, bool kGrads>
+// P pairs per access, kAtOnce accesses of a lane in flight.  kAxes > 0: `in` is the gradient, turned back, and the
+// coordinates' gradient (of at most kAxes axes) is taken from it and `feats` when pt_grads is given.
+template <class T, int P, int kAxes>
 __global__ void __launch_bounds__(kRotaryThreads)
 rotary_kernel(int64_t rows, int heads, int size, const T* __restrict__ in, RotaryRows ld_in, const T* __restrict__ feats,
               RotaryRows ld_feats, const float* __restrict__ pts, const float* __restrict__ frequencies, RotaryAxes axes,
               int lanes_per_row, T* __restrict__ out, float* __restrict__ pt_grads) {
-    extern __shared__ float2 table[];  // [rows of the block][pairs]
+    constexpr bool kGrads = kAxes > 0;
+    constexpr int kSums = kGrads ? kAxes : 1, kAtOnce = 4;
+    extern __shared__ float2 table[];  // [pairs] (frequency, axis), then [rows of the block][pairs] (cosine, sine)
     const int pairs = axes.last[axes.count - 1];
     const int rows_per_block = kRotaryThreads / lanes_per_row;
     const int slot = threadIdx.x / lanes_per_row, lane = threadIdx.x % lanes_per_row;
-    float2* cs = table + slot * pairs;
+    float2* cs = table + (1 + slot) * pairs;
+    for (int j = threadIdx.x; j < pairs; j += kRotaryThreads) table[j] = make_float2(frequencies[j], __int_as_float(axis_of(axes, j)));
+    __syncthreads();
     const int accesses = (size + 2 * P - 1) / (2 * P), total = heads * accesses;
+    const bool both = kGrads && pt_grads;
     for (int64_t base = (int64_t)blockIdx.x * rows_per_block; base < rows; base += (int64_t)gridDim.x * rows_per_block) {
         const int64_t row = base + slot;
         const bool live = row < rows;
-        if (live)
-            for (int j = lane; j < pairs; j += lanes_per_row)
-                cs[j] = turn_of(pts[row * axes.count + axis_of(axes, j)], frequencies[j]);
-        __syncwarp();
-        float sum[kMaxDims] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int i = live ? lane : total; i < total; i += lanes_per_row) {
-            const int h = i / accesses, d = (i - h * accesses) * 2 * P;
-            const T* src = in + row * ld_in.row + h * ld_in.head + d;
-            T* dst = out + ((int64_t)row * heads + h) * size + d;
-            const bool whole = P > 1 || d + 1 < size;  // P > 1: the size is a multiple of the access
-            float x[2 * P], y[2 * P];
-            if (whole) load_vec<T, 2 * P>(src, x);
-            else x[0] = to_float(src[0]), x[1] = 0.f;
-            float f[2 * P];
-            if (kGrads && pt_grads) {
-                const T* from = feats + row * ld_feats.row + h * ld_feats.head + d;
-                if (whole) load_vec<T, 2 * P>(from, f);
-                else f[0] = f[1] = 0.f;
-            }
+        float sum[kSums];
 #pragma unroll
-            for (int p = 0; p < P; ++p) {
-                const int j = d / 2 + p;
-                const float2 t = j < pairs ? cs[j] : make_float2(1.f, 0.f);
-                const float s = kGrads ? -t.y : t.y, x0 = x[2 * p], x1 = x[2 * p + 1];
-                // a pair that is not turned passes as it is, infinities included
-                y[2 * p] = j < pairs ? x0 * t.x - x1 * s : x0;
-                y[2 * p + 1] = j < pairs ? x0 * s + x1 * t.x : x1;
-                if (kGrads && pt_grads && j < pairs) {
-                    const float f0 = f[2 * p], f1 = f[2 * p + 1];
-                    const float term = (x1 * (f0 * t.x - f1 * t.y) - x0 * (f0 * t.y + f1 * t.x)) * frequencies[j];
-                    const int a = axis_of(axes, j);
+        for (int a = 0; a < kSums; ++a) sum[a] = 0.f;
+        for (int first = 0; first < total; first += kAtOnce * lanes_per_row) {  // the same for the lanes of a warp
+            float x[kAtOnce][2 * P], f[kGrads ? kAtOnce : 1][2 * P];
 #pragma unroll
-                    for (int b = 0; b < kMaxDims; ++b) sum[b] += a == b ? term : 0.f;
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int i = first + u * lanes_per_row + lane;
+                if (live && i < total) {
+                    const int h = i / accesses, d = (i - h * accesses) * 2 * P;
+                    const T* src = in + row * ld_in.row + h * ld_in.head + d;
+                    const bool whole = P > 1 || d + 1 < size;  // P > 1: the size is a multiple of the access
+                    if (whole) load_vec<T, 2 * P>(src, x[u]);
+                    else x[u][0] = to_float(src[0]), x[u][1] = 0.f;
+                    if constexpr (kGrads) {
+                        if (both && whole) load_vec<T, 2 * P>(feats + row * ld_feats.row + h * ld_feats.head + d, f[u]);
+                    }
                 }
             }
-            if (whole) store_vec<T, 2 * P>(dst, y);
-            else dst[0] = from_float<T>(y[0]);
+            if (first == 0) {  // the row's angles, while its features are on their way
+                if (live)
+                    for (int j = lane; j < pairs; j += lanes_per_row) {
+                        const float2 fa = table[j];
+                        cs[j] = turn_of(pts[row * axes.count + __float_as_int(fa.y)], fa.x);
+                    }
+                __syncwarp();
+            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int i = first + u * lanes_per_row + lane;
+                if (live && i < total) {
+                    const int h = i / accesses, d = (i - h * accesses) * 2 * P;
+                    T* dst = out + ((int64_t)row * heads + h) * size + d;
+                    float y[2 * P];
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        const int j = d / 2 + p;
+                        const float x0 = x[u][2 * p], x1 = x[u][2 * p + 1];
+                        y[2 * p] = x0;  // a pair that is not turned passes as it is, infinities included
+                        y[2 * p + 1] = x1;
+                        if (j < pairs) {
+                            const float2 t = cs[j];
+                            const float s = kGrads ? -t.y : t.y;
+                            y[2 * p] = x0 * t.x - x1 * s;
+                            y[2 * p + 1] = x0 * s + x1 * t.x;
+                            if constexpr (kGrads) {
+                                if (both) {
+                                    const float2 fa = table[j];
+                                    const float f0 = f[u][2 * p], f1 = f[u][2 * p + 1];
+                                    const float term = (x1 * (f0 * t.x - f1 * t.y) - x0 * (f0 * t.y + f1 * t.x)) * fa.x;
+#pragma unroll
+                                    for (int a = 0; a < kSums; ++a) sum[a] += __float_as_int(fa.y) == a ? term : 0.f;
+                                }
+                            }
+                        }
+                    }
+                    if (P > 1 || d + 1 < size) store_vec<T, 2 * P>(dst, y);
+                    else dst[0] = from_float<T>(y[0]);
+                }
+            }
         }
-        if (kGrads && pt_grads) {
-            for (int a = 0; a < axes.count; ++a) {
-                float v = a == 0 ? sum[0] : a == 1 ? sum[1] : a == 2 ? sum[2] : a == 3 ? sum[3] : a == 4 ? sum[4] : sum[5];
-                for (int o = lanes_per_row / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
-                if (live && lane == 0) pt_grads[row * axes.count + a] = v;
+        if constexpr (kGrads) {
+            if (both) {
+#pragma unroll
+                for (int a = 0; a < kSums; ++a) {
+                    if (a >= axes.count) break;
+                    float v = sum[a];
+                    for (int o = lanes_per_row / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+                    if (live && lane == 0) pt_grads[row * axes.count + a] = v;
+                }
             }
         }
         __syncwarp();  // the table is rewritten for the next row
     }
 }
 
-template <class T, int P, bool kGrads>
+template <class T, int P, int kAxes>
 static int launch_rotary(int64_t rows, int heads, int size, const void* in, RotaryRows ld_in, const void* feats, RotaryRows ld_feats,
                          const float* pts, const float* frequencies, const RotaryAxes& axes, void* out, float* pt_grads,
                          cudaStream_t s) {
@@ -115,12 +149,12 @@ static int launch_rotary(int64_t rows, int heads, int size, const void* in, Rota
     int lanes = 4;
     while (lanes < 32 && lanes < total) lanes *= 2;
     const int pairs = axes.last[axes.count - 1];
-    // the table of the block's rows stays within 48 KB of shared memory: 8 rows of 512 pairs are 32 KB
-    while (lanes < 32 && (size_t)(kRotaryThreads / lanes) * pairs * sizeof(float2) > 48 * 1024) lanes *= 2;
+    // the tables stay within 48 KB of shared memory: (1 + 8 rows) of 512 pairs are 36 KB
+    while (lanes < 32 && (size_t)(1 + kRotaryThreads / lanes) * pairs * sizeof(float2) > 48 * 1024) lanes *= 2;
     const int per_block = kRotaryThreads / lanes;
-    const size_t smem = (size_t)per_block * pairs * sizeof(float2);
+    const size_t smem = (size_t)(1 + per_block) * pairs * sizeof(float2);
     const int64_t blocks = (rows + per_block - 1) / per_block, cap = (int64_t)sm_count() * 32;
-    rotary_kernel<T, P, kGrads><<<(unsigned)(blocks < cap ? blocks : cap), kRotaryThreads, smem, s>>>(
+    rotary_kernel<T, P, kAxes><<<(unsigned)(blocks < cap ? blocks : cap), kRotaryThreads, smem, s>>>(
         rows, heads, size, (const T*)in, ld_in, (const T*)feats, ld_feats, pts, frequencies, axes, lanes, (T*)out, pt_grads);
     PCCNN_LAUNCH_CHECK();
     return PCCNN_OK;
@@ -151,11 +185,19 @@ static int rotary(const char* who, int64_t rows, int heads, int size, const void
     PCCNN_CHECK_ARG(in && pts && out && (frequencies || pairs == 0) && (!pt_grads || feats), "%s: null pointer", who);
     const int v = is_bf16 ? 8 : 4;
     const bool vec = size % v == 0 && vector_rows(in, ld_in, v) && aligned16(out) && (!pt_grads || vector_rows(feats, ld_feats, v));
-    if (is_bf16)
-        return vec ? launch_rotary<__nv_bfloat16, 4, kGrads>(rows, heads, size, in, ld_in, feats, ld_feats, pts, frequencies, axes, out, pt_grads, s)
-                   : launch_rotary<__nv_bfloat16, 1, kGrads>(rows, heads, size, in, ld_in, feats, ld_feats, pts, frequencies, axes, out, pt_grads, s);
-    return vec ? launch_rotary<float, 2, kGrads>(rows, heads, size, in, ld_in, feats, ld_feats, pts, frequencies, axes, out, pt_grads, s)
-               : launch_rotary<float, 1, kGrads>(rows, heads, size, in, ld_in, feats, ld_feats, pts, frequencies, axes, out, pt_grads, s);
+    // the sums over the axes are unrolled for three of them, the usual case, or for all six
+    auto launch = [&](auto type, auto pairs_at_once) {
+        using T = decltype(type);
+        constexpr int kP = decltype(pairs_at_once)::value;
+        if constexpr (kGrads) {
+            if (num_axes <= 3) return launch_rotary<T, kP, 3>(rows, heads, size, in, ld_in, feats, ld_feats, pts, frequencies, axes, out, pt_grads, s);
+            return launch_rotary<T, kP, kMaxDims>(rows, heads, size, in, ld_in, feats, ld_feats, pts, frequencies, axes, out, pt_grads, s);
+        } else {
+            return launch_rotary<T, kP, 0>(rows, heads, size, in, ld_in, feats, ld_feats, pts, frequencies, axes, out, pt_grads, s);
+        }
+    };
+    if (is_bf16) return vec ? launch(__nv_bfloat16(), std::integral_constant<int, 4>()) : launch(__nv_bfloat16(), std::integral_constant<int, 1>());
+    return vec ? launch(0.f, std::integral_constant<int, 2>()) : launch(0.f, std::integral_constant<int, 1>());
 }
 
 }  // namespace pccnn
