@@ -76,9 +76,11 @@ __device__ __forceinline__ void add_over_block(float (&x)[NC][V], int lanes_per_
     }
 }
 
-// The part of [begin, end) that split s of `splits` works on.
+// The part of [begin, end) that split s of `splits` works on: equal parts, but none of fewer than 192 rows while there are
+// more, so that the splits of a small cloud are few and those of a large one are not longer than need be.
 __device__ __forceinline__ void split_range(int64_t& begin, int64_t& end, int s, int splits) {
-    const int64_t per = (end - begin + splits - 1) / splits;
+    int64_t per = (end - begin + splits - 1) / splits;
+    if (splits > 1 && per < 192) per = 192;
     const int64_t lo = begin + s * per, hi = lo + per;
     end = hi < end ? hi : end;
     begin = lo < end ? lo : end;
@@ -291,33 +293,53 @@ attention_row_kernel(AttentionCall a, int lanes_per_row, int warp_heads, int spl
     }
 }
 
-// Joins the splits of a query: one warp per (query, head).
-template <class T>
+// Joins the splits of a query: W warps of a block per (query, head), each with every W-th split, joined in ascending order.
+template <class T, int W>
 __global__ void __launch_bounds__(256)
 attention_join_kernel(int64_t num_queries, int heads, int size, int splits, const float* __restrict__ part_out,
                       const float2* __restrict__ part_stat, T* __restrict__ out, float* __restrict__ lse) {
-    const int64_t rows = num_queries * heads, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (row >= rows) return;
+    constexpr int kRows = 8 / W, kColumns = kMaxHeadSize / 32;
+    __shared__ float sums[W > 1 ? 8 : 1][kMaxHeadSize + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % W;
+    const int64_t rows = num_queries * heads, row = (int64_t)blockIdx.x * kRows + warp / W;
+    const bool live = row < rows;
     float top = -INFINITY;
-    for (int s = 0; s < splits; ++s) top = fmaxf(top, part_stat[s * rows + row].x);
+    if (live)
+        for (int s = lane; s < splits; s += 32) top = fmaxf(top, part_stat[s * rows + row].x);
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
     const float from = top == -INFINITY ? 0.f : top;
-    float total = 0.f, acc[kMaxHeadSize / 32];
+    float total = 0.f, acc[kColumns];
 #pragma unroll
-    for (int i = 0; i < kMaxHeadSize / 32; ++i) acc[i] = 0.f;
-    for (int s = 0; s < splits; ++s) {
-        const float2 st = part_stat[s * rows + row];
-        if (st.y == 0.f) continue;  // a split without keys: its sum is not read
-        const float f = exp2_fast(st.x - from);
-        total += st.y * f;
+    for (int i = 0; i < kColumns; ++i) acc[i] = 0.f;
+    if (live) {
+#pragma unroll 4
+        for (int s = part; s < splits; s += W) {
+            const float2 st = part_stat[s * rows + row];
+            if (st.y == 0.f) continue;  // a split without keys: its sum is not read
+            const float f = exp2_fast(st.x - from);
+            total += st.y * f;
 #pragma unroll
-        for (int i = 0; i < kMaxHeadSize / 32; ++i)
-            if (i * 32 + lane < size) acc[i] = fmaf(f, part_out[(s * rows + row) * size + i * 32 + lane], acc[i]);
+            for (int i = 0; i < kColumns; ++i)
+                if (i * 32 + lane < size) acc[i] = fmaf(f, part_out[(s * rows + row) * size + i * 32 + lane], acc[i]);
+        }
     }
+    if (W > 1) {
+#pragma unroll
+        for (int i = 0; i < kColumns; ++i) sums[warp][i * 32 + lane] = acc[i];
+        if (lane == 0) sums[warp][kMaxHeadSize] = total;
+        __syncthreads();
+        if (part != 0) return;
+        for (int w = warp + 1; w < warp + W; ++w) {
+            total += sums[w][kMaxHeadSize];
+#pragma unroll
+            for (int i = 0; i < kColumns; ++i) acc[i] += sums[w][i * 32 + lane];
+        }
+    }
+    if (!live) return;
     const float inv = total == 0.f ? 0.f : 1.f / total;
     if (lane == 0) lse[(row % heads) * num_queries + row / heads] = total == 0.f ? -INFINITY : (top + log2f(total)) * kLn2;
 #pragma unroll
-    for (int i = 0; i < kMaxHeadSize / 32; ++i)
+    for (int i = 0; i < kColumns; ++i)
         if (i * 32 + lane < size) out[row * size + i * 32 + lane] = from_float<T>(acc[i] * inv);
 }
 
@@ -538,12 +560,17 @@ static int key_grad_splits(const AttentionCall& a) {
     return choose_splits(a.num_keys * a.kv_heads, mean_rows(a.num_queries, a.clouds));
 }
 
-int join_splits(const AttentionCall& a, int splits, const float* part, const float2* stat, void* out, float* lse, cudaStream_t s) {
-    const unsigned blocks = (unsigned)((a.num_queries * a.heads + 7) / 8);
-    if (a.is_bf16) attention_join_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(a.num_queries, a.heads, a.size, splits, part, stat, (__nv_bfloat16*)out, lse);
-    else attention_join_kernel<float><<<blocks, 256, 0, s>>>(a.num_queries, a.heads, a.size, splits, part, stat, (float*)out, lse);
+template <class T>
+static int join_splits_as(const AttentionCall& a, int splits, const float* part, const float2* stat, void* out, float* lse, cudaStream_t s) {
+    // one warp per row reads its splits one after the other: with many of them (few rows) the whole block shares a row
+    const int64_t rows = a.num_queries * a.heads;
+    if (splits >= 16) attention_join_kernel<T, 8><<<(unsigned)rows, 256, 0, s>>>(a.num_queries, a.heads, a.size, splits, part, stat, (T*)out, lse);
+    else attention_join_kernel<T, 1><<<(unsigned)((rows + 7) / 8), 256, 0, s>>>(a.num_queries, a.heads, a.size, splits, part, stat, (T*)out, lse);
     PCCNN_LAUNCH_CHECK();
     return PCCNN_OK;
+}
+int join_splits(const AttentionCall& a, int splits, const float* part, const float2* stat, void* out, float* lse, cudaStream_t s) {
+    return a.is_bf16 ? join_splits_as<__nv_bfloat16>(a, splits, part, stat, out, lse, s) : join_splits_as<float>(a, splits, part, stat, out, lse, s);
 }
 
 template <class T, int V, int NC>

@@ -21,7 +21,7 @@ struct AttentionCall {
     float scale;
 };
 
-constexpr int kMaxSplits = 64;
+constexpr int kMaxSplits = 128;
 
 // Tensor-core kernels (attention_tc.cu).  Whether a call may use them goes by its shape (tc_shape: the workspace does not
 // depend on anything else) and then by the layout of its tensors (tc_layout).

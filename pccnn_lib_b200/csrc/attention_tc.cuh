@@ -8,9 +8,11 @@
 // A streamed tile in which the cloud ends gets zeros behind the cloud's last row: the rows that follow belong to another cloud
 // and may hold infinities, which would reach this one as 0 * inf.
 //
-// Roles of the ten warps of a CTA: two groups of four warps do the element-wise work (one row of a 128-row tile per thread,
-// which is one lane of tensor memory), warp 8 loads, an elected lane of warp 9 issues the products.  The element-wise groups work
-// on different units in turn, so one of them computes while the tensor cores run the products of the other.
+// Roles of the eleven warps of a CTA: two groups of four warps do the element-wise work (one row of a 128-row tile per thread,
+// which is one lane of tensor memory), warp 8 loads, and elected lanes of warps 9 and 10 issue the products, the logits and
+// the weighted sums: each of the two waits for barriers of its own, and a wait costs as much as issuing a product (measured with one
+// warp for both, 64-row units: 460 of the 1120 cycles of a unit).  The element-wise groups work on different units in turn, so
+// one of them computes while the tensor cores run the products of the other.
 // Every wait is bounded: a role whose wait runs out sets a flag that ends the other roles' waits, the CTA waits for its
 // copies and products in flight, frees its tensor memory and records the failure in the pinned status word.
 #pragma once
@@ -24,7 +26,7 @@
 
 namespace pccnn {
 
-constexpr int kTcThreads = 320;
+constexpr int kTcThreads = 352;
 constexpr int kTcRows = 128;  // rows of the tile whose products have them as the M dimension
 constexpr int kTcMaxStages = 8;
 
@@ -42,8 +44,8 @@ struct TcControl {
 };
 
 struct TcShared {
-    uint64_t fixed_full, fixed_full2, full[kTcMaxStages], full2[kTcMaxStages], empty[kTcMaxStages], s_full[2], s_free[2], e_ready[2],
-        e_done[2], all_done, drained, round_done, acc_free;
+    uint64_t fixed_full, full[kTcMaxStages], empty[kTcMaxStages], s_full[2], s_free[2], e_ready[2],
+        e_done[2], all_done, drained[2], round_done, acc_free;
     uint32_t tmem;
     int failed;
 };
@@ -261,13 +263,11 @@ __device__ __forceinline__ void tc_write16(T* __restrict__ dst, int c, int size,
 
 // ---- set-up and teardown -----------------------------------------------------------------------------------------
 template <int COLUMNS>
-__device__ __forceinline__ uint32_t tc_begin(TcShared* sh, int stages) {
+__device__ __forceinline__ uint32_t tc_begin(TcShared* sh, int stages, int tiles_of_a_stage) {
     if (threadIdx.x == 0) {
         mbar_init(&sh->fixed_full, 1);
-        mbar_init(&sh->fixed_full2, 1);
         for (int i = 0; i < stages; ++i) {
-            mbar_init(&sh->full[i], 1);
-            mbar_init(&sh->full2[i], 1);
+            mbar_init(&sh->full[i], tiles_of_a_stage);
             mbar_init(&sh->empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -277,7 +277,8 @@ __device__ __forceinline__ uint32_t tc_begin(TcShared* sh, int stages) {
             mbar_init(&sh->e_done[i], 1);
         }
         mbar_init(&sh->all_done, 1);
-        mbar_init(&sh->drained, 1);
+        mbar_init(&sh->drained[0], 1);
+        mbar_init(&sh->drained[1], 1);
         mbar_init(&sh->round_done, 1);
         mbar_init(&sh->acc_free, 8);
         sh->failed = 0;
@@ -303,16 +304,16 @@ __device__ __forceinline__ void tc_fail(TcShared* sh, const TcControl& ctl, int 
     *(volatile int*)&sh->failed = 1;
     atomicCAS_system(ctl.sticky, 0, ctl.status | code);
 }
-// The end of the warp that issues the products: all of them have finished when all_done completes; after a failure it waits for
-// those in flight, since tensor memory may only be released after them.
-__device__ __forceinline__ void tc_finish_products(TcShared* sh, const TcControl& ctl, bool ok, bool leader) {
+// The end of a warp that issues products.  Every logit is waited for by the rows, and all sums have finished when all_done
+// completes; after a failure the warp waits for its products in flight, since tensor memory may only be released after them.
+__device__ __forceinline__ void tc_finish_products(TcShared* sh, const TcControl& ctl, bool ok, bool leader, bool sums) {
     if (leader) {
-        if (ok) {
-            tc_commit(&sh->all_done);
-        } else {
+        if (!ok) {
             tc_fail(sh, ctl, 2);
-            tc_commit(&sh->drained);
-            mbar_wait(&sh->drained, 0, ctl.poll_limit);
+            tc_commit(&sh->drained[sums]);
+            mbar_wait(&sh->drained[sums], 0, ctl.poll_limit);
+        } else if (sums) {
+            tc_commit(&sh->all_done);
         }
     }
     __syncwarp();
@@ -345,7 +346,7 @@ struct TcForward {
     static constexpr int kAcc = kWeights + 2 * kWeightCols;
     static constexpr int kBytes = kQ + kStages * kSlot + 1024 + 512;
     static_assert(QT == 1 || NP == 1, "two query tiles are loaded as one plane");
-    static_assert(kStages >= 4 && kAcc + 2 * GR * 64 <= 512, "does not fit");
+    static_assert(kStages >= 4 && kStages % 2 == 0 && kAcc + 2 * GR * 64 <= 512, "does not fit");
     static_assert(kTcRows * GR * 64 * 4 + 2 * kTcRows * 4 <= kQ + kStages * kSlot, "no room to join the two groups");
 };
 
@@ -392,7 +393,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         return;
     }
-    const uint32_t tmem = tc_begin<512>(sh, kStages);
+    const uint32_t tmem = tc_begin<512>(sh, kStages, 1);
     const int tiles = (int)((end - begin + BN - 1) / BN), q_tiles = rows_here > kTcRows ? 2 : 1, units = tiles * q_tiles;
     const int last_valid = (int)(end - begin) - (tiles - 1) * BN;
     const int steps = (a.size + 15) >> 4, n_out = steps * 16;
@@ -401,6 +402,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const uint32_t limit = ctl.poll_limit;
 
     int issued = 0;  // streamed tiles that the loader has started
+    const int ahead = min(tiles, q_tiles == 2 ? 1 : 2);  // key tiles in front of the first value tile
     if (warp == 8) {
         // ---- loader: the tiles in the order in which the products use them
         bool ok = true;
@@ -412,7 +414,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         __syncwarp();
         // the logits run ahead by two units: K0 K1 V0 K2 V1 ... for two query tiles, K0 K1 K2 V0 K3 V1 ... for one
-        const int loads = 2 * tiles, ahead = min(tiles, q_tiles == 2 ? 1 : 2);
+        const int loads = 2 * tiles;
         for (; issued < loads; ++issued) {
             const int it = issued;
             if (ctl.withhold_from >= 0 && it >= ctl.withhold_from) ok = false;
@@ -428,53 +430,56 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         if (!ok && lane == 0) tc_fail(sh, ctl, 1);
     } else if (warp == 9) {
-        // ---- products: logits of units 0 and 1, then (logits of unit u + 2, output of unit u)
+        // ---- logits
         const bool leader = tc_elect();
-        int used = 0, key_slot = 0, value_slot = 0;
-        auto take = [&](int& slot) {  // the next tile of the ring
-            slot = used % kStages;
-            const bool good = tc_wait_warp(&sh->full[slot], (used / kStages) & 1, limit, failed);
-            ++used;
-            tc_fence_after();
-            return good;
-        };
-        auto logits = [&](int u) {
+        bool ok = tc_wait_warp(&sh->fixed_full, 0, limit, failed);
+        int slot = 0;
+        for (int u = 0; u < units && ok; ++u) {
             const bool first = q_tiles == 1 || !(u & 1), last = q_tiles == 1 || (u & 1);
-            if (first && !take(key_slot)) return false;
-            if (u >= 2) {  // the rows of unit u - 2 have been read
-                if (!tc_wait_warp(&sh->s_free[u & 1], ((u >> 1) - 1) & 1, limit, failed)) return false;
-                tc_fence_after();
+            if (first) {  // key tile j is load j, or from `ahead` on every other one (an even ring: no value tile was in its slot)
+                const int j = q_tiles == 2 ? u >> 1 : u, it = j < ahead ? j : 2 * j - ahead;
+                slot = it % kStages;
+                ok = tc_wait_warp(&sh->full[slot], (it / kStages) & 1, limit, failed);
             }
-            const int t = q_tiles == 2 ? u & 1 : 0;
+            if (u >= 2) ok = ok && tc_wait_warp(&sh->s_free[u & 1], ((u >> 1) - 1) & 1, limit, failed);  // unit u - 2 has been read
+            if (!ok) break;
+            tc_fence_after();
             if (leader) {
-                tc_rows_by_rows<NP, GR, BN>(tmem + (u & 1) * BN, smem_u32(smem + t * NP * GR * kTcRows * 128),
-                                            smem_u32(ring + key_slot * Cfg::kSlot), steps);
-                if (last) tc_commit(&sh->empty[key_slot]);
+                tc_rows_by_rows<NP, GR, BN>(tmem + (u & 1) * BN, smem_u32(smem + (q_tiles == 2 ? u & 1 : 0) * NP * GR * kTcRows * 128),
+                                            smem_u32(ring + slot * Cfg::kSlot), steps);
+                if (last) tc_commit(&sh->empty[slot]);
                 tc_commit(&sh->s_full[u & 1]);
             }
             __syncwarp();
-            return true;
-        };
-        auto weigh = [&](int u) {
+        }
+        tc_finish_products(sh, ctl, ok, leader, false);
+    } else if (warp == 10) {
+        // ---- sums of the values
+        const bool leader = tc_elect();
+        bool ok = true;
+        int slot = 0;
+        for (int u = 0; u < units && ok; ++u) {
             const bool first = q_tiles == 1 || !(u & 1), last = q_tiles == 1 || (u & 1);
-            if (first && !take(value_slot)) return false;
-            if (!tc_wait_warp(&sh->e_ready[u & 1], (u >> 1) & 1, limit, failed)) return false;
-            tc_fence_after();
             const int j = q_tiles == 2 ? u >> 1 : u, valid = j == tiles - 1 ? last_valid : BN;
+            // First the probabilities: they exist only after the logits of this unit, hence after every key tile that can have been
+            // in this value tile's slot before it (the ring has at least four slots), so the slot's barrier is not a phase behind.
+            ok = tc_wait_warp(&sh->e_ready[u & 1], (u >> 1) & 1, limit, failed);
+            if (first) {
+                const int it = j < tiles - ahead ? ahead + 2 * j + 1 : tiles + j;
+                slot = it % kStages;
+                ok = ok && tc_wait_warp(&sh->full[slot], (it / kStages) & 1, limit, failed);
+            }
+            if (!ok) break;
+            tc_fence_after();
             if (leader) {
                 tc_weights_by_rows<NP, GR, BN>(acc + (u & 1) * GR * 64, tmem + Cfg::kWeights + (u & 1) * Cfg::kWeightCols,
-                                               smem_u32(ring + value_slot * Cfg::kSlot), n_out, (valid + 15) >> 4, NP == 1 && u >= 2);
-                if (last) tc_commit(&sh->empty[value_slot]);
+                                               smem_u32(ring + slot * Cfg::kSlot), n_out, (valid + 15) >> 4, NP == 1 && u >= 2);
+                if (last) tc_commit(&sh->empty[slot]);
                 tc_commit(&sh->e_done[u & 1]);
             }
             __syncwarp();
-            return true;
-        };
-        bool ok = tc_wait_warp(&sh->fixed_full, 0, limit, failed);
-        tc_fence_after();
-        ok = ok && logits(0) && (units < 2 || logits(1));
-        for (int u = 0; u < units && ok; ++u) ok = (u + 2 >= units || logits(u + 2)) && weigh(u);
-        tc_finish_products(sh, ctl, ok, leader);
+        }
+        tc_finish_products(sh, ctl, ok, leader, true);
     }
 
     const int group = warp >> 2, row = threadIdx.x & 127;
@@ -721,7 +726,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
             }
         return;
     }
-    const uint32_t tmem = tc_begin<512>(sh, kStages);
+    const uint32_t tmem = tc_begin<512>(sh, kStages, 2);
     const int tiles = (int)((end - begin + BN - 1) / BN), units = tiles * (KEYS ? share : 1);
     const int last_valid = (int)(end - begin) - (tiles - 1) * BN;
     const int steps = (a.size + 15) >> 4, n_out = steps * 16;
@@ -732,13 +737,12 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
 
     int issued = 0;
     if (warp == 8) {
-        // ---- loader: a barrier for each of the two tiles that stay, and for each tile of a slot
+        // ---- loader: the two tiles of a slot share a barrier
         bool ok = true;
         if (lane == 0) {  // rows behind the cloud's last one: see the forward kernel
-            mbar_expect_tx(&sh->fixed_full, Cfg::kFixed);
+            mbar_expect_tx(&sh->fixed_full, 2 * Cfg::kFixed);
             tc_load_whole<kTcRows, NP, GR>(smem, &map_f1, num_rows, head, row0, &sh->fixed_full);
-            mbar_expect_tx(&sh->fixed_full2, Cfg::kFixed);
-            tc_load_whole<kTcRows, NP, GR>(smem + Cfg::kFixed, &map_f2, num_rows, head, row0, &sh->fixed_full2);
+            tc_load_whole<kTcRows, NP, GR>(smem + Cfg::kFixed, &map_f2, num_rows, head, row0, &sh->fixed_full);
         }
         __syncwarp();
         // KEYS: the columns' statistics of the next unit are on their way while the loader waits for its slot
@@ -773,17 +777,18 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                 fetch(issued + 1);
             }
             tc_load_tile<BN, NP, GR>(slot, &map_y1, &map_y18, rows_y1, num_stream, h, from, valid, a.size, &sh->full[s]);
-            tc_load_tile<BN, NP, GR>(slot + Cfg::kTile, &map_y2, &map_y28, rows_y2, num_stream, h, from, valid, a.size, &sh->full2[s]);
+            tc_load_tile<BN, NP, GR>(slot + Cfg::kTile, &map_y2, &map_y28, rows_y2, num_stream, h, from, valid, a.size, &sh->full[s]);
         }
         if (!ok && lane == 0) tc_fail(sh, ctl, 1);
     } else if (warp == 9) {
+        // ---- logits
         const bool leader = tc_elect();
-        // ---- products: logits of units 0 and 1, then (logits of unit u + 2, sums of unit u)
-        auto logits = [&](int u) {
+        bool ok = tc_wait_warp(&sh->fixed_full, 0, limit, failed);
+        for (int u = 0; u < units && ok; ++u) {
             const int s = u % kStages;
-            if (!tc_wait_warp(&sh->full[s], (u / kStages) & 1, limit, failed)) return false;
-            if (!tc_wait_warp(&sh->full2[s], (u / kStages) & 1, limit, failed)) return false;
-            if (u >= 2 && !tc_wait_warp(&sh->s_free[u & 1], ((u >> 1) - 1) & 1, limit, failed)) return false;
+            ok = tc_wait_warp(&sh->full[s], (u / kStages) & 1, limit, failed);
+            if (u >= 2) ok = ok && tc_wait_warp(&sh->s_free[u & 1], ((u >> 1) - 1) & 1, limit, failed);  // unit u - 2 has been read
+            if (!ok) break;
             tc_fence_after();
             const uint32_t buf = tmem + (u & 1) * 2 * BN, slot = smem_u32(ring + s * 2 * Cfg::kTile);
             if (leader) {
@@ -792,12 +797,17 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                 tc_commit(&sh->s_full[u & 1]);
             }
             __syncwarp();
-            return true;
-        };
-        auto weigh = [&](int u) {
-            if (!tc_wait_warp(&sh->e_ready[u & 1], (u >> 1) & 1, limit, failed)) return false;
+        }
+        tc_finish_products(sh, ctl, ok, leader, false);
+    } else if (warp == 10) {
+        // ---- sums
+        const bool leader = tc_elect();
+        bool ok = true;
+        for (int u = 0; u < units && ok; ++u) {
+            ok = tc_wait_warp(&sh->e_ready[u & 1], (u >> 1) & 1, limit, failed);
             const bool fresh = u == 0 || (NP == 3 && u % Cfg::kRound == 0);
-            if (u > 0 && fresh && !tc_wait_warp(&sh->acc_free, (u / Cfg::kRound - 1) & 1, limit, failed)) return false;
+            if (u > 0 && fresh) ok = ok && tc_wait_warp(&sh->acc_free, (u / Cfg::kRound - 1) & 1, limit, failed);
+            if (!ok) break;
             tc_fence_after();
             const int s = u % kStages, valid = u % tiles == tiles - 1 ? last_valid : BN;
             const uint32_t weights = tmem + Cfg::kWeights + (u & 1) * Cfg::kWeightCols, slot = smem_u32(ring + s * 2 * Cfg::kTile);
@@ -811,13 +821,8 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                 if (NP == 3 && (u + 1) % Cfg::kRound == 0 && u + 1 < units) tc_commit(&sh->round_done);
             }
             __syncwarp();
-            return true;
-        };
-        bool ok = tc_wait_warp(&sh->fixed_full, 0, limit, failed) && tc_wait_warp(&sh->fixed_full2, 0, limit, failed);
-        tc_fence_after();
-        ok = ok && logits(0) && (units < 2 || logits(1));
-        for (int u = 0; u < units && ok; ++u) ok = (u + 2 >= units || logits(u + 2)) && weigh(u);
-        tc_finish_products(sh, ctl, ok, leader);
+        }
+        tc_finish_products(sh, ctl, ok, leader, true);
     }
 
     const int group = warp >> 2, row = threadIdx.x & 127;
@@ -909,11 +914,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
     }
     __syncthreads();
     const bool good = !*failed;
-    if (!good && warp == 8) {
-        mbar_wait(&sh->fixed_full2, 0, limit);
-        for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i) mbar_wait(&sh->full2[i % kStages], (i / kStages) & 1, limit);
-        tc_drain_loads(sh, issued, kStages, limit);
-    }
+    if (!good && warp == 8) tc_drain_loads(sh, issued, kStages, limit);
     if (good && warp < 8) {
         const float factor = KEYS && group == 1 ? 1.f : a.scale;
         const int64_t at = out0 + (int64_t)row * out_heads * a.size;

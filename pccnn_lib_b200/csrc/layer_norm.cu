@@ -284,28 +284,36 @@ layer_norm_grads_wide_kernel(int64_t rows, int channels, const T* __restrict__ f
     }
 }
 
-// Column sums of the blocks' rows: 32 columns x 8 row strides per block, added in a fixed order.
-__global__ void __launch_bounds__(256)
+// Column sums of the blocks' rows: 32 columns x 32 row strides per block, added in a fixed order.
+__global__ void __launch_bounds__(1024)
 column_sums_kernel(int num_rows, int columns, const float* __restrict__ partial, int channels, float* __restrict__ weight_grads,
                    float* __restrict__ bias_grads) {
-    __shared__ float part[8][33];
+    __shared__ float part[32][33];
     const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float sum = 0.f;
-    if (c < columns)
-        for (int r = slice; r < num_rows; r += 8) sum += partial[(int64_t)r * columns + c];
+    if (c < columns) {
+#pragma unroll 8
+        for (int r = slice; r < num_rows; r += 32) sum += partial[(int64_t)r * columns + c];
+    }
     part[slice][lane] = sum;
     __syncthreads();
-    if (slice == 0 && c < columns) {
-        for (int s = 1; s < 8; ++s) sum += part[s][lane];
-        if (c < channels) weight_grads[c] = sum;
-        else bias_grads[c - channels] = sum;
+    sum = warp_sum(part[lane][slice]);  // warp s adds column s
+    const int column = blockIdx.x * 32 + slice;
+    if (lane == 0 && column < columns) {
+        if (column < channels) weight_grads[column] = sum;
+        else bias_grads[column - channels] = sum;
     }
 }
 
-constexpr int kNormMaxBlocksPerSm = 4;
+constexpr int kNormMaxBlocksPerSm = 8;
 
-static int norm_blocks(int64_t rows, int rows_per_block) {
-    const int64_t need = (rows + rows_per_block - 1) / rows_per_block, cap = (int64_t)sm_count() * kNormMaxBlocksPerSm;
+// Blocks of the backward kernel: what is resident at once (every block writes a row of partial sums), at most the rows' share.
+template <class Kernel>
+static int norm_blocks(Kernel kernel, size_t shared, int64_t rows, int rows_per_block) {
+    int per_sm = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kNormThreads, shared) != cudaSuccess || per_sm < 1) per_sm = 1;
+    if (per_sm > kNormMaxBlocksPerSm) per_sm = kNormMaxBlocksPerSm;
+    const int64_t need = (rows + rows_per_block - 1) / rows_per_block, cap = (int64_t)sm_count() * per_sm;
     return (int)(need < 1 ? 1 : need < cap ? need : cap);
 }
 
@@ -329,12 +337,13 @@ static int dispatch_norm(int channels, bool vectors, const Launch& launch) {
     if (channels <= 32) return launch.template run<T, 1, 8, 4, 4>();
     if (channels <= 128) return launch.template run<T, 1, 32, 4, 4>();
     if (channels <= 512) return launch.template run<T, 1, 32, 16, 1>();
-    if (channels <= 1024) return launch.template run<T, 1, 256, 4, 4>();
+    if (channels <= 1024) return Launch::kBackward ? launch.template run<T, 1, 256, 4, 1>() : launch.template run<T, 1, 32, 32, 1>();
     if (channels <= 4096) return launch.template run<T, 1, 256, 16, 1>();
     return launch.template wide<T>();
 }
 
 struct NormForward {
+    static constexpr bool kBackward = false;
     int64_t rows; int channels; const void* feats; int64_t ld; const float *weights, *bias; float eps;
     void* out; float *mean, *rstd; cudaStream_t s;
     template <class T, int V, int TPR, int K, int R> int run() const {
@@ -354,22 +363,24 @@ struct NormForward {
 };
 
 struct NormBackward {
+    static constexpr bool kBackward = true;
     int64_t rows; int channels; const void* feats; int64_t ld; const float *weights, *mean, *rstd; const void* grads;
     int64_t ld_g; void* out; float *weight_grads, *bias_grads, *partial; cudaStream_t s;
     int sums(int blocks) const {
-        column_sums_kernel<<<(2 * channels + 31) / 32, 256, 0, s>>>(blocks, 2 * channels, partial, channels, weight_grads, bias_grads);
+        column_sums_kernel<<<(2 * channels + 31) / 32, 1024, 0, s>>>(blocks, 2 * channels, partial, channels, weight_grads, bias_grads);
         PCCNN_LAUNCH_CHECK();
         return PCCNN_OK;
     }
     template <class T, int V, int TPR, int K, int R> int run() const {
-        const int blocks = norm_blocks(rows, kNormThreads / TPR * R);
-        layer_norm_grads_kernel<T, V, TPR, K, R><<<blocks, kNormThreads, TPR < kNormThreads ? (size_t)2 * channels * 4 : 0, s>>>(
+        const size_t shared = TPR < kNormThreads ? (size_t)2 * channels * 4 : 0;
+        const int blocks = norm_blocks(layer_norm_grads_kernel<T, V, TPR, K, R>, shared, rows, kNormThreads / TPR * R);
+        layer_norm_grads_kernel<T, V, TPR, K, R><<<blocks, kNormThreads, shared, s>>>(
             rows, channels, (const T*)feats, ld, weights, mean, rstd, (const T*)grads, ld_g, (T*)out, partial);
         PCCNN_LAUNCH_CHECK();
         return sums(blocks);
     }
     template <class T> int wide() const {
-        const int blocks = norm_blocks(rows, 1);
+        const int blocks = norm_blocks(layer_norm_grads_wide_kernel<T>, 0, rows, 1);
         layer_norm_grads_wide_kernel<T><<<blocks, kNormThreads, 0, s>>>(rows, channels, (const T*)feats, ld, weights, mean, rstd,
                                                                        (const T*)grads, ld_g, (T*)out, partial);
         PCCNN_LAUNCH_CHECK();
