@@ -211,27 +211,38 @@ __device__ __forceinline__ void tc_weights_by_rows(uint32_t d, uint32_t e, uint3
 }
 
 // ---- element-wise ------------------------------------------------------------------------------------------------
-// 32 values of this thread's row as bf16 planes into tensor memory, 16 columns of each plane.
-template <int NP, int PLANE_COLS>
-__device__ __forceinline__ void tc_store_weights(uint32_t dst, const float (&p)[32]) {
-    uint32_t w[16];
+__device__ __forceinline__ unsigned long long add_f32x2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// N values of this thread's row as bf16 planes into tensor memory, N / 2 columns of each plane.
+template <int N>
+__device__ __forceinline__ void tc_store_columns(uint32_t dst, const uint32_t (&w)[N / 2]) {
+    if constexpr (N == 32) tc_st_32x16(dst, w);
+    else tc_st_32x8(dst, w);
+}
+template <int NP, int PLANE_COLS, int N>
+__device__ __forceinline__ void tc_store_weights(uint32_t dst, const float (&p)[N]) {
+    uint32_t w[N / 2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = pack_bf16(p[2 * i], p[2 * i + 1]);
-    tc_st_32x16(dst, w);
+    for (int i = 0; i < N / 2; ++i) w[i] = pack_bf16(p[2 * i], p[2 * i + 1]);
+    tc_store_columns<N>(dst, w);
     if constexpr (NP == 3) {
-        float r[32];
+        float r[N];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < N / 2; ++i) {
             r[2 * i] = p[2 * i] - __uint_as_float(w[i] << 16);
             r[2 * i + 1] = p[2 * i + 1] - __uint_as_float(w[i] & 0xffff0000u);
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = pack_bf16(r[2 * i], r[2 * i + 1]);
-        tc_st_32x16(dst + PLANE_COLS, w);
+        for (int i = 0; i < N / 2; ++i) w[i] = pack_bf16(r[2 * i], r[2 * i + 1]);
+        tc_store_columns<N>(dst + PLANE_COLS, w);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int i = 0; i < N / 2; ++i)
             w[i] = pack_bf16(r[2 * i] - __uint_as_float(w[i] << 16), r[2 * i + 1] - __uint_as_float(w[i] & 0xffff0000u));
-        tc_st_32x16(dst + 2 * PLANE_COLS, w);
+        tc_store_columns<N>(dst + 2 * PLANE_COLS, w);
     }
 }
 
@@ -545,23 +556,30 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 }
             }
             const float from = base == -INFINITY ? 0.f : base;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const unsigned long long scale2 = pack_f32x2(c2, c2), from2 = pack_f32x2(-from, -from);
+            unsigned long long sum[2] = {0ull, 0ull};
 #pragma unroll
             for (int i = 0; i < BN / 32; ++i) {
                 float p[32];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) p[e] = exp2_fast(fmaf(__uint_as_float(s[i][e]), c2, -from));
+                for (int e = 0; e < 32; e += 2) {
+                    unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1])), scale2, from2), p[e], p[e + 1]);
+                    p[e] = exp2_fast(p[e]);
+                    p[e + 1] = exp2_fast(p[e + 1]);
+                }
                 if (valid < BN) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
                         if (i * 32 + e >= valid) p[e] = 0.f;
                 }
 #pragma unroll
-                for (int e = 0; e < 32; ++e) sum[e & 3] += p[e];
+                for (int e = 0; e < 32; e += 2) sum[(e >> 1) & 1] = add_f32x2(sum[(e >> 1) & 1], pack_f32x2(p[e], p[e + 1]));
                 // rounded to bf16 (NP = 1) only as the weights of the values; their sum is taken before
                 tc_store_weights<NP, BN / 2>(weights + 16 * i, p);
             }
-            total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            float sum0, sum1;
+            unpack_f32x2(add_f32x2(sum[0], sum[1]), sum0, sum1);
+            total += sum0 + sum1;
             tc_wait_st();
             tc_arrive_warp(&sh->e_ready[group]);
         }
@@ -862,41 +880,61 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
             tc_fence_after();
             const int valid = u % tiles == tiles - 1 ? last_valid : BN;
             const float* stats = column_stats + (u % kStages) * 2 * BN;
+            if constexpr (KEYS) {
+                // 16 columns at a time, their statistics read ahead of the tensor memory: the products' operands keep the
+                // shared memory busy
+                float4 base[4], d[4];
+                auto read_stats = [&](int i) {
 #pragma unroll
-            for (int i = 0; i < BN / 32; ++i) {
-                uint32_t s[32], t[32];
-                tc_ld_32x32(buf + 32 * i, s);
-                tc_ld_32x32(buf + BN + 32 * i, t);
-                if (i == BN / 32 - 1) tc_arrive_warp(&sh->s_free[group]);
-                if (i == 0 && u >= 2) {  // the group's last unit has been added: its columns of weights are free
-                    if (!(ok = tc_wait_warp(&sh->e_done[group], ((u >> 1) - 1) & 1, limit, failed))) break;
-                    tc_fence_after();
-                }
-                float p[32], e[32];
-#pragma unroll
-                for (int c = 0; c < 32; c += 4) {
-                    float4 base = make_float4(row_base, row_base, row_base, row_base), d = make_float4(row_delta, row_delta, row_delta, row_delta);
-                    if (KEYS) {
-                        base = *reinterpret_cast<const float4*>(stats + i * 32 + c);
-                        d = *reinterpret_cast<const float4*>(stats + BN + i * 32 + c);
+                    for (int c = 0; c < 4; ++c) {
+                        base[c] = *reinterpret_cast<const float4*>(stats + i * 16 + 4 * c);
+                        d[c] = *reinterpret_cast<const float4*>(stats + BN + i * 16 + 4 * c);
                     }
-                    p[c] = exp2_fast(fmaf(__uint_as_float(s[c]), c2, -base.x));
-                    p[c + 1] = exp2_fast(fmaf(__uint_as_float(s[c + 1]), c2, -base.y));
-                    p[c + 2] = exp2_fast(fmaf(__uint_as_float(s[c + 2]), c2, -base.z));
-                    p[c + 3] = exp2_fast(fmaf(__uint_as_float(s[c + 3]), c2, -base.w));
-                    e[c] = p[c] * (__uint_as_float(t[c]) - d.x);
-                    e[c + 1] = p[c + 1] * (__uint_as_float(t[c + 1]) - d.y);
-                    e[c + 2] = p[c + 2] * (__uint_as_float(t[c + 2]) - d.z);
-                    e[c + 3] = p[c + 3] * (__uint_as_float(t[c + 3]) - d.w);
-                }
-                if (!KEYS && valid < BN) {
+                };
+                read_stats(0);
 #pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (i * 32 + c >= valid) e[c] = 0.f;  // a key behind the cloud: its probability may overflow
+                for (int i = 0; i < BN / 16; ++i) {
+                    uint32_t s[16], t[16];
+                    tc_ld_32x16(buf + 16 * i, s);
+                    tc_ld_32x16(buf + BN + 16 * i, t);
+                    if (i == BN / 16 - 1) tc_arrive_warp(&sh->s_free[group]);
+                    float p[16], e[16];
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        p[c] = exp2_fast(fmaf(__uint_as_float(s[c]), c2, -(&base[c / 4].x)[c % 4]));
+                        e[c] = p[c] * (__uint_as_float(t[c]) - (&d[c / 4].x)[c % 4]);
+                    }
+                    if (i + 1 < BN / 16) read_stats(i + 1);
+                    if (i == 0 && u >= 2) {  // the group's last unit has been added: its columns of weights are free
+                        if (!(ok = tc_wait_warp(&sh->e_done[group], ((u >> 1) - 1) & 1, limit, failed))) break;
+                        tc_fence_after();
+                    }
+                    // rounded to bf16 (NP = 1) as the weights of the last two products, as the probabilities of the forward pass
+                    tc_store_weights<NP, Cfg::kPlane>(weights + 8 * i, e);
+                    tc_store_weights<NP, Cfg::kPlane>(weights + NP * Cfg::kPlane + 8 * i, p);
                 }
-                // rounded to bf16 (NP = 1) as the weights of the last two products, as the probabilities of the forward pass
-                tc_store_weights<NP, Cfg::kPlane>(weights + 16 * i, e);
-                if (KEYS) tc_store_weights<NP, Cfg::kPlane>(weights + NP * Cfg::kPlane + 16 * i, p);
+            } else {
+                uint32_t s[BN / 32][32], t[BN / 32][32];
+#pragma unroll
+                for (int i = 0; i < BN / 32; ++i) {
+                    tc_ld_32x32(buf + 32 * i, s[i]);
+                    tc_ld_32x32(buf + BN + 32 * i, t[i]);
+                }
+                tc_arrive_warp(&sh->s_free[group]);
+#pragma unroll
+                for (int i = 0; i < BN / 32; ++i) {
+                    float e[32];
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) {
+                        e[c] = exp2_fast(fmaf(__uint_as_float(s[i][c]), c2, -row_base)) * (__uint_as_float(t[i][c]) - row_delta);
+                        if (valid < BN && i * 32 + c >= valid) e[c] = 0.f;  // a key behind the cloud: its probability may overflow
+                    }
+                    if (i == 0 && u >= 2) {
+                        if (!(ok = tc_wait_warp(&sh->e_done[group], ((u >> 1) - 1) & 1, limit, failed))) break;
+                        tc_fence_after();
+                    }
+                    tc_store_weights<NP, Cfg::kPlane>(weights + 16 * i, e);
+                }
             }
             if (!ok) break;
             tc_wait_st();

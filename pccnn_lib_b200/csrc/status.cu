@@ -53,12 +53,13 @@ int publish_status(const int* status_dev, int origin, cudaStream_t s) {
 }
 
 int* sticky_status_device() {
-    int* sticky = sticky_status_word();
-    int* dev = nullptr;
-    if (!sticky || cudaHostGetDevicePointer((void**)&dev, sticky, 0) != cudaSuccess) {
-        set_error("no pinned status word: %s", cudaGetErrorString(g_status_err));
-        return nullptr;
-    }
+    static std::once_flag once;
+    static int* dev = nullptr;  // portable memory of one address space: the same address on every device
+    std::call_once(once, [] {
+        int* sticky = sticky_status_word();
+        if (!sticky || cudaHostGetDevicePointer((void**)&dev, sticky, 0) != cudaSuccess) dev = nullptr;
+    });
+    if (!dev) set_error("no pinned status word: %s", cudaGetErrorString(g_status_err));
     return dev;
 }
 

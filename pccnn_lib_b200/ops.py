@@ -44,8 +44,11 @@ def _p(t):
     return None if t is None or t.numel() == 0 else t.data_ptr()
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the handle without a Stream object around it
+
+
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    return torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(torch.cuda.current_device())
 
 
 _SAME_DEVICE = contextlib.nullcontext()
