@@ -27,33 +27,44 @@ static int allow_shared(Kernel kernel, int bytes, std::atomic<uint64_t>& done) {
     return PCCNN_OK;
 }
 
-// x -> (h, m, l): planes [3][rows, heads, size] of bf16.  size is a multiple of 8; one thread per 8 features.
+// x -> (h, m, l): planes [3][rows, heads, size] of bf16, for the tensors of one call (blockIdx.y).  size is a multiple of 8; one
+// thread per 8 features.
+struct SplitTensor {
+    const float* src;
+    int64_t row, head, rows;
+    int heads;
+    bool vectors;
+    __nv_bfloat16* planes;
+};
+struct SplitTensors {
+    SplitTensor t[4];
+};
 __global__ void __launch_bounds__(256)
-split_planes_kernel(int64_t rows, int heads, int size, const float* __restrict__ src, int64_t row_stride, int64_t head_stride, bool vectors,
-                    __nv_bfloat16* __restrict__ planes) {
-    const int per_head = size / 8, per_row = heads * per_head;
-    const int64_t total = rows * per_row, plane = rows * heads * size;
+split_planes_kernel(const __grid_constant__ SplitTensors all, int size) {
+    const SplitTensor& x = all.t[blockIdx.y];
+    const int per_head = size / 8, per_row = x.heads * per_head;
+    const int64_t total = x.rows * per_row, plane = x.rows * x.heads * size;
     for (int64_t i = blockIdx.x * 256LL + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / per_row;
         const int in_row = (int)(i - r * per_row), h = in_row / per_head, c = (in_row - h * per_head) * 8;
-        const float* p = src + r * row_stride + h * head_stride + c;
-        float x[8];
-        if (vectors) {
-            load_vec<float, 8>(p, x);
+        const float* p = x.src + r * x.row + h * x.head + c;
+        float v[8];
+        if (x.vectors) {
+            load_vec<float, 8>(p, v);
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = p[e];
+            for (int e = 0; e < 8; ++e) v[e] = p[e];
         }
 #pragma unroll
         for (int k = 0; k < 3; ++k) {
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                w[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
-                x[2 * e] -= __uint_as_float(w[e] << 16);
-                x[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
+                w[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+                v[2 * e] -= __uint_as_float(w[e] << 16);
+                v[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
             }
-            *reinterpret_cast<uint4*>(planes + k * plane + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(x.planes + k * plane + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
 }
@@ -65,22 +76,38 @@ struct TcOperand {
     int heads;
 };
 
-static int tc_operand(TcOperand& o, const HeadRows& x, int64_t rows, int heads, int size, bool planes, char*& ws, cudaStream_t s) {
-    o.count = rows;
-    o.heads = heads;
-    if (!planes) {
-        o.rows = {(const __nv_bfloat16*)x.data, x.row, x.head, 0};
+// Describes the tensors of a call, and brings 32-bit ones into planes (one launch for all of them).
+struct TcOperands {
+    TcOperand o[4];
+    SplitTensors split;
+    int n = 0;
+    char* ws;
+    int size;
+    bool planes;
+
+    TcOperands(char* ws_, int size_, bool planes_) : ws(ws_), size(size_), planes(planes_) {}
+    const TcOperand& add(const HeadRows& x, int64_t rows, int heads) {
+        TcOperand& r = o[n];
+        r.count = rows;
+        r.heads = heads;
+        r.rows = {(const __nv_bfloat16*)x.data, x.row, x.head, 0};
+        if (planes) {
+            const int64_t plane = rows * heads * size;
+            r.rows = {(const __nv_bfloat16*)ws, (int64_t)heads * size, size, plane};
+            split.t[n] = {(const float*)x.data, x.row, x.head, rows, heads, aligned16(x.data) && x.row % 4 == 0 && x.head % 4 == 0, (__nv_bfloat16*)ws};
+            ws += align_up((size_t)plane * 6);
+        }
+        return o[n++];
+    }
+    int make_planes(cudaStream_t s) const {
+        if (!planes) return PCCNN_OK;
+        int64_t most = 0;
+        for (int i = 0; i < n; ++i) most = split.t[i].rows * split.t[i].heads > most ? split.t[i].rows * split.t[i].heads : most;
+        split_planes_kernel<<<dim3(grid_for(most * (size / 8), 256, 8), (unsigned)n), 256, 0, s>>>(split, size);
+        PCCNN_LAUNCH_CHECK();
         return PCCNN_OK;
     }
-    const int64_t plane = rows * heads * size;
-    o.rows = {(const __nv_bfloat16*)ws, (int64_t)heads * size, size, plane};
-    const bool vectors = aligned16(x.data) && x.row % 4 == 0 && x.head % 4 == 0;
-    split_planes_kernel<<<grid_for(plane / 8, 256, 16), 256, 0, s>>>(rows, heads, size, (const float*)x.data, x.row, x.head, vectors,
-                                                                    (__nv_bfloat16*)ws);
-    PCCNN_LAUNCH_CHECK();
-    ws += align_up((size_t)plane * 6);
-    return PCCNN_OK;
-}
+};
 static size_t operand_bytes(int64_t rows, int heads, int size, bool planes) {
     return planes ? align_up((size_t)rows * heads * size * 6) : 0;
 }
@@ -89,11 +116,22 @@ static int operand_map(CUtensorMap* map, const TcOperand& o, int size, bool plan
 }
 
 // ---- which calls ------------------------------------------------------------------------------------------------
-// Tiles of 128 queries pay once a cloud has more than a handful of them; below that the row kernels read the keys once
-// and do no product for absent rows.
+static bool tc_any_shape(const AttentionCall& a) {
+    return a.size % 8 == 0 && a.size <= 128 && a.num_queries > 0 && a.num_keys > 0 && a.num_queries < 0x7fffffffLL / 3 && a.num_keys < 0x7fffffffLL / 3;
+}
+// Multiply-adds of one of the products, with the mean cloud's keys and heads that share keys counted once.
+static double tc_work(const AttentionCall& a) {
+    return (double)a.num_queries * ((double)a.num_keys / (a.clouds > 0 ? a.clouds : 1)) * a.kv_heads * a.size;
+}
+// Forward: tiles, except for
+//  - small calls: 150 queries, 301 keys, 2 clouds, 4 heads of 32: 9.7 us with rows, 13.5 us with tiles in bf16, 11.7 and 20 us in
+//    32 bits; one cloud of 64 queries, 300 keys, 4 heads of 64 (5e6 multiply-adds): 14.1 and 11.6, 21.2 and 19.3 us;
+//  - a query per cloud (or four 32-bit ones, which would have to be split into planes first): 16 queries, 40000 keys, 8 heads
+//    on 2: 35 us with rows, 42 us with tiles in bf16; 64 queries, 40000 keys, 16 clouds, 8 heads, 32 bits: 146 and 183 us,
+//    with 256 queries 458 and 181 us.
 bool tc_shape(const AttentionCall& a) {
-    return a.size % 8 == 0 && a.size <= 128 && a.num_queries > 8 * (int64_t)a.clouds && a.num_keys > 0 && a.num_queries < 0x7fffffffLL / 3 &&
-           a.num_keys < 0x7fffffffLL / 3;
+    if (!tc_any_shape(a) || tc_work(a) < 4e6) return false;
+    return a.is_bf16 ? a.num_queries > a.clouds : a.num_queries * (a.heads / a.kv_heads) > 4 * (int64_t)a.clouds;
 }
 static bool tc_heads(const HeadRows& x) { return aligned16(x.data) && x.row % 8 == 0 && x.head % 8 == 0; }
 bool tc_layout(const AttentionCall& a, const HeadRows* grads) {
@@ -136,10 +174,11 @@ static int launch_forward(const AttentionCall& a, void* out, float* lse, char* w
     if (int rc = allow_shared(kernel, Cfg::kBytes, done)) return rc;
     TcControl ctl;
     if (int rc = tc_control(ctl)) return rc;
-    TcOperand q, k, v;
-    if (int rc = tc_operand(q, a.q, a.num_queries, a.heads, a.size, NP == 3, ws, s)) return rc;
-    if (int rc = tc_operand(k, a.k, a.num_keys, a.kv_heads, a.size, NP == 3, ws, s)) return rc;
-    if (int rc = tc_operand(v, a.v, a.num_keys, a.kv_heads, a.size, NP == 3, ws, s)) return rc;
+    TcOperands operands(ws, a.size, NP == 3);
+    const TcOperand &q = operands.add(a.q, a.num_queries, a.heads), &k = operands.add(a.k, a.num_keys, a.kv_heads),
+                    &v = operands.add(a.v, a.num_keys, a.kv_heads);
+    if (int rc = operands.make_planes(s)) return rc;
+    ws = operands.ws;
     CUtensorMap map_q, map_k, map_v, map_k8, map_v8;
     if (int rc = operand_map(&map_q, q, a.size, NP == 3, kTcRows)) return rc;
     if (int rc = operand_map(&map_k, k, a.size, NP == 3, BN)) return rc;
@@ -162,10 +201,13 @@ int tc_forward(const AttentionCall& a, void* out, float* lse, char* ws, cudaStre
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------
-// The tiles that stay in shared memory: 32-bit heads of more than 64 features need 192 KB for them alone and take the row kernels.
+// Backward: tiles, except for small 32-bit calls (150 queries, 301 keys, 2 clouds, 4 heads of 32: 24 us with rows, 40 us with
+// tiles; 300 queries, 600 keys, 4 heads of 64: 107 and 65 us; in bf16 tiles are faster from one query on: 20.4 and 19.1 us for
+// one query and 300 keys) and for 32-bit heads of more than 64 features, whose tiles that stay in shared memory take 192 KB.
 // The streamed tiles of all heads that share a key head are counted in 32 bits.
 bool tc_grads_shape(const AttentionCall& a) {
-    return tc_shape(a) && (a.is_bf16 || a.size <= 64) && (a.num_queries / 64 + 1) * (a.heads / a.kv_heads) < 0x7fffffffLL;
+    return tc_any_shape(a) && (a.is_bf16 || (a.size <= 64 && tc_work(a) >= 6e6)) &&
+           (a.num_queries / 32 + 1) * (a.heads / a.kv_heads) < 0x7fffffffLL;
 }
 
 static int tc_grad_splits(const AttentionCall& a, bool keys) {
@@ -217,11 +259,11 @@ static int launch_grads(const AttentionCall& a, const TcOperand& f1, const TcOpe
 template <int GR, int NP, class T>
 static int launch_both_grads(const AttentionCall& a, const HeadRows& grads, const float* lse, const float* delta, void* dq, void* dk, void* dv,
                              char* ws, cudaStream_t s) {
-    TcOperand q, k, v, g;
-    if (int rc = tc_operand(q, a.q, a.num_queries, a.heads, a.size, NP == 3, ws, s)) return rc;
-    if (int rc = tc_operand(g, grads, a.num_queries, a.heads, a.size, NP == 3, ws, s)) return rc;
-    if (int rc = tc_operand(k, a.k, a.num_keys, a.kv_heads, a.size, NP == 3, ws, s)) return rc;
-    if (int rc = tc_operand(v, a.v, a.num_keys, a.kv_heads, a.size, NP == 3, ws, s)) return rc;
+    TcOperands operands(ws, a.size, NP == 3);
+    const TcOperand &q = operands.add(a.q, a.num_queries, a.heads), &g = operands.add(grads, a.num_queries, a.heads),
+                    &k = operands.add(a.k, a.num_keys, a.kv_heads), &v = operands.add(a.v, a.num_keys, a.kv_heads);
+    if (int rc = operands.make_planes(s)) return rc;
+    ws = operands.ws;
     if (int rc = launch_grads<false, GR, NP, T>(a, q, g, k, v, lse, delta, dq, nullptr, ws, s)) return rc;
     return launch_grads<true, GR, NP, T>(a, k, v, q, g, lse, delta, dk, dv, ws, s);
 }

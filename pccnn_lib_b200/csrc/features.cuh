@@ -1,5 +1,5 @@
-// Loads and stores of feature vectors in float32 or bfloat16: V consecutive elements as one 16-byte access where V says
-// so, as single elements for V = 1 (and element by element for the other small V).  Arithmetic is 32-bit throughout.
+// Loads and stores of feature vectors in float32 or bfloat16: V consecutive elements (1, 2, 4 or 8) as accesses of up to 16
+// bytes, which the address has to be aligned to.  Arithmetic is 32-bit throughout.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -34,9 +34,19 @@ __device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&v)[V])
             v[2 * i] = __uint_as_float(w[i] << 16);
             v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         }
+    } else if constexpr (sizeof(T) == 4 && V == 2) {
+        const float2 r = *reinterpret_cast<const float2*>(p);
+        v[0] = r.x, v[1] = r.y;
+    } else if constexpr (sizeof(T) == 2 && V == 4) {
+        const uint2 r = *reinterpret_cast<const uint2*>(p);
+        v[0] = __uint_as_float(r.x << 16), v[1] = __uint_as_float(r.x & 0xffff0000u);
+        v[2] = __uint_as_float(r.y << 16), v[3] = __uint_as_float(r.y & 0xffff0000u);
+    } else if constexpr (sizeof(T) == 2 && V == 2) {
+        const uint32_t r = *reinterpret_cast<const uint32_t*>(p);
+        v[0] = __uint_as_float(r << 16), v[1] = __uint_as_float(r & 0xffff0000u);
     } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = to_float(p[i]);
+        static_assert(V == 1, "1, 2, 4 or 8 elements");
+        v[0] = to_float(p[0]);
     }
 }
 
@@ -53,9 +63,15 @@ __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&v)[V]
     } else if constexpr (sizeof(T) == 2 && V == 8) {
         *reinterpret_cast<uint4*>(p) =
             make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    } else if constexpr (sizeof(T) == 4 && V == 2) {
+        *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+    } else if constexpr (sizeof(T) == 2 && V == 4) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+    } else if constexpr (sizeof(T) == 2 && V == 2) {
+        *reinterpret_cast<uint32_t*>(p) = pack_bf16(v[0], v[1]);
     } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) p[i] = from_float<T>(v[i]);
+        static_assert(V == 1, "1, 2, 4 or 8 elements");
+        p[0] = from_float<T>(v[0]);
     }
 }
 

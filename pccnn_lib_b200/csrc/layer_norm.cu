@@ -10,6 +10,8 @@
 // order: no atomics, the same bits on every run.  Statistics and sums are 32-bit floats whatever the features' type.
 #include <cuda_bf16.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "features.cuh"
 
@@ -317,33 +319,51 @@ static int norm_blocks(Kernel kernel, size_t shared, int64_t rows, int rows_per_
     return (int)(need < 1 ? 1 : need < cap ? need : cap);
 }
 
-// The vector width, threads per row, vectors per thread and rows at once: 16-byte vectors where every row starts on a 16-byte
-// boundary, single elements otherwise; few threads per row while that keeps it to a few vectors each, and then as many rows
-// at once as keep about four vectors (or sixteen single elements) of a thread in flight.
-template <class T, class Launch>
-static int dispatch_norm(int channels, bool vectors, const Launch& launch) {
-    constexpr int kV = 16 / sizeof(T);
-    if (vectors) {
-        const int n = channels / kV;
-        if (n <= 8) return launch.template run<T, kV, 8, 1, 4>();
-        if (n <= 16) return launch.template run<T, kV, 8, 2, 2>();
-        if (n <= 32) return launch.template run<T, kV, 32, 1, 4>();
-        if (n <= 64) return launch.template run<T, kV, 32, 2, 2>();
-        if (n <= 128) return launch.template run<T, kV, 32, 4, 1>();
-        if (n <= 256) return launch.template run<T, kV, 256, 1, 4>();
-        if (n <= 1024) return launch.template run<T, kV, 256, 4, 1>();
-        return launch.template wide<T>();
+// Threads per row, vectors per thread and rows at once for rows of n vectors of V elements: few threads per row while that
+// keeps it to a few vectors each, and then as many rows at once as keep 32 to 64 bytes of a thread in flight.  (A detour of
+// unaligned rows through shared memory with 16-byte accesses was no faster: 20011 x 1001 bf16 36 us forward, 81 us backward,
+// against 41 and 40 us.)
+template <class T, int V, class Launch>
+static int dispatch_rows_of(int n, const Launch& launch) {
+    if constexpr (V * sizeof(T) >= 8) {
+        if (n <= 8) return launch.template run<T, V, 8, 1, 4>();
+        if (n <= 16) return launch.template run<T, V, 8, 2, 2>();
+        if (n <= 32) return launch.template run<T, V, 32, 1, 4>();
+        if (n <= 64) return launch.template run<T, V, 32, 2, 2>();
+        if (n <= 128) return launch.template run<T, V, 32, 4, 1>();
+        if (n <= 256) return launch.template run<T, V, 256, 1, 4>();
+        if (n <= 1024) return launch.template run<T, V, 256, 4, 1>();
+    } else {
+        if (n <= 8) return launch.template run<T, V, 8, 1, 8>();
+        if (n <= 16) return launch.template run<T, V, 8, 2, 4>();
+        if (n <= 32) return launch.template run<T, V, 8, 4, 4>();
+        if (n <= 64) return launch.template run<T, V, 32, 2, 8>();
+        if (n <= 128) return launch.template run<T, V, 32, 4, 4>();
+        if (n <= 256) return launch.template run<T, V, 32, 8, 2>();
+        if (n <= 512) return launch.template run<T, V, 32, 16, 1>();
+        if (n <= 1024) return launch.template run<T, V, 256, 4, 1>();
+        if (n <= 4096) return launch.template run<T, V, 256, 16, 1>();
     }
-    if (channels <= 32) return launch.template run<T, 1, 8, 4, 4>();
-    if (channels <= 128) return launch.template run<T, 1, 32, 4, 4>();
-    if (channels <= 512) return launch.template run<T, 1, 32, 16, 1>();
-    if (channels <= 1024) return Launch::kBackward ? launch.template run<T, 1, 256, 4, 1>() : launch.template run<T, 1, 32, 32, 1>();
-    if (channels <= 4096) return launch.template run<T, 1, 256, 16, 1>();
     return launch.template wide<T>();
+}
+// `width`: the most elements of one access that every row of every tensor is aligned to.
+template <class T, class Launch>
+static int dispatch_norm(int channels, int width, const Launch& launch) {
+    if constexpr (sizeof(T) == 2) {
+        if (width >= 8) return dispatch_rows_of<T, 8>(channels / 8, launch);
+    }
+    if (width >= 4) return dispatch_rows_of<T, 4>(channels / 4, launch);
+    if (width >= 2) return dispatch_rows_of<T, 2>(channels / 2, launch);
+    return dispatch_rows_of<T, 1>(channels, launch);
+}
+// The largest power of two (at most 16 bytes) that divides the channels and the row stride and fits the address.
+static int row_width(const void* p, int64_t ld, int channels, int element) {
+    int v = 16 / element;
+    while (v > 1 && (channels % v || ld % v || ((uintptr_t)p & (v * element - 1)))) v /= 2;
+    return v;
 }
 
 struct NormForward {
-    static constexpr bool kBackward = false;
     int64_t rows; int channels; const void* feats; int64_t ld; const float *weights, *bias; float eps;
     void* out; float *mean, *rstd; cudaStream_t s;
     template <class T, int V, int TPR, int K, int R> int run() const {
@@ -363,7 +383,6 @@ struct NormForward {
 };
 
 struct NormBackward {
-    static constexpr bool kBackward = true;
     int64_t rows; int channels; const void* feats; int64_t ld; const float *weights, *mean, *rstd; const void* grads;
     int64_t ld_g; void* out; float *weight_grads, *bias_grads, *partial; cudaStream_t s;
     int sums(int blocks) const {
@@ -403,9 +422,11 @@ int pccnn_layer_norm(int64_t rows, int channels, const void* feats, int64_t ld_f
     if (rows == 0) return PCCNN_OK;
     PCCNN_CHECK_ARG(feats && weights && bias && out && out_mean && out_rstd, "layer_norm: null pointer");
     const NormForward f{rows, channels, feats, ld_feats, weights, bias, eps, out, out_mean, out_rstd, (cudaStream_t)stream};
-    const int v = is_bf16 ? 8 : 4;
-    const bool vec = channels % v == 0 && ld_feats % v == 0 && aligned16(feats) && aligned16(weights) && aligned16(bias) && aligned16(out);
-    return is_bf16 ? dispatch_norm<__nv_bfloat16>(channels, vec, f) : dispatch_norm<float>(channels, vec, f);
+    const int e = is_bf16 ? 2 : 4;
+    int width = row_width(feats, rows > 1 ? ld_feats : channels, channels, e);
+    width = std::min({width, row_width(out, channels, channels, e), row_width(weights, channels, channels, 4) * (channels % 8 ? 1 : 2),
+                      row_width(bias, channels, channels, 4) * (channels % 8 ? 1 : 2)});
+    return is_bf16 ? dispatch_norm<__nv_bfloat16>(channels, width, f) : dispatch_norm<float>(channels, width, f);
 }
 
 size_t pccnn_layer_norm_grads_workspace_bytes(int64_t rows, int channels) {
@@ -436,10 +457,11 @@ int pccnn_layer_norm_grads(int64_t rows, int channels, const void* feats, int64_
     }
     const NormBackward b{rows, channels, feats, ld_feats, weights, mean, rstd, in_grads, ld_grads, out_feat_grads,
                          out_weight_grads, out_bias_grads, (float*)workspace, s};
-    const int v = is_bf16 ? 8 : 4;
-    const bool vec = channels % v == 0 && ld_feats % v == 0 && ld_grads % v == 0 && aligned16(feats) && aligned16(weights) &&
-                     aligned16(in_grads) && aligned16(out_feat_grads);
-    return is_bf16 ? dispatch_norm<__nv_bfloat16>(channels, vec, b) : dispatch_norm<float>(channels, vec, b);
+    const int e = is_bf16 ? 2 : 4;
+    const int width = std::min({row_width(feats, rows > 1 ? ld_feats : channels, channels, e), row_width(out_feat_grads, channels, channels, e),
+                                row_width(in_grads, rows > 1 ? ld_grads : channels, channels, e),
+                                row_width(weights, channels, channels, 4) * (channels % 8 ? 1 : 2)});
+    return is_bf16 ? dispatch_norm<__nv_bfloat16>(channels, width, b) : dispatch_norm<float>(channels, width, b);
 }
 
 }  // extern "C"

@@ -44,6 +44,17 @@ __device__ __forceinline__ int axis_of(const RotaryAxes& axes, int pair) {
     return a;
 }
 
+// P > 1: one aligned access.  P = 1: two elements, of which the second may be absent (an odd head size).
+template <class T, int P>
+__device__ __forceinline__ void load_pairs(const T* __restrict__ p, bool whole, float (&x)[2 * P]) {
+    if constexpr (P > 1) {
+        load_vec<T, 2 * P>(p, x);
+    } else {
+        x[0] = to_float(p[0]);
+        x[1] = whole ? to_float(p[1]) : 0.f;
+    }
+}
+
 // P pairs per access, kAtOnce accesses of a lane in flight.  kAxes > 0: `in` is the gradient, turned back, and the
 // coordinates' gradient (of at most kAxes axes) is taken from it and `feats` when pt_grads is given.
 template <class T, int P, int kAxes>
@@ -77,10 +88,9 @@ rotary_kernel(int64_t rows, int heads, int size, const T* __restrict__ in, Rotar
                     const int h = i / accesses, d = (i - h * accesses) * 2 * P;
                     const T* src = in + row * ld_in.row + h * ld_in.head + d;
                     const bool whole = P > 1 || d + 1 < size;  // P > 1: the size is a multiple of the access
-                    if (whole) load_vec<T, 2 * P>(src, x[u]);
-                    else x[u][0] = to_float(src[0]), x[u][1] = 0.f;
+                    load_pairs<T, P>(src, whole, x[u]);
                     if constexpr (kGrads) {
-                        if (both && whole) load_vec<T, 2 * P>(feats + row * ld_feats.row + h * ld_feats.head + d, f[u]);
+                        if (both) load_pairs<T, P>(feats + row * ld_feats.row + h * ld_feats.head + d, whole, f[u]);
                     }
                 }
             }
@@ -121,8 +131,12 @@ rotary_kernel(int64_t rows, int heads, int size, const T* __restrict__ in, Rotar
                             }
                         }
                     }
-                    if (P > 1 || d + 1 < size) store_vec<T, 2 * P>(dst, y);
-                    else dst[0] = from_float<T>(y[0]);
+                    if constexpr (P > 1) {
+                        store_vec<T, 2 * P>(dst, y);
+                    } else {
+                        dst[0] = from_float<T>(y[0]);
+                        if (d + 1 < size) dst[1] = from_float<T>(y[1]);
+                    }
                 }
             }
         }
