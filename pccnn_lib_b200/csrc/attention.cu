@@ -92,36 +92,6 @@ __device__ __forceinline__ void split_range(int64_t& begin, int64_t& end, int s,
 // lane has the next kUnroll keys and values in flight while it works on the last ones, as raw 16-byte vectors.
 // Without splits the output and lse are written; with splits the block leaves its unnormalised sum (relative to its own
 // maximum), the maximum and the sum of the probabilities.
-template <class T, int V> struct RawRow { uint4 v; };
-template <class T> struct RawRow<T, 1> { T v; };
-template <class T, int V>
-__device__ __forceinline__ void load_raw(RawRow<T, V>& r, const T* __restrict__ p) {
-    if constexpr (V == 1) r.v = *p;
-    else r.v = *reinterpret_cast<const uint4*>(p);
-}
-template <class T, int V>
-__device__ __forceinline__ void clear_raw(RawRow<T, V>& r) {
-    if constexpr (V == 1) r.v = from_float<T>(0.f);
-    else r.v = make_uint4(0, 0, 0, 0);
-}
-template <class T, int V>
-__device__ __forceinline__ void widen(const RawRow<T, V>& r, float (&x)[V]) {
-    if constexpr (V == 1) {
-        x[0] = to_float(r.v);
-    } else {
-        const uint32_t w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (V == 4) {
-                x[i] = __uint_as_float(w[i]);
-            } else {
-                x[2 * i] = __uint_as_float(w[i] << 16);
-                x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            }
-        }
-    }
-}
-
 template <class T, int V, int NC, int GH>
 __global__ void __launch_bounds__(kRowThreads)
 attention_row_kernel(AttentionCall a, int lanes_per_row, int warp_heads, int splits, T* __restrict__ out, float* __restrict__ lse,
@@ -159,7 +129,7 @@ attention_row_kernel(AttentionCall a, int lanes_per_row, int warp_heads, int spl
     const T* keys = (const T*)a.k.data + kv * a.k.head;
     const T* values = (const T*)a.v.data + kv * a.v.head;
     const int step = slices * per_warp;
-    RawRow<T, V> key[kUnroll][NC], val[kUnroll][NC];
+    RawVec<T, V> key[kUnroll][NC], val[kUnroll][NC];
     auto fetch = [&](int64_t first) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
@@ -168,11 +138,11 @@ attention_row_kernel(AttentionCall a, int lanes_per_row, int warp_heads, int spl
             for (int c = 0; c < NC; ++c) {
                 const int d = (c * lanes_per_row + in_row) * V;
                 if (n < end && d < a.size) {
-                    load_raw<T, V>(key[u][c], keys + n * a.k.row + d);
-                    load_raw<T, V>(val[u][c], values + n * a.v.row + d);
+                    key[u][c].load(keys + n * a.k.row + d);
+                    val[u][c].load(values + n * a.v.row + d);
                 } else {
-                    clear_raw<T, V>(key[u][c]);
-                    clear_raw<T, V>(val[u][c]);
+                    key[u][c].clear();
+                    val[u][c].clear();
                 }
             }
         }
@@ -185,11 +155,11 @@ attention_row_kernel(AttentionCall a, int lanes_per_row, int warp_heads, int spl
         for (int u = 0; u < kUnroll; ++u) {
             float x[NC][V];
 #pragma unroll
-            for (int c = 0; c < NC; ++c) widen<T, V>(key[u][c], x[c]);
+            for (int c = 0; c < NC; ++c) key[u][c].widen(x[c]);
 #pragma unroll
             for (int g = 0; g < GH; ++g) s[g][u] = dot<V, NC>(q[g], x);
         }
-        RawRow<T, V> now_val[kUnroll][NC];
+        RawVec<T, V> now_val[kUnroll][NC];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
@@ -222,7 +192,7 @@ attention_row_kernel(AttentionCall a, int lanes_per_row, int warp_heads, int spl
         for (int u = 0; u < kUnroll; ++u) {
             float x[NC][V];
 #pragma unroll
-            for (int c = 0; c < NC; ++c) widen<T, V>(now_val[u][c], x[c]);
+            for (int c = 0; c < NC; ++c) now_val[u][c].widen(x[c]);
 #pragma unroll
             for (int g = 0; g < GH; ++g)
 #pragma unroll

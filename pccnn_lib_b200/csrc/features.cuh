@@ -50,6 +50,35 @@ __device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&v)[V])
     }
 }
 
+// The same vector as it lies in memory, for loads that stay in flight while other rows are worked on.
+template <int BYTES> struct RawBytes;
+template <> struct RawBytes<16> { using type = uint4; };
+template <> struct RawBytes<8> { using type = uint2; };
+template <> struct RawBytes<4> { using type = uint32_t; };
+template <> struct RawBytes<2> { using type = uint16_t; };
+template <class T, int V>
+struct RawVec {
+    typename RawBytes<V * sizeof(T)>::type v;
+    __device__ __forceinline__ void load(const T* __restrict__ p) { v = *reinterpret_cast<const decltype(v)*>(p); }
+    __device__ __forceinline__ void clear() { v = decltype(v)(); }
+    __device__ __forceinline__ void widen(float (&x)[V]) const {
+        constexpr int kWords = V * sizeof(T) < 4 ? 1 : V * sizeof(T) / 4;
+        uint32_t w[kWords];
+        if constexpr (sizeof(v) == 16) w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        else if constexpr (sizeof(v) == 8) w[0] = v.x, w[1] = v.y;
+        else w[0] = v;
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                x[i] = __uint_as_float(w[i]);
+            } else {
+                x[2 * i] = __uint_as_float(w[i] << 16);
+                if constexpr (V > 1) x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+    }
+};
+
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);

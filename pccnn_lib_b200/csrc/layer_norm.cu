@@ -45,76 +45,82 @@ __device__ __forceinline__ void row_sums(float (&v)[R], float (*slots)[kNormThre
     }
 }
 
-// R rows per TPR threads at once (their loads are in flight together), K vectors of V elements per thread and row.
+// R rows per TPR threads at once, K vectors of V elements per thread and row.  The blocks are those resident at once and walk
+// the rows; the next rows are on their way while the last ones are worked on.
 template <class T, int V, int TPR, int K, int R>
 __global__ void __launch_bounds__(kNormThreads)
 layer_norm_kernel(int64_t rows, int channels, const T* __restrict__ feats, int64_t ld, const float* __restrict__ weights,
                   const float* __restrict__ bias, float eps, T* __restrict__ out, float* __restrict__ out_mean,
                   float* __restrict__ out_rstd) {
+    constexpr int kGroups = kNormThreads / TPR;
     __shared__ float slots[2][kNormThreads / 32][R];
-    const int t = threadIdx.x % TPR;
-    const int64_t row0 = ((int64_t)blockIdx.x * (kNormThreads / TPR) + threadIdx.x / TPR) * R;
-    float x[R][K][V], mean[R], rstd[R];
+    const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    const int64_t stride = (int64_t)gridDim.x * kGroups * R;
+    RawVec<T, V> next[R][K];
+    auto fetch = [&](int64_t row0) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const T* src = feats + (row0 + i < rows ? row0 + i : 0) * ld;
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int c = (k * TPR + t) * V;
+                if (row0 + i < rows && c < channels) next[i][k].load(feats + (row0 + i) * ld + c);
+                else next[i][k].clear();
+            }
+    };
+    fetch(((int64_t)blockIdx.x * kGroups + group) * R);
+    for (int64_t base = (int64_t)blockIdx.x * kGroups * R; base < rows; base += stride) {  // the same for the block
+        const int64_t row0 = base + group * R;
+        float x[R][K][V], mean[R], rstd[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            mean[i] = 0.f;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                next[i][k].widen(x[i][k]);
+#pragma unroll
+                for (int e = 0; e < V; ++e) mean[i] += x[i][k][e];
+            }
+        }
+        if (base + stride < rows) fetch(row0 + stride);
+        row_sums<TPR, R>(mean, &slots[0]);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            mean[i] /= (float)channels;
+            rstd[i] = 0.f;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const bool in = (k * TPR + t) * V < channels;
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float d = x[i][k][e] - mean[i];
+                    rstd[i] += in ? d * d : 0.f;
+                }
+            }
+        }
+        row_sums<TPR, R>(rstd, &slots[1]);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            rstd[i] = 1.f / sqrtf(rstd[i] / (float)channels + eps);
+            if (t == 0 && row0 + i < rows) {
+                out_mean[row0 + i] = mean[i];
+                out_rstd[row0 + i] = rstd[i];
+            }
+        }
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = (k * TPR + t) * V;
-            if (row0 + i < rows && c < channels) {
-                load_vec<T, V>(src + c, x[i][k]);
-            } else {
+            if (c >= channels) break;
+            float w[V], b[V];
+            load_vec<float, V>(weights + c, w);
+            load_vec<float, V>(bias + c, b);
 #pragma unroll
-                for (int e = 0; e < V; ++e) x[i][k][e] = 0.f;
+            for (int i = 0; i < R; ++i) {
+                if (row0 + i >= rows) break;
+                float y[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) y[e] = (x[i][k][e] - mean[i]) * rstd[i] * w[e] + b[e];
+                store_vec<T, V>(out + (row0 + i) * channels + c, y);
             }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        mean[i] = 0.f;
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int e = 0; e < V; ++e) mean[i] += x[i][k][e];
-    }
-    row_sums<TPR, R>(mean, &slots[0]);
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        mean[i] /= (float)channels;
-        rstd[i] = 0.f;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const bool in = (k * TPR + t) * V < channels;
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float d = x[i][k][e] - mean[i];
-                rstd[i] += in ? d * d : 0.f;
-            }
-        }
-    }
-    row_sums<TPR, R>(rstd, &slots[1]);
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        rstd[i] = 1.f / sqrtf(rstd[i] / (float)channels + eps);
-        if (t == 0 && row0 + i < rows) {
-            out_mean[row0 + i] = mean[i];
-            out_rstd[row0 + i] = rstd[i];
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const int c = (k * TPR + t) * V;
-        if (c >= channels) break;
-        float w[V], b[V];
-        load_vec<float, V>(weights + c, w);
-        load_vec<float, V>(bias + c, b);
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            if (row0 + i >= rows) break;
-            float y[V];
-#pragma unroll
-            for (int e = 0; e < V; ++e) y[e] = (x[i][k][e] - mean[i]) * rstd[i] * w[e] + b[e];
-            store_vec<T, V>(out + (row0 + i) * channels + c, y);
         }
     }
 }
@@ -171,28 +177,44 @@ layer_norm_grads_kernel(int64_t rows, int channels, const T* __restrict__ feats,
         if (c < channels) load_vec<float, V>(weights + c, w[k]);
     }
     const float inv = 1.f / (float)channels;
-    int turn = 0;
-    for (int64_t base = (int64_t)blockIdx.x * kGroups * R; base < rows; base += (int64_t)gridDim.x * kGroups * R, turn ^= 1) {
-        const int64_t row0 = base + group * R;
-        float x[R][K][V], g[R][K][V], mu[R], r[R], s[2 * R];
+    const int64_t stride = (int64_t)gridDim.x * kGroups * R;
+    RawVec<T, V> next_x[R][K], next_g[R][K];
+    float next_mu[R], next_r[R];
+    auto fetch = [&](int64_t row0) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const int64_t row = row0 + i;
-            const bool live = row < rows;  // every thread of the warp stays for the shuffles
-            mu[i] = live ? mean[row] : 0.f;
-            r[i] = live ? rstd[row] : 0.f;
+            const bool live = row0 + i < rows;  // every thread of the warp stays for the shuffles
+            next_mu[i] = live ? mean[row0 + i] : 0.f;
+            next_r[i] = live ? rstd[row0 + i] : 0.f;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 const int c = (k * TPR + t) * V;
                 if (live && c < channels) {
-                    load_vec<T, V>(feats + row * ld + c, x[i][k]);
-                    load_vec<T, V>(grads + row * ld_g + c, g[i][k]);
+                    next_x[i][k].load(feats + (row0 + i) * ld + c);
+                    next_g[i][k].load(grads + (row0 + i) * ld_g + c);
                 } else {
-#pragma unroll
-                    for (int e = 0; e < V; ++e) x[i][k][e] = mu[i], g[i][k][e] = 0.f;
+                    next_x[i][k].clear();
+                    next_g[i][k].clear();
                 }
             }
         }
+    };
+    fetch(((int64_t)blockIdx.x * kGroups + group) * R);
+    int turn = 0;
+    for (int64_t base = (int64_t)blockIdx.x * kGroups * R; base < rows; base += stride, turn ^= 1) {
+        const int64_t row0 = base + group * R;
+        float x[R][K][V], g[R][K][V], mu[R], r[R], s[2 * R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            mu[i] = next_mu[i];
+            r[i] = next_r[i];
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                next_x[i][k].widen(x[i][k]);
+                next_g[i][k].widen(g[i][k]);
+            }
+        }
+        if (base + stride < rows) fetch(row0 + stride);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             s[2 * i] = s[2 * i + 1] = 0.f;
@@ -368,8 +390,8 @@ struct NormForward {
     void* out; float *mean, *rstd; cudaStream_t s;
     template <class T, int V, int TPR, int K, int R> int run() const {
         const int per_block = kNormThreads / TPR * R;
-        const int64_t blocks = (rows + per_block - 1) / per_block;
-        layer_norm_kernel<T, V, TPR, K, R><<<(unsigned)blocks, kNormThreads, 0, s>>>(rows, channels, (const T*)feats, ld, weights, bias,
+        const int64_t need = (rows + per_block - 1) / per_block;
+        layer_norm_kernel<T, V, TPR, K, R><<<resident_grid(layer_norm_kernel<T, V, TPR, K, R>, need * kNormThreads, kNormThreads), kNormThreads, 0, s>>>(rows, channels, (const T*)feats, ld, weights, bias,
                                                                                  eps, (T*)out, mean, rstd);
         PCCNN_LAUNCH_CHECK();
         return PCCNN_OK;
