@@ -246,7 +246,7 @@ static int launch_grads(const AttentionCall& a, const TcOperand& f1, const TcOpe
     const int64_t count = rows * heads * a.size;
     float* part = (float*)ws;
     const dim3 grid((unsigned)tc_blocks(rows, kTcRows, a.clouds), (unsigned)heads, (unsigned)splits);
-    kernel<<<grid, kTcThreads, Cfg::kBytes, s>>>(m[0], m[1], m[2], m[3], m[4], m[5], a, y1.rows, y2.rows, splits, lse, delta, (T*)out1,
+    kernel<<<grid, kTcThreads, Cfg::kBytes, s>>>(m[0], m[1], m[2], m[3], m[4], m[5], a, f1.rows, f2.rows, y1.rows, y2.rows, splits, lse, delta, (T*)out1,
                                                  (T*)out2, part, part + splits * count, ctl);
     PCCNN_LAUNCH_CHECK();
     if (splits > 1) {

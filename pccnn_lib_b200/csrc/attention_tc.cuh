@@ -194,6 +194,22 @@ __device__ __forceinline__ void tc_rows_by_rows(uint32_t d, uint32_t a, uint32_t
     }
 }
 
+// The same with A in tensor memory (planes of GR x 32 columns): the products of tiles of few rows are bound by reading A from
+// shared memory otherwise (128 rows x 16 features are 4 KB, 32 cycles; with 32 rows of B the product itself takes 16).
+template <int NP, int GR, int RB>
+__device__ __forceinline__ void tc_kept_by_rows(uint32_t d, uint32_t a, uint32_t b, int steps) {
+    const uint32_t idesc = tc_idesc(RB, false);
+    const uint64_t db = umma_desc_k_sw128(b);
+#pragma unroll
+    for (int i = 0; i < TcPairs<NP>::kCount; ++i) {
+#pragma unroll
+        for (int k = 0; k < GR * 4; ++k) {
+            const int at_b = (TcPairs<NP>::b(i) * GR + (k >> 2)) * RB * 8 + 2 * (k & 3);
+            if (k < steps) tc_mma_bf16_ts(d, a + TcPairs<NP>::a(i) * GR * 32 + k * 8, db + at_b, idesc, (i > 0 || k > 0) ? 1u : 0u);
+        }
+    }
+}
+
 // D[128, n] (+)= E[128, RB] B[RB, n]: E in tensor memory (planes of RB / 2 columns), B's tile in shared memory; `steps` blocks
 // of 16 rows of B.
 template <int NP, int GR, int RB>
@@ -274,9 +290,9 @@ __device__ __forceinline__ void tc_write16(T* __restrict__ dst, int c, int size,
 
 // ---- set-up and teardown -----------------------------------------------------------------------------------------
 template <int COLUMNS>
-__device__ __forceinline__ uint32_t tc_begin(TcShared* sh, int stages, int tiles_of_a_stage) {
+__device__ __forceinline__ uint32_t tc_begin(TcShared* sh, int stages, int tiles_of_a_stage, int fixed_arrivals) {
     if (threadIdx.x == 0) {
-        mbar_init(&sh->fixed_full, 1);
+        mbar_init(&sh->fixed_full, fixed_arrivals);
         for (int i = 0; i < stages; ++i) {
             mbar_init(&sh->full[i], tiles_of_a_stage);
             mbar_init(&sh->empty[i], 1);
@@ -404,7 +420,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         return;
     }
-    const uint32_t tmem = tc_begin<512>(sh, kStages, 1);
+    const uint32_t tmem = tc_begin<512>(sh, kStages, 1, 1);
     const int tiles = (int)((end - begin + BN - 1) / BN), q_tiles = rows_here > kTcRows ? 2 : 1, units = tiles * q_tiles;
     const int last_valid = (int)(end - begin) - (tiles - 1) * BN;
     const int steps = (a.size + 15) >> 4, n_out = steps * 16;
@@ -672,24 +688,33 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 //   s = K Q^T, t = V dO^T, p = exp(scale s - lse), e = p (t - delta),  dK += e Q,  dV += p dO.
 // For 32-bit features the accumulators are emptied into registers every kRound units (see the forward kernel on truncation).
 // Two kernels, each recomputing the logits, instead of one that adds dQ with atomics: every sum is taken in a fixed order.
+// 32-bit features: the two tiles that stay are kept as planes in tensor memory (kKeepInTmem), which leaves the keys' kernel no
+// columns of their own for the weights: there they take the place of the logits (kInPlace), and the logits of a group's
+// next unit wait until this one has been added.  Measured on 16001 x 8003 points, 8 heads on 4 of 64, with the tiles in shared
+// memory and columns of their own: queries' gradient 534 us, keys' 598 us.
 template <bool KEYS, int GR, int NP>
 struct TcBackward {
+    static constexpr bool kKeepInTmem = NP == 3, kInPlace = NP == 3 && KEYS;
     // streamed rows of a unit: as many as leave columns for s, t, the weights and the accumulators, and three slots of the ring (a
     // slot is held until its unit has been added, and the logits run ahead by two units)
     static constexpr int kBN = NP == 3 || (KEYS && GR == 2) ? 32 : 64;
-    static constexpr int kFixed = NP * GR * kTcRows * 128;   // one of the two tiles that stay
-    static constexpr int kTile = NP * GR * kBN * 128;        // one of the two tiles of a slot
+    static constexpr int kFixed = kKeepInTmem ? 0 : NP * GR * kTcRows * 128;  // one of the two tiles that stay
+    static constexpr int kTile = NP * GR * kBN * 128;                        // one of the two tiles of a slot
     static constexpr int kFit = (200 * 1024 - 2 * kFixed) / (2 * kTile);
     static constexpr int kStages = kFit > kTcMaxStages ? kTcMaxStages : kFit;
     static constexpr int kPlane = kBN / 2;
-    static constexpr int kWeights = 4 * kBN;                                     // columns of the weights, behind s and t of both groups
-    static constexpr int kWeightCols = (KEYS ? 2 : 1) * NP * kPlane;             // of one group: e, then p
-    static constexpr int kAccStart = kWeights + 2 * kWeightCols;
+    static constexpr int kWeightCols = (KEYS ? 2 : 1) * NP * kPlane;          // weights of one group: e, then p
+    static constexpr int kBuffer = kInPlace ? (kWeightCols > 2 * kBN ? kWeightCols : 2 * kBN) : 2 * kBN;  // s and t of one group
+    static constexpr int kWeights = kInPlace ? 0 : 2 * kBuffer;               // columns of the weights
+    static constexpr int kWeightStride = kInPlace ? kBuffer : kWeightCols;
+    static constexpr int kAccStart = 2 * kBuffer + (kInPlace ? 0 : 2 * kWeightCols);
     static constexpr int kAcc = GR * 64;
-    static constexpr int kRound = 4;                                             // even: both groups have units in a round
-    static constexpr int kKept = NP == 3 ? (KEYS ? kAcc : kAcc / 2) : 1;         // columns that a thread adds up in registers
+    static constexpr int kKeep = kAccStart + (KEYS ? 2 : 1) * kAcc;           // the tiles that stay: planes of GR x 32 columns
+    static constexpr int kKeepCols = NP * GR * 32;
+    static constexpr int kRound = 4;                                          // even: both groups have units in a round
+    static constexpr int kKept = NP == 3 ? (KEYS ? kAcc : kAcc / 2) : 1;      // columns that a thread adds up in registers
     static constexpr int kBytes = 2 * kFixed + kStages * (2 * kTile + 2 * kBN * 4) + 1024 + 512;
-    static_assert(kStages >= 3 && kAccStart + (KEYS ? 2 : 1) * kAcc <= 512 && kBytes <= 227 * 1024, "does not fit");
+    static_assert(kStages >= 3 && kKeep + (kKeepInTmem ? 2 * kKeepCols : 0) <= 512 && kBytes <= 227 * 1024, "does not fit");
 };
 
 template <bool KEYS, int GR, int NP, class T>
@@ -697,7 +722,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __grid_constant__ CUtensorMap map_f2,
                           const __grid_constant__ CUtensorMap map_y1, const __grid_constant__ CUtensorMap map_y2,
                           const __grid_constant__ CUtensorMap map_y18, const __grid_constant__ CUtensorMap map_y28, AttentionCall a,
-                          TcRows rows_y1, TcRows rows_y2, int splits, const float* __restrict__ lse,
+                          TcRows rows_f1, TcRows rows_f2, TcRows rows_y1, TcRows rows_y2, int splits, const float* __restrict__ lse,
                           const float* __restrict__ delta, T* __restrict__ out1, T* __restrict__ out2, float* __restrict__ part1,
                           float* __restrict__ part2, TcControl ctl) {
     using Cfg = TcBackward<KEYS, GR, NP>;
@@ -744,7 +769,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
             }
         return;
     }
-    const uint32_t tmem = tc_begin<512>(sh, kStages, 2);
+    const uint32_t tmem = tc_begin<512>(sh, kStages, 2, Cfg::kKeepInTmem ? 8 : 1);
     const int tiles = (int)((end - begin + BN - 1) / BN), units = tiles * (KEYS ? share : 1);
     const int last_valid = (int)(end - begin) - (tiles - 1) * BN;
     const int steps = (a.size + 15) >> 4, n_out = steps * 16;
@@ -757,7 +782,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
     if (warp == 8) {
         // ---- loader: the two tiles of a slot share a barrier
         bool ok = true;
-        if (lane == 0) {  // rows behind the cloud's last one: see the forward kernel
+        if (!Cfg::kKeepInTmem && lane == 0) {  // rows behind the cloud's last one: see the forward kernel
             mbar_expect_tx(&sh->fixed_full, 2 * Cfg::kFixed);
             tc_load_whole<kTcRows, NP, GR>(smem, &map_f1, num_rows, head, row0, &sh->fixed_full);
             tc_load_whole<kTcRows, NP, GR>(smem + Cfg::kFixed, &map_f2, num_rows, head, row0, &sh->fixed_full);
@@ -805,13 +830,19 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
         for (int u = 0; u < units && ok; ++u) {
             const int s = u % kStages;
             ok = tc_wait_warp(&sh->full[s], (u / kStages) & 1, limit, failed);
-            if (u >= 2) ok = ok && tc_wait_warp(&sh->s_free[u & 1], ((u >> 1) - 1) & 1, limit, failed);  // unit u - 2 has been read
+            if (u >= 2)  // unit u - 2 has been read (or, where its weights are in its place, added)
+                ok = ok && tc_wait_warp(Cfg::kInPlace ? &sh->e_done[u & 1] : &sh->s_free[u & 1], ((u >> 1) - 1) & 1, limit, failed);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t buf = tmem + (u & 1) * 2 * BN, slot = smem_u32(ring + s * 2 * Cfg::kTile);
+            const uint32_t buf = tmem + (u & 1) * Cfg::kBuffer, slot = smem_u32(ring + s * 2 * Cfg::kTile);
             if (leader) {
-                tc_rows_by_rows<NP, GR, BN>(buf, smem_u32(smem), slot, steps);
-                tc_rows_by_rows<NP, GR, BN>(buf + BN, smem_u32(smem + Cfg::kFixed), slot + Cfg::kTile, steps);
+                if constexpr (Cfg::kKeepInTmem) {
+                    tc_kept_by_rows<NP, GR, BN>(buf, tmem + Cfg::kKeep, slot, steps);
+                    tc_kept_by_rows<NP, GR, BN>(buf + BN, tmem + Cfg::kKeep + Cfg::kKeepCols, slot + Cfg::kTile, steps);
+                } else {
+                    tc_rows_by_rows<NP, GR, BN>(buf, smem_u32(smem), slot, steps);
+                    tc_rows_by_rows<NP, GR, BN>(buf + BN, smem_u32(smem + Cfg::kFixed), slot + Cfg::kTile, steps);
+                }
                 tc_commit(&sh->s_full[u & 1]);
             }
             __syncwarp();
@@ -828,7 +859,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
             if (!ok) break;
             tc_fence_after();
             const int s = u % kStages, valid = u % tiles == tiles - 1 ? last_valid : BN;
-            const uint32_t weights = tmem + Cfg::kWeights + (u & 1) * Cfg::kWeightCols, slot = smem_u32(ring + s * 2 * Cfg::kTile);
+            const uint32_t weights = tmem + Cfg::kWeights + (u & 1) * Cfg::kWeightStride, slot = smem_u32(ring + s * 2 * Cfg::kTile);
             if (leader) {
                 tc_weights_by_rows<NP, GR, BN>(acc, weights, slot, n_out, (valid + 15) >> 4, !fresh);
                 if (KEYS)
@@ -854,7 +885,29 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
     if (warp < 8) {
         // ---- element-wise
         bool ok = true;
-        const uint32_t buf = tmem + lanes + group * 2 * BN, weights = tmem + lanes + Cfg::kWeights + group * Cfg::kWeightCols;
+        const uint32_t buf = tmem + lanes + group * Cfg::kBuffer, weights = tmem + lanes + Cfg::kWeights + group * Cfg::kWeightStride;
+        if constexpr (Cfg::kKeepInTmem) {
+            // the first group brings the first tile that stays into tensor memory, the second the second: a row per thread
+            const TcRows& from = group == 0 ? rows_f1 : rows_f2;
+            const int chunks = row < rows_here ? a.size >> 3 : 0;
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                const __nv_bfloat16* src = from.data + p * from.plane + (row0 + row) * from.row + head * from.head;
+#pragma unroll
+                for (int c = 0; c < GR * 8; c += 4) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint4 v = make_uint4(0, 0, 0, 0);
+                        if (c + i < chunks) v = *reinterpret_cast<const uint4*>(src + (c + i) * 8);
+                        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+                    }
+                    tc_st_32x16(tmem + lanes + Cfg::kKeep + group * Cfg::kKeepCols + p * GR * 32 + c * 4, w);
+                }
+            }
+            tc_wait_st();
+            tc_arrive_warp(&sh->fixed_full);
+        }
         int emptied = 0;
         auto empty_until = [&](int round) {  // the accumulators of the rounds before `round` into registers
             if constexpr (NP == 3) {
@@ -883,6 +936,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
             if constexpr (KEYS) {
                 // 16 columns at a time, their statistics read ahead of the tensor memory: the products' operands keep the
                 // shared memory busy
+                constexpr int kParts = BN / 16;
                 float4 base[4], d[4];
                 auto read_stats = [&](int i) {
 #pragma unroll
@@ -892,20 +946,30 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                     }
                 };
                 read_stats(0);
+                uint32_t s[Cfg::kInPlace ? kParts : 1][16], t[Cfg::kInPlace ? kParts : 1][16];
+                if constexpr (Cfg::kInPlace) {  // all of them before the first weight is stored
 #pragma unroll
-                for (int i = 0; i < BN / 16; ++i) {
-                    uint32_t s[16], t[16];
-                    tc_ld_32x16(buf + 16 * i, s);
-                    tc_ld_32x16(buf + BN + 16 * i, t);
-                    if (i == BN / 16 - 1) tc_arrive_warp(&sh->s_free[group]);
+                    for (int i = 0; i < kParts; ++i) {
+                        tc_ld_32x16(buf + 16 * i, s[i]);
+                        tc_ld_32x16(buf + BN + 16 * i, t[i]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kParts; ++i) {
+                    const int at = Cfg::kInPlace ? i : 0;
+                    if constexpr (!Cfg::kInPlace) {
+                        tc_ld_32x16(buf + 16 * i, s[0]);
+                        tc_ld_32x16(buf + BN + 16 * i, t[0]);
+                        if (i == kParts - 1) tc_arrive_warp(&sh->s_free[group]);
+                    }
                     float p[16], e[16];
 #pragma unroll
                     for (int c = 0; c < 16; ++c) {
-                        p[c] = exp2_fast(fmaf(__uint_as_float(s[c]), c2, -(&base[c / 4].x)[c % 4]));
-                        e[c] = p[c] * (__uint_as_float(t[c]) - (&d[c / 4].x)[c % 4]);
+                        p[c] = exp2_fast(fmaf(__uint_as_float(s[at][c]), c2, -(&base[c / 4].x)[c % 4]));
+                        e[c] = p[c] * (__uint_as_float(t[at][c]) - (&d[c / 4].x)[c % 4]);
                     }
-                    if (i + 1 < BN / 16) read_stats(i + 1);
-                    if (i == 0 && u >= 2) {  // the group's last unit has been added: its columns of weights are free
+                    if (i + 1 < kParts) read_stats(i + 1);
+                    if (!Cfg::kInPlace && i == 0 && u >= 2) {  // the group's last unit has been added: its columns of weights are free
                         if (!(ok = tc_wait_warp(&sh->e_done[group], ((u >> 1) - 1) & 1, limit, failed))) break;
                         tc_fence_after();
                     }

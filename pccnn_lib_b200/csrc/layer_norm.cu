@@ -359,7 +359,7 @@ static int dispatch_rows_of(int n, const Launch& launch) {
         if (n <= 8) return launch.template run<T, V, 8, 1, 8>();
         if (n <= 16) return launch.template run<T, V, 8, 2, 4>();
         if (n <= 32) return launch.template run<T, V, 8, 4, 4>();
-        if (n <= 64) return launch.template run<T, V, 32, 2, 8>();
+        if (n <= 64) return launch.template run<T, V, 32, 2, 4>();
         if (n <= 128) return launch.template run<T, V, 32, 4, 4>();
         if (n <= 256) return launch.template run<T, V, 32, 8, 2>();
         if (n <= 512) return launch.template run<T, V, 32, 16, 1>();
