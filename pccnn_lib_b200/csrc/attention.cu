@@ -314,20 +314,31 @@ attention_join_kernel(int64_t num_queries, int heads, int size, int splits, cons
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------
-// delta[h, m] = sum_d out g: one warp per (query, head).
-template <class T>
+// delta[h, m] = sum_d out g: LPK lanes of a warp per (query, head), V elements each at a time.
+template <class T, int V>
 __global__ void __launch_bounds__(256)
-attention_delta_kernel(int64_t num_queries, int heads, int size, const T* __restrict__ out, HeadRows grads, float* __restrict__ delta) {
-    const int64_t rows = num_queries * heads, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (row >= rows) return;
-    const int64_t m = row / heads;
-    const int h = (int)(row % heads);
-    const T* g = (const T*)grads.data + m * grads.row + h * grads.head;
-    float s = 0.f;
-    for (int d = lane; d < size; d += 32) s = fmaf(to_float(out[row * size + d]), to_float(g[d]), s);
-    s = warp_sum(s);
-    if (lane == 0) delta[(int64_t)h * num_queries + m] = s;
+attention_delta_kernel(int64_t num_queries, int heads, int size, int lanes_per_row, const T* __restrict__ out, HeadRows grads,
+                       float* __restrict__ delta) {
+    const int64_t rows = num_queries * heads, per_block = 256 / lanes_per_row;
+    const int lane = threadIdx.x % lanes_per_row;
+    for (int64_t first = blockIdx.x * per_block; first < rows; first += gridDim.x * per_block) {  // the same for the block
+        const int64_t row = first + threadIdx.x / lanes_per_row;
+        const int64_t m = row / heads;
+        const int h = (int)(row - m * heads);
+        float s = 0.f;
+        if (row < rows) {
+            const T* g = (const T*)grads.data + m * grads.row + h * grads.head;
+            for (int d = lane * V; d < size; d += lanes_per_row * V) {
+                float a[V], b[V];
+                load_vec<T, V>(out + row * size + d, a);
+                load_vec<T, V>(g + d, b);
+#pragma unroll
+                for (int e = 0; e < V; ++e) s = fmaf(a[e], b[e], s);
+            }
+        }
+        s = sum_lanes(s, lanes_per_row);
+        if (row < rows && lane == 0) delta[(int64_t)h * num_queries + m] = s;
+    }
 }
 
 // Queries' gradient: block = one query and head x one split of its keys.
@@ -610,6 +621,19 @@ struct BackwardRows {
     template <class T, int V, int NC> int run() const { return launch_grad_rows<T, V, NC>(a, grads, l, lse, delta, dq, dk, dv, ws, s); }
 };
 
+static int launch_delta(const AttentionCall& a, const void* out, const HeadRows& grads, float* delta, cudaStream_t s) {
+    const int v = a.is_bf16 ? 8 : 4;
+    const bool vectors = a.size % v == 0 && aligned16(out) && vector_heads(grads, v);
+    int lanes = 1;
+    while (lanes < 32 && lanes * (vectors ? v : 1) < a.size) lanes *= 2;
+    const unsigned blocks = grid_for(a.num_queries * a.heads * lanes, 256, 16);
+    auto run = [&](auto kernel, auto* typed) { kernel<<<blocks, 256, 0, s>>>(a.num_queries, a.heads, a.size, lanes, typed, grads, delta); };
+    if (a.is_bf16) run(vectors ? attention_delta_kernel<__nv_bfloat16, 8> : attention_delta_kernel<__nv_bfloat16, 1>, (const __nv_bfloat16*)out);
+    else run(vectors ? attention_delta_kernel<float, 4> : attention_delta_kernel<float, 1>, (const float*)out);
+    PCCNN_LAUNCH_CHECK();
+    return PCCNN_OK;
+}
+
 static int check_call(const char* who, const AttentionCall& a) {
     PCCNN_CHECK_ARG(a.num_queries >= 0 && a.num_queries < 0x7fffffffLL && a.num_keys >= 0 && a.num_keys < 0x7fffffffLL && a.clouds >= 0,
                     "%s: bad number of rows", who);
@@ -702,12 +726,8 @@ int pccnn_cross_attention_grads(int64_t num_queries, int64_t num_keys, int cloud
     const HeadRows grads{in_grads, grad_strides_host[0], grad_strides_host[1]};
     float* delta = (float*)workspace;
     char* rest = (char*)workspace + align_up((size_t)num_queries * heads * 4 + 256);
-    if (num_queries > 0) {
-        const unsigned blocks = (unsigned)((num_queries * heads + 7) / 8);
-        if (is_bf16) attention_delta_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(num_queries, heads, size, (const __nv_bfloat16*)out, grads, delta);
-        else attention_delta_kernel<float><<<blocks, 256, 0, s>>>(num_queries, heads, size, (const float*)out, grads, delta);
-        PCCNN_LAUNCH_CHECK();
-    }
+    if (num_queries > 0)
+        if (int rc = launch_delta(a, out, grads, delta, s)) return rc;
     if (num_queries > 0 && num_keys > 0 && tc_grads_shape(a) && tc_layout(a, &grads) && aligned16(out_query_grads) && aligned16(out_key_grads) &&
         aligned16(out_value_grads))
         return tc_grads(a, grads, lse, delta, out_query_grads, out_key_grads, out_value_grads, rest, s);
