@@ -9,6 +9,8 @@
 // blocks whose results are joined by a second kernel.  Sums, maxima and probabilities are 32-bit floats.
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "attention.cuh"
 #include "common.cuh"
 #include "features.cuh"
@@ -92,6 +94,83 @@ __device__ __forceinline__ void split_range(int64_t& begin, int64_t& end, int s,
 // lane has the next kUnroll keys and values in flight while it works on the last ones, as raw 16-byte vectors.
 // Without splits the output and lse are written; with splits the block leaves its unnormalised sum (relative to its own
 // maximum), the maximum and the sum of the probabilities.
+// V values held as packed pairs where there are pairs: two multiply-adds per instruction.
+template <int V>
+struct Lanes {
+    static constexpr int kN = V > 1 ? V / 2 : 1;
+    using Word = typename std::conditional<(V > 1), unsigned long long, float>::type;
+    Word w[kN];
+    __device__ __forceinline__ void set(const float (&x)[V]) {
+        if constexpr (V > 1) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) w[i] = pack_f32x2(x[2 * i], x[2 * i + 1]);
+        } else {
+            w[0] = x[0];
+        }
+    }
+    __device__ __forceinline__ void get(float (&x)[V]) const {
+        if constexpr (V > 1) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) unpack_f32x2(w[i], x[2 * i], x[2 * i + 1]);
+        } else {
+            x[0] = w[0];
+        }
+    }
+    // this += a * b, element by element
+    __device__ __forceinline__ void add_product(const Lanes& a, const Lanes& b) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            if constexpr (V > 1) w[i] = fma_f32x2(a.w[i], b.w[i], w[i]);
+            else w[i] = fmaf(a.w[i], b.w[i], w[i]);
+        }
+    }
+    __device__ __forceinline__ void add_scaled(const Lanes& a, float s) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            if constexpr (V > 1) w[i] = fma_f32x2(a.w[i], pack_f32x2(s, s), w[i]);
+            else w[i] = fmaf(a.w[i], s, w[i]);
+        }
+    }
+    __device__ __forceinline__ void scale(float s) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            if constexpr (V > 1) w[i] = mul_f32x2(w[i], pack_f32x2(s, s));
+            else w[i] *= s;
+        }
+    }
+    __device__ __forceinline__ float sum() const {
+        float x[V], s = 0.f;
+        get(x);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s += x[e];
+        return s;
+    }
+};
+
+// Sums of U values over lanes_per_row lanes (at least U), each value's sum in its own part of the lanes: value `mine` in this one.
+template <int U>
+__device__ __forceinline__ float sum_and_spread(const float (&s)[U], int lanes_per_row, int in_row, int& mine) {
+    static_assert(U == 2 || U == 4, "two or four values");
+    int o = lanes_per_row >> 1;
+    float v;
+    if constexpr (U == 4) {
+        const bool hi = in_row & o;
+        float a = hi ? s[2] : s[0], b = hi ? s[3] : s[1];
+        a += __shfl_xor_sync(kFullMask, hi ? s[0] : s[2], o);
+        b += __shfl_xor_sync(kFullMask, hi ? s[1] : s[3], o);
+        o >>= 1;
+        const bool odd = in_row & o;
+        v = (odd ? b : a) + __shfl_xor_sync(kFullMask, odd ? a : b, o);
+        mine = (hi ? 2 : 0) + (odd ? 1 : 0);
+    } else {
+        const bool odd = in_row & o;
+        v = (odd ? s[1] : s[0]) + __shfl_xor_sync(kFullMask, odd ? s[0] : s[1], o);
+        mine = odd ? 1 : 0;
+    }
+    for (o >>= 1; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+    return v;
+}
+
 template <class T, int V, int NC, int GH>
 __global__ void __launch_bounds__(kRowThreads)
 attention_row_kernel(AttentionCall a, int lanes_per_row, int warp_heads, int splits, T* __restrict__ out, float* __restrict__ lse,
@@ -115,49 +194,71 @@ attention_row_kernel(AttentionCall a, int lanes_per_row, int warp_heads, int spl
     split_range(begin, end, split, splits);
 
     const float c2 = a.scale * kLog2e;
-    float q[GH][NC][V], acc[GH][NC][V], top[GH], total[GH];
+    Lanes<V> q[GH][NC], sums[GH][NC];
+    float top[GH], total[GH];
 #pragma unroll
     for (int g = 0; g < GH; ++g) {
         top[g] = -INFINITY;
         total[g] = 0.f;
-        load_row<T, V, NC>((const T*)a.q.data + m * a.q.row + (h0 + min(g, heads_here - 1)) * a.q.head, in_row, lanes_per_row, a.size, q[g]);
+        float x[NC][V];
+        load_row<T, V, NC>((const T*)a.q.data + m * a.q.row + (h0 + min(g, heads_here - 1)) * a.q.head, in_row, lanes_per_row, a.size, x);
+        const float zero[V] = {};
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int e = 0; e < V; ++e) acc[g][c][e] = 0.f;
+        for (int c = 0; c < NC; ++c) {
+            q[g][c].set(x[c]);
+            sums[g][c].set(zero);
+        }
     }
     const T* keys = (const T*)a.k.data + kv * a.k.head;
     const T* values = (const T*)a.v.data + kv * a.v.head;
     const int step = slices * per_warp;
     RawVec<T, V> key[kUnroll][NC], val[kUnroll][NC];
     auto fetch = [&](int64_t first) {
+        const T *k0 = keys + (first + sub) * a.k.row, *v0 = values + (first + sub) * a.v.row;
+        const bool whole = first + (int64_t)step * (kUnroll - 1) + per_warp <= end;  // the same for the warp
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            const int64_t n = first + u * step + sub;
+            const bool in = whole || first + u * step + sub < end;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const int d = (c * lanes_per_row + in_row) * V;
-                if (n < end && d < a.size) {
-                    key[u][c].load(keys + n * a.k.row + d);
-                    val[u][c].load(values + n * a.v.row + d);
+                if (in && d < a.size) {
+                    key[u][c].load(k0 + d);
+                    val[u][c].load(v0 + d);
                 } else {
                     key[u][c].clear();
                     val[u][c].clear();
                 }
             }
+            k0 += step * a.k.row;
+            v0 += step * a.v.row;
         }
     };
+    // A logit is summed over the lanes of its row while the four of an iteration part: every lane ends with one of them, and
+    // its exponential is taken once and handed round.  (The kernel is bound by the instructions it issues, 68% of the slots
+    // with a full sum and exponential per lane: 205 us for 400000 keys, 8 heads of 64, bf16.)
     const int64_t start = begin + slice * per_warp;
     if (start < end) fetch(start);
     for (int64_t first = start; first < end; first += (int64_t)step * kUnroll) {  // the same for the warp's lanes
         float s[GH][kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            float x[NC][V];
+            Lanes<V> x[NC];
 #pragma unroll
-            for (int c = 0; c < NC; ++c) key[u][c].widen(x[c]);
+            for (int c = 0; c < NC; ++c) {
+                float f[V];
+                key[u][c].widen(f);
+                x[c].set(f);
+            }
 #pragma unroll
-            for (int g = 0; g < GH; ++g) s[g][u] = dot<V, NC>(q[g], x);
+            for (int g = 0; g < GH; ++g) {
+                const float zero[V] = {};
+                Lanes<V> dot;
+                dot.set(zero);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) dot.add_product(q[g][c], x[c]);
+                s[g][u] = dot.sum();
+            }
         }
         RawVec<T, V> now_val[kUnroll][NC];
 #pragma unroll
@@ -167,39 +268,43 @@ attention_row_kernel(AttentionCall a, int lanes_per_row, int warp_heads, int spl
         if (first + (int64_t)step * kUnroll < end) fetch(first + (int64_t)step * kUnroll);
 #pragma unroll
         for (int g = 0; g < GH; ++g) {
-            float now = top[g];
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                s[g][u] = sum_lanes(s[g][u], lanes_per_row) * c2;
-                if (first + u * step + sub >= end) s[g][u] = -INFINITY;
-                now = fmaxf(now, s[g][u]);
-            }
+            int mine;
+            float v = sum_and_spread<kUnroll>(s[g], lanes_per_row, in_row, mine) * c2;
+            if (first + mine * step + sub >= end) v = -INFINITY;
+            float now = fmaxf(v, __shfl_xor_sync(kFullMask, v, lanes_per_row >> 1));
+            if (kUnroll == 4) now = fmaxf(now, __shfl_xor_sync(kFullMask, now, lanes_per_row >> 2));
+            now = fmaxf(top[g], now);
             const float from = now == -INFINITY ? 0.f : now;
-            const float fade = exp2_fast(top[g] - from);
+            const float fade = exp2_fast(top[g] - from), p = exp2_fast(v - from);
             top[g] = now;
-            total[g] *= fade;
+            total[g] = fmaf(total[g], fade, p);
 #pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int e = 0; e < V; ++e) acc[g][c][e] *= fade;
+            for (int c = 0; c < NC; ++c) sums[g][c].scale(fade);
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
-                s[g][u] = exp2_fast(s[g][u] - from);
-                total[g] += s[g][u];
+                const int at = kUnroll == 4 ? (u >> 1) * (lanes_per_row >> 1) + (u & 1) * (lanes_per_row >> 2) : u * (lanes_per_row >> 1);
+                s[g][u] = __shfl_sync(kFullMask, p, sub * lanes_per_row + at);
             }
         }
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            float x[NC][V];
 #pragma unroll
-            for (int c = 0; c < NC; ++c) now_val[u][c].widen(x[c]);
+            for (int c = 0; c < NC; ++c) {
+                float f[V];
+                now_val[u][c].widen(f);
+                Lanes<V> x;
+                x.set(f);
 #pragma unroll
-            for (int g = 0; g < GH; ++g)
-#pragma unroll
-                for (int c = 0; c < NC; ++c)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) acc[g][c][e] = fmaf(s[g][u], x[c][e], acc[g][c][e]);
+                for (int g = 0; g < GH; ++g) sums[g][c].add_scaled(x, s[g][u]);
+            }
         }
+    }
+    float acc[GH][NC][V];
+#pragma unroll
+    for (int g = 0; g < GH; ++g) {
+        total[g] *= (float)kUnroll / (float)lanes_per_row;  // a probability is held by that many lanes (a power of two)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) sums[g][c].get(acc[g][c]);
     }
     // join the row groups of a warp, then the warps of a head in ascending order
 #pragma unroll
@@ -213,7 +318,7 @@ attention_row_kernel(AttentionCall a, int lanes_per_row, int warp_heads, int spl
         const float from = now == -INFINITY ? 0.f : now;
         const float fade = exp2_fast(top[g] - from);
         float sum = total[g] * fade;
-        for (int o = lanes_per_row; o < 32; o <<= 1) sum += __shfl_xor_sync(kFullMask, sum, o);
+        sum = warp_sum(sum);
         if (lane == 0) stat[warp][1] = sum;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
@@ -499,7 +604,7 @@ static RowLayout row_layout(const AttentionCall& a, const HeadRows* grads) {
     RowLayout l;
     l.vectors = a.size % v == 0 && vector_heads(a.q, v) && vector_heads(a.k, v) && vector_heads(a.v, v) && (!grads || vector_heads(*grads, v));
     const int n = l.vectors ? a.size / v : a.size;
-    l.lanes = 1;
+    l.lanes = 4;  // at least: the forward kernel spreads four keys over a row's lanes
     while (l.lanes < 32 && l.lanes < n) l.lanes *= 2;
     l.chunks = 1;
     while (l.chunks * l.lanes < n) l.chunks *= 2;
