@@ -370,6 +370,121 @@ def test_captured_calls_follow_new_inputs_and_lengths(lengths, dtype):
             check_attention(held[:2], want, held[2:])
 
 
+EDGES = [(1, 127), (127, 1), (128, 128), (129, 129), (255, 64), (256, 63), (257, 65), (7, 8), (8, 7), (9, 9), (31, 33), (32, 32), (33, 31), (64, 255),
+         (65, 257), (63, 256), (3, 0), (0, 3), (130, 16), (16, 130)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("size", [24, 64, 120])
+def test_clouds_that_end_at_and_around_the_borders_of_tiles(size, dtype):
+    lengths = ([q for q, _ in EDGES], [k for _, k in EDGES])
+    run_and_check(*attention_case(lengths, (4, 2), size, dtype, seed=70), lengths)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+def test_thousands_of_tiny_clouds(dtype):
+    gen = torch.Generator()
+    gen.manual_seed(4)
+    lengths = tuple(torch.randint(0, 5, (1500,), generator=gen).tolist() for _ in range(2))
+    run_and_check(*attention_case(lengths, (2, 1), 32, dtype, seed=80), lengths)
+
+
+@pytest.mark.parametrize("queries", [1, 300], ids=["rows", "tiles"])
+def test_keys_beyond_32_bits_of_offset(queries):
+    """The last cloud's keys lie behind 2^31 elements (and 2^32 bytes)."""
+    from pccnn_lib_b200 import ops
+    n, tail = (1 << 31) // (8 * 128) + 1000, 700
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(1)
+    keys, values = (torch.randn((n, 8, 128), generator=gen, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    q, g = draw((queries + 1, 8, 128), 2, torch.bfloat16, 1.5), draw((queries + 1, 8, 128), 3, torch.bfloat16)
+    qe, ke = ends_of([1, queries]), ends_of([n - tail, tail])
+    out, lse = ops.cross_attention(q, keys, values, qe, ke)
+    dq, dk, dv = ops.cross_attention_grads(q, keys, values, qe, ke, out, lse, g)
+    ops.check_status()
+    want = attention(q[1:], keys[-tail:], values[-tail:], [queries], [tail], 128 ** -0.5, g[1:])
+    check_attention([out[1:], lse[:, 1:].contiguous()], want, [dq[1:], dk[-tail:], dv[-tail:]])
+
+
+def test_norm_and_positions_beyond_32_bits_of_offset():
+    from pccnn_lib_b200 import ops
+    n = (1 << 31) // 128 + 64
+    x = torch.zeros((n, 128), dtype=torch.bfloat16, device="cuda")
+    tail, g = draw((64, 128), 1, torch.bfloat16), torch.zeros((n, 128), dtype=torch.bfloat16, device="cuda")
+    x[-64:], g[-64:] = tail, draw((64, 128), 2, torch.bfloat16)
+    w, b = 1 + draw((128,), 3, scale=0.3), draw((128,), 4)
+    want = norm_reference(tail, w, b, 1e-5, g[-64:])
+    out, mean, rstd = ops.layer_norm(x, w, b)
+    check(out[-64:], want["out"], want["out_bound"], "out")
+    dx, dw, db = ops.layer_norm_grads(x, w, mean, rstd, g)
+    check(dx[-64:], want["dx"], want["dx_bound"], "dx")
+    check(dw, want["dw"], want["dw_bound"], "dw")  # the other rows' gradients are zeros, exactly
+    check(db, want["db"], want["db_bound"], "db")
+    del out, dx
+    pts, freq = torch.zeros((n, 3), device="cuda"), torch.exp(draw((15,), 5))
+    pts[-64:] = draw((64, 3), 6, scale=20.0)
+    want = rotary_reference(tail.view(64, 4, 32), pts[-64:], freq, [5, 5, 5], g[-64:].view(64, 4, 32))
+    check(ops.rotary_positions(x.view(n, 4, 32), pts, freq, [5, 5, 5])[-64:], want["out"], want["out_bound"], "out")
+    dx, dp = ops.rotary_positions_grads(x.view(n, 4, 32), pts, freq, [5, 5, 5], g.view(n, 4, 32))
+    check(dx[-64:], want["dx"], want["dx_bound"], "dx")
+    check(dp[-64:], want["dp"], want["dp_bound"], "dp")
+
+
+class short_waits_and_a_silent_loader(object):
+    """The loader issues nothing from its second tile on and the poll limit is lowered, so the waits of the other roles run
+    out with no copy in flight."""
+
+    def __enter__(self):
+        from pccnn_lib_b200 import _capi
+        _capi.check(_capi.lib.pccnn_gemm_set_test_hooks(4000, 1), "set_test_hooks")
+
+    def __exit__(self, *exc):
+        from pccnn_lib_b200 import _capi
+        torch.cuda.synchronize()
+        _capi.check(_capi.lib.pccnn_gemm_set_test_hooks(0, -1), "set_test_hooks")
+        return False
+
+
+@pytest.mark.parametrize("size", [64, 128])
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+def test_attention_reports_a_wait_that_ran_out_and_recovers(dtype, size):
+    from pccnn_lib_b200 import ops
+    lengths = ([500, 300], [900, 1100])
+    q, k, v, qe, ke, g = attention_case(lengths, (4, 2), size, dtype)
+    out, lse = ops.cross_attention(q, k, v, qe, ke)
+    ops.check_status()
+    with short_waits_and_a_silent_loader():
+        ops.cross_attention(q, k, v, qe, ke)  # asynchronous: the call itself cannot know yet
+        with pytest.raises(RuntimeError, match="cross attention .* gave up"):
+            ops.check_status(synchronize=True)
+    ops.check_status()  # the record was consumed
+    if dtype == torch.bfloat16 or size <= 64:  # larger 32-bit heads take the kernels without tensor cores
+        with short_waits_and_a_silent_loader():
+            ops.cross_attention_grads(q, k, v, qe, ke, out, lse, g)
+            torch.cuda.synchronize()
+            with pytest.raises(RuntimeError, match="gave up"):
+                ops.cross_attention(q, k, v, qe, ke)  # found by the next call
+    run_and_check(q, k, v, qe, ke, g, lengths)
+
+
+def test_attention_on_two_streams_at_once():
+    from pccnn_lib_b200 import ops
+    cases = [attention_case(LENGTHS["tiles"], (4, 2), 64, dtype, seed=90 + i) for i, dtype in enumerate(TYPES * 2)]
+    want = [attention(q, k, v, *LENGTHS["tiles"], 0.125, g) for q, k, v, _, _, g in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    held = []
+    for _ in range(5):
+        for stream, (q, k, v, qe, ke, g) in zip(streams, cases):
+            with torch.cuda.stream(stream):
+                out, lse = ops.cross_attention(q, k, v, qe, ke)
+                held.append((out, lse, ops.cross_attention_grads(q, k, v, qe, ke, out, lse, g)))
+    torch.cuda.synchronize()
+    ops.check_status()
+    for i, (out, lse, grads) in enumerate(held):
+        check_attention([out, lse], want[i % len(cases)], grads)
+
+
 # ---- autograd and the layer ----------------------------------------------------------------------
 def test_autograd_wrappers_return_the_operators_gradients():
     from pccnn_lib_b200 import ops
