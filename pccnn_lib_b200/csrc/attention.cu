@@ -447,10 +447,12 @@ attention_delta_kernel(int64_t num_queries, int heads, int size, int lanes_per_r
 }
 
 // Queries' gradient: block = one query and head x one split of its keys.
-template <class T, int V, int NC>
+// DELTA: instead of the gradient, delta = sum_n p dp itself, for clouds of few keys (splits = 1): the rounding of a bf16 output is a
+// large part of dp - delta there (see attention_tc_grads_kernel).
+template <class T, int V, int NC, bool DELTA>
 __global__ void __launch_bounds__(kRowThreads)
 attention_query_grads_row_kernel(AttentionCall a, HeadRows grads, int lanes_per_row, int splits, const float* __restrict__ lse,
-                                 const float* __restrict__ delta, T* __restrict__ out, float* __restrict__ part) {
+                                 float* __restrict__ delta, T* __restrict__ out, float* __restrict__ part) {
     __shared__ float scratch[kRowWarps * NC * 32 * V];
     const int64_t m = blockIdx.x;
     const int h = blockIdx.y, kv = h / (a.heads / a.kv_heads), split = blockIdx.z;
@@ -465,7 +467,8 @@ attention_query_grads_row_kernel(AttentionCall a, HeadRows grads, int lanes_per_
     split_range(begin, end, split, splits);
     const float c2 = a.scale * kLog2e;
     const float row_lse = lse[(int64_t)h * a.num_queries + m], base = row_lse == -INFINITY ? INFINITY : row_lse * kLog2e;
-    const float row_delta = delta[(int64_t)h * a.num_queries + m];
+    const float row_delta = DELTA ? 0.f : delta[(int64_t)h * a.num_queries + m];
+    float weighted = 0.f;
     float q[NC][V], g[NC][V], acc[NC][V];
     load_row<T, V, NC>((const T*)a.q.data + m * a.q.row + h * a.q.head, in_row, lanes_per_row, a.size, q);
     load_row<T, V, NC>((const T*)grads.data + m * grads.row + h * grads.head, in_row, lanes_per_row, a.size, g);
@@ -484,12 +487,24 @@ attention_query_grads_row_kernel(AttentionCall a, HeadRows grads, int lanes_per_
         const float s = sum_lanes(dot<V, NC>(q, key), lanes_per_row);
         const float dp = sum_lanes(dot<V, NC>(g, val), lanes_per_row);
         const float ds = exp2_fast(s * c2 - base) * (dp - row_delta);
-        if (in) {
+        if (DELTA) {
+            weighted += in && in_row == 0 ? ds : 0.f;
+        } else if (in) {
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
                 for (int e = 0; e < V; ++e) acc[c][e] = fmaf(ds, key[c][e], acc[c][e]);
         }
+    }
+    if constexpr (DELTA) {
+        weighted = warp_sum(weighted);
+        if (lane == 0) scratch[warp] = weighted;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < kRowWarps; ++w) weighted += scratch[w];
+            delta[(int64_t)h * a.num_queries + m] = weighted;
+        }
+        return;
     }
     add_over_block<V, NC>(acc, lanes_per_row, scratch);
     if (warp == 0 && lane < lanes_per_row) {
@@ -683,12 +698,19 @@ int add_splits(int is_bf16, int64_t count, int splits, const float* part, void* 
 }
 
 template <class T, int V, int NC>
-static int launch_grad_rows(const AttentionCall& a, const HeadRows& grads, const RowLayout& l, const float* lse, const float* delta,
+static int launch_grad_rows(const AttentionCall& a, const HeadRows& grads, const RowLayout& l, const float* lse, float* delta,
                             void* dq, void* dk, void* dv, char* ws, cudaStream_t s) {
     float* part = (float*)ws;
     if (a.num_queries > 0) {
         const int splits = query_grad_splits(a);
-        attention_query_grads_row_kernel<T, V, NC><<<dim3((unsigned)a.num_queries, (unsigned)a.heads, (unsigned)splits), kRowThreads, 0, s>>>(
+        if constexpr (sizeof(T) == 2) {
+            if (mean_rows(a.num_keys, a.clouds) <= 256) {
+                attention_query_grads_row_kernel<T, V, NC, true><<<dim3((unsigned)a.num_queries, (unsigned)a.heads), kRowThreads, 0, s>>>(
+                    a, grads, l.lanes, 1, lse, delta, (T*)dq, part);
+                PCCNN_LAUNCH_CHECK();
+            }
+        }
+        attention_query_grads_row_kernel<T, V, NC, false><<<dim3((unsigned)a.num_queries, (unsigned)a.heads, (unsigned)splits), kRowThreads, 0, s>>>(
             a, grads, l.lanes, splits, lse, delta, (T*)dq, part);
         PCCNN_LAUNCH_CHECK();
         if (splits > 1)
@@ -722,7 +744,7 @@ struct ForwardRows {
     template <class T, int V, int NC> int run() const { return launch_rows<T, V, NC>(a, l, out, lse, ws, s); }
 };
 struct BackwardRows {
-    const AttentionCall& a; const HeadRows& grads; RowLayout l; const float *lse, *delta; void *dq, *dk, *dv; char* ws; cudaStream_t s;
+    const AttentionCall& a; const HeadRows& grads; RowLayout l; const float* lse; float* delta; void *dq, *dk, *dv; char* ws; cudaStream_t s;
     template <class T, int V, int NC> int run() const { return launch_grad_rows<T, V, NC>(a, grads, l, lse, delta, dq, dk, dv, ws, s); }
 };
 

@@ -32,7 +32,7 @@ int tc_forward(const AttentionCall& a, void* out, float* lse, char* ws, cudaStre
 
 bool tc_grads_shape(const AttentionCall& a);
 size_t tc_grads_workspace(const AttentionCall& a);
-int tc_grads(const AttentionCall& a, const HeadRows& grads, const float* lse, const float* delta, void* dq, void* dk, void* dv, char* ws,
+int tc_grads(const AttentionCall& a, const HeadRows& grads, const float* lse, float* delta, void* dq, void* dk, void* dv, char* ws,
              cudaStream_t s);
 
 // out = the sum of the splits' parts [splits, count].

@@ -227,7 +227,7 @@ size_t tc_grads_workspace(const AttentionCall& a) {
 
 template <bool KEYS, int GR, int NP, class T>
 static int launch_grads(const AttentionCall& a, const TcOperand& f1, const TcOperand& f2, const TcOperand& y1, const TcOperand& y2,
-                        const float* lse, const float* delta, void* out1, void* out2, char* ws, cudaStream_t s) {
+                        const float* lse, float* delta, void* out1, void* out2, char* ws, cudaStream_t s) {
     using Cfg = TcBackward<KEYS, GR, NP>;
     static std::atomic<uint64_t> done{0};
     const auto kernel = attention_tc_grads_kernel<KEYS, GR, NP, T>;
@@ -257,7 +257,7 @@ static int launch_grads(const AttentionCall& a, const TcOperand& f1, const TcOpe
 }
 
 template <int GR, int NP, class T>
-static int launch_both_grads(const AttentionCall& a, const HeadRows& grads, const float* lse, const float* delta, void* dq, void* dk, void* dv,
+static int launch_both_grads(const AttentionCall& a, const HeadRows& grads, const float* lse, float* delta, void* dq, void* dk, void* dv,
                              char* ws, cudaStream_t s) {
     TcOperands operands(ws, a.size, NP == 3);
     const TcOperand &q = operands.add(a.q, a.num_queries, a.heads), &g = operands.add(grads, a.num_queries, a.heads),
@@ -268,7 +268,7 @@ static int launch_both_grads(const AttentionCall& a, const HeadRows& grads, cons
     return launch_grads<true, GR, NP, T>(a, k, v, q, g, lse, delta, dk, dv, ws, s);
 }
 
-int tc_grads(const AttentionCall& a, const HeadRows& grads, const float* lse, const float* delta, void* dq, void* dk, void* dv, char* ws,
+int tc_grads(const AttentionCall& a, const HeadRows& grads, const float* lse, float* delta, void* dq, void* dk, void* dv, char* ws,
              cudaStream_t s) {
     if (!a.is_bf16) return launch_both_grads<1, 3, float>(a, grads, lse, delta, dq, dk, dv, ws, s);
     return a.size <= 64 ? launch_both_grads<1, 1, __nv_bfloat16>(a, grads, lse, delta, dq, dk, dv, ws, s)

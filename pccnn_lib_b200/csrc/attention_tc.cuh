@@ -723,7 +723,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                           const __grid_constant__ CUtensorMap map_y1, const __grid_constant__ CUtensorMap map_y2,
                           const __grid_constant__ CUtensorMap map_y18, const __grid_constant__ CUtensorMap map_y28, AttentionCall a,
                           TcRows rows_f1, TcRows rows_f2, TcRows rows_y1, TcRows rows_y2, int splits, const float* __restrict__ lse,
-                          const float* __restrict__ delta, T* __restrict__ out1, T* __restrict__ out2, float* __restrict__ part1,
+                          float* __restrict__ delta, T* __restrict__ out1, T* __restrict__ out2, float* __restrict__ part1,
                           float* __restrict__ part2, TcControl ctl) {
     using Cfg = TcBackward<KEYS, GR, NP>;
     constexpr int kStages = Cfg::kStages, BN = Cfg::kBN;
@@ -881,6 +881,11 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
     for (int c = 0; c < Cfg::kKept; ++c) kept[c] = 0.f;
     // KEYS: the first group holds dK, the second dV.  Otherwise each group holds half the columns of dQ.
     const uint32_t my_acc = acc + lanes + group * (KEYS ? Cfg::kAcc : Cfg::kAcc / 2);
+    // KEYS = false: of this thread's query (an absent one: probability 0).  delta comes from the forward pass' output, in bf16 rounded to
+    // 8 bits; with few keys dp - delta is a small difference of the two (two keys: 0.4% of the gradients).  The sum of p dp over
+    // the row, which delta is, comes out here: a cloud of one unit uses it at once, and the keys' kernel, which runs after this one,
+    // finds it in delta's place wherever the keys have not been split.
+    float row_base = INFINITY, row_delta = 0.f, weighted_sum = 0.f;
     const int my_columns = KEYS ? n_out : min(max(n_out - group * (Cfg::kAcc / 2), 0), Cfg::kAcc / 2);
     if (warp < 8) {
         // ---- element-wise
@@ -919,7 +924,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                 }
             }
         };
-        float row_base = INFINITY, row_delta = 0.f;  // KEYS = false: of this thread's query (an absent one: probability 0)
+        const bool whole = splits == 1 && units == 1;  // this unit has all keys of the cloud
         if (!KEYS && row < rows_here) {
             const float l = lse[(int64_t)head * num_rows + row0 + row];
             row_base = l == -INFINITY ? INFINITY : l * kLog2e;
@@ -985,14 +990,23 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                     tc_ld_32x32(buf + BN + 32 * i, t[i]);
                 }
                 tc_arrive_warp(&sh->s_free[group]);
+                float p[BN / 32][32], weighted = 0.f;
+#pragma unroll
+                for (int i = 0; i < BN / 32; ++i) {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) {
+                        p[i][c] = exp2_fast(fmaf(__uint_as_float(s[i][c]), c2, -row_base));
+                        if (valid < BN && i * 32 + c >= valid) p[i][c] = 0.f;  // a key behind the cloud: its probability may overflow
+                        if (NP == 1) weighted = fmaf(p[i][c], __uint_as_float(t[i][c]), weighted);
+                    }
+                }
+                if (NP == 1 && whole) row_delta = weighted;
+                if (NP == 1) weighted_sum += weighted;
 #pragma unroll
                 for (int i = 0; i < BN / 32; ++i) {
                     float e[32];
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        e[c] = exp2_fast(fmaf(__uint_as_float(s[i][c]), c2, -row_base)) * (__uint_as_float(t[i][c]) - row_delta);
-                        if (valid < BN && i * 32 + c >= valid) e[c] = 0.f;  // a key behind the cloud: its probability may overflow
-                    }
+                    for (int c = 0; c < 32; ++c) e[c] = p[i][c] * (__uint_as_float(t[i][c]) - row_delta);
                     if (i == 0 && u >= 2) {
                         if (!(ok = tc_wait_warp(&sh->e_done[group], ((u >> 1) - 1) & 1, limit, failed))) break;
                         tc_fence_after();
@@ -1017,6 +1031,12 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
     __syncthreads();
     const bool good = !*failed;
     if (!good && warp == 8) tc_drain_loads(sh, issued, kStages, limit);
+    if (!KEYS && NP == 1 && splits == 1) {
+        float* swap = (float*)smem;  // all products have finished
+        if (good && warp >= 4 && warp < 8) swap[row] = weighted_sum;
+        __syncthreads();
+        if (good && warp < 4 && row < rows_here) delta[(int64_t)head * num_rows + row0 + row] = weighted_sum + swap[row];
+    }
     if (good && warp < 8) {
         const float factor = KEYS && group == 1 ? 1.f : a.scale;
         const int64_t at = out0 + (int64_t)row * out_heads * a.size;
