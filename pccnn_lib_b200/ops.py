@@ -975,7 +975,7 @@ def _feature_rows(t, name, ndim, dtype=None):
         raise TypeError("%s must be a torch.Tensor" % name)
     if not t.is_cuda:
         raise RuntimeError("%s must be a CUDA tensor (pccnn_lib_b200 has no CPU path)" % name)
-    if t.dtype not in (_FEATURE_TYPES if dtype is None else (dtype,)):
+    if t.dtype != dtype and (dtype is not None or t.dtype not in _FEATURE_TYPES):
         raise RuntimeError("%s must have dtype %s, got %s" % (name, " or ".join(str(d) for d in _FEATURE_TYPES) if dtype is None
                                                               else dtype, t.dtype))
     if t.dim() != ndim:
@@ -986,10 +986,12 @@ def _feature_rows(t, name, ndim, dtype=None):
     return t if in_place else t.contiguous()
 
 
-def _same_device(**tensors):
-    devices = {t.device for t in tensors.values()}
-    if len(devices) > 1:
-        raise RuntimeError("%s must be on one device, got %s" % (", ".join(tensors), sorted(str(d) for d in devices)))
+def _same_device(*tensors):
+    device = tensors[0].device
+    for t in tensors:
+        if t.device != device:
+            raise RuntimeError("all tensors must be on one device, got %s" % sorted({str(t.device) for t in tensors}))
+    return device
 
 
 def _head_strides(t):
@@ -1001,14 +1003,13 @@ def layer_norm(features, weights, bias, eps=1e-5):
     features = _feature_rows(features, "features", 2)
     weights = _need(weights, "weights", torch.float32, 1)
     bias = _need(bias, "bias", torch.float32, 1)
-    _same_device(features=features, weights=weights, bias=bias)
+    device = _same_device(features, weights, bias)
     n, c = features.shape
     if c == 0 or weights.shape[0] != c or bias.shape[0] != c:
         raise RuntimeError("weights and bias must have one entry for each of the %d (at least one) channels" % c)
-    out = torch.empty((n, c), dtype=features.dtype, device=features.device)
-    stats = torch.empty((2, n), dtype=torch.float32, device=features.device)
-    mean, rstd = stats[0], stats[1]
-    with _on(features.device):
+    out = torch.empty((n, c), dtype=features.dtype, device=device)
+    mean, rstd = torch.empty((2, n), dtype=torch.float32, device=device).unbind(0)
+    with _on(device):
         _capi.check(_lib.pccnn_layer_norm(n, c, _p(features), features.stride(0), features.dtype == torch.bfloat16, _p(weights),
                                           _p(bias), float(eps), _p(out), _p(mean), _p(rstd), _stream()), "layer_norm")
     return [out, mean, rstd]
@@ -1020,7 +1021,7 @@ def layer_norm_grads(features, weights, mean, rstd, in_grads):
     in_grads = _feature_rows(in_grads, "in_grads", 2, features.dtype)
     weights = _need(weights, "weights", torch.float32, 1)
     mean, rstd = _need(mean, "mean", torch.float32, 1), _need(rstd, "rstd", torch.float32, 1)
-    _same_device(features=features, weights=weights, mean=mean, rstd=rstd, in_grads=in_grads)
+    _same_device(features, weights, mean, rstd, in_grads)
     n, c = features.shape
     if c == 0 or weights.shape[0] != c or mean.shape[0] != n or rstd.shape[0] != n or tuple(in_grads.shape) != (n, c):
         raise RuntimeError("layer_norm_grads: weights [C], mean and rstd [N] and in_grads [N, C] must match features [N, C]")
@@ -1038,7 +1039,7 @@ def _rotary_args(features, pts, frequencies, axis_pairs):
     features = _feature_rows(features, "features", 3)
     pts = _need(pts, "pts", torch.float32, 2)
     frequencies = _need(frequencies, "frequencies", torch.float32, 1)
-    _same_device(features=features, pts=pts, frequencies=frequencies)
+    _same_device(features, pts, frequencies)
     pairs = [int(p) for p in axis_pairs]
     if pts.shape[0] != features.shape[0] or pts.shape[1] != len(pairs):
         raise RuntimeError("pts must be [%d, %d]: a coordinate of every row for each entry of axis_pairs"
@@ -1066,7 +1067,7 @@ def rotary_positions_grads(features, pts, frequencies, axis_pairs, in_grads, wit
     """[dFeatures [N, H, D], dPts [N, A] (None where with_pts is false)] of rotary_positions."""
     features, pts, frequencies, pairs, axes = _rotary_args(features, pts, frequencies, axis_pairs)
     in_grads = _feature_rows(in_grads, "in_grads", 3, features.dtype)
-    _same_device(features=features, in_grads=in_grads)
+    _same_device(features, in_grads)
     n, h, d = features.shape
     if tuple(in_grads.shape) != (n, h, d):
         raise RuntimeError("in_grads must be [N, H, D] as features")
@@ -1086,7 +1087,7 @@ def _attention_args(queries, keys, values, query_ends, key_ends, scale):
     values = _feature_rows(values, "values", 3, queries.dtype)
     query_ends = _need(query_ends, "query_ends", torch.int32, 1)
     key_ends = _need(key_ends, "key_ends", torch.int32, 1)
-    _same_device(queries=queries, keys=keys, values=values, query_ends=query_ends, key_ends=key_ends)
+    _same_device(queries, keys, values, query_ends, key_ends)
     m, h, d = queries.shape
     if keys.shape != values.shape or keys.shape[2] != d:
         raise RuntimeError("keys and values must be [N, Hkv, %d]" % d)
@@ -1145,7 +1146,7 @@ def cross_attention_grads(queries, keys, values, query_ends, key_ends, out, lse,
     in_grads = _feature_rows(in_grads, "in_grads", 3, queries.dtype)
     out = _need(out, "out", queries.dtype, 3)
     lse = _need(lse, "lse", torch.float32, 2)
-    _same_device(queries=queries, out=out, lse=lse, in_grads=in_grads)
+    _same_device(queries, out, lse, in_grads)
     m, n, _, h, _, d, _ = shape
     if tuple(in_grads.shape) != (m, h, d) or tuple(out.shape) != (m, h, d) or tuple(lse.shape) != (h, m):
         raise RuntimeError("out and in_grads must be [M, H, D] as queries and lse [H, M]")
