@@ -762,8 +762,8 @@ static int launch_delta(const AttentionCall& a, const void* out, const HeadRows&
 }
 
 static int check_call(const char* who, const AttentionCall& a) {
-    PCCNN_CHECK_ARG(a.num_queries >= 0 && a.num_queries < 0x7fffffffLL && a.num_keys >= 0 && a.num_keys < 0x7fffffffLL && a.clouds >= 0,
-                    "%s: bad number of rows", who);
+    PCCNN_CHECK_ARG(a.num_queries >= 0 && a.num_queries < 0x7fffffffLL && a.num_keys >= 0 && a.num_keys < 0x7fffffffLL && a.clouds >= 0 && a.clouds < (1 << 30),
+                    "%s: bad number of rows or clouds", who);
     PCCNN_CHECK_ARG(a.heads > 0 && a.heads <= 1024 && a.kv_heads > 0 && a.heads % a.kv_heads == 0,
                     "%s: %d heads cannot share %d key heads (at most 1024 heads, a multiple of the key heads)", who, a.heads, a.kv_heads);
     PCCNN_CHECK_ARG(a.size > 0 && a.size <= kMaxHeadSize, "%s: head size %d outside [1, %d]", who, a.size, kMaxHeadSize);
@@ -772,13 +772,19 @@ static int check_call(const char* who, const AttentionCall& a) {
     return PCCNN_OK;
 }
 
+// The stride of a dimension of one element means nothing: it becomes that of contiguous rows.
+static HeadRows head_rows(const void* data, const int64_t* strides, int64_t rows, int heads, int size) {
+    if (!strides) return {data, 0, 0};
+    return {data, rows > 1 ? strides[0] : (int64_t)heads * size, heads > 1 ? strides[1] : size};
+}
+
 static AttentionCall describe(int64_t num_queries, int64_t num_keys, int clouds, int heads, int kv_heads, int size, int is_bf16,
                               const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                               const int64_t* v_strides, const int32_t* query_ends, const int32_t* key_ends, float scale) {
     AttentionCall a{num_queries, num_keys, clouds, heads, kv_heads, size, is_bf16, {q, 0, 0}, {k, 0, 0}, {v, 0, 0}, query_ends, key_ends, scale};
-    if (q_strides) a.q.row = q_strides[0], a.q.head = q_strides[1];
-    if (k_strides) a.k.row = k_strides[0], a.k.head = k_strides[1];
-    if (v_strides) a.v.row = v_strides[0], a.v.head = v_strides[1];
+    a.q = head_rows(q, q_strides, num_queries, heads, size);
+    a.k = head_rows(k, k_strides, num_keys, kv_heads, size);
+    a.v = head_rows(v, v_strides, num_keys, kv_heads, size);
     return a;
 }
 
@@ -850,7 +856,7 @@ int pccnn_cross_attention_grads(int64_t num_queries, int64_t num_keys, int cloud
     }
     cudaStream_t s = (cudaStream_t)stream;
     if (int rc = take_sticky_status("cross_attention_grads")) return rc;
-    const HeadRows grads{in_grads, grad_strides_host[0], grad_strides_host[1]};
+    const HeadRows grads = head_rows(in_grads, grad_strides_host, num_queries, heads, size);
     float* delta = (float*)workspace;
     char* rest = (char*)workspace + align_up((size_t)num_queries * heads * 4 + 256);
     if (num_queries > 0)

@@ -331,14 +331,16 @@ column_sums_kernel(int num_rows, int columns, const float* __restrict__ partial,
 
 constexpr int kNormMaxBlocksPerSm = 8;
 
-// Blocks of the backward kernel: what is resident at once (every block writes a row of partial sums), at most the rows' share.
+// Blocks: what is resident at once (in the backward pass every block writes a row of partial sums), at most the rows' share.
 template <class Kernel>
 static int norm_blocks(Kernel kernel, size_t shared, int64_t rows, int rows_per_block) {
+    const int64_t need = (rows + rows_per_block - 1) / rows_per_block;
+    if (need <= sm_count()) return (int)(need < 1 ? 1 : need);
     int per_sm = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kNormThreads, shared) != cudaSuccess || per_sm < 1) per_sm = 1;
     if (per_sm > kNormMaxBlocksPerSm) per_sm = kNormMaxBlocksPerSm;
-    const int64_t need = (rows + rows_per_block - 1) / rows_per_block, cap = (int64_t)sm_count() * per_sm;
-    return (int)(need < 1 ? 1 : need < cap ? need : cap);
+    const int64_t cap = (int64_t)sm_count() * per_sm;
+    return (int)(need < cap ? need : cap);
 }
 
 // Threads per row, vectors per thread and rows at once for rows of n vectors of V elements: few threads per row while that
@@ -389,9 +391,8 @@ struct NormForward {
     int64_t rows; int channels; const void* feats; int64_t ld; const float *weights, *bias; float eps;
     void* out; float *mean, *rstd; cudaStream_t s;
     template <class T, int V, int TPR, int K, int R> int run() const {
-        const int per_block = kNormThreads / TPR * R;
-        const int64_t need = (rows + per_block - 1) / per_block;
-        layer_norm_kernel<T, V, TPR, K, R><<<resident_grid(layer_norm_kernel<T, V, TPR, K, R>, need * kNormThreads, kNormThreads), kNormThreads, 0, s>>>(rows, channels, (const T*)feats, ld, weights, bias,
+        const int blocks = norm_blocks(layer_norm_kernel<T, V, TPR, K, R>, 0, rows, kNormThreads / TPR * R);
+        layer_norm_kernel<T, V, TPR, K, R><<<blocks, kNormThreads, 0, s>>>(rows, channels, (const T*)feats, ld, weights, bias,
                                                                                  eps, (T*)out, mean, rstd);
         PCCNN_LAUNCH_CHECK();
         return PCCNN_OK;

@@ -8,6 +8,7 @@
 //     in pccnn_check_status, which can also synchronise the stream first.  The word is sticky until it is read.
 //   * pccnn_validate_neighbors checks a [T, 2] list and its end offsets on the device and reports the first bad
 //     row as an error code instead of letting a later kernel fault on it.
+#include <atomic>
 #include <mutex>
 
 #include "common.cuh"
@@ -15,17 +16,22 @@
 
 namespace pccnn {
 
-static int* g_status_host = nullptr;  // one int, pinned + mapped + portable: visible to every device of the process
+static std::atomic<int*> g_status_host{nullptr};  // one int, pinned + mapped + portable: visible to every device of the process
 static std::once_flag g_status_once;
 static cudaError_t g_status_err = cudaSuccess;
 
 int* sticky_status_word() {
     std::call_once(g_status_once, [] {
-        g_status_err = cudaHostAlloc((void**)&g_status_host, 64, cudaHostAllocPortable | cudaHostAllocMapped);
+        // the first call of a process may be one that a graph captures, where an allocation is refused unless the thread says
+        // that it has nothing to do with the capture
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        int* word = nullptr;
+        g_status_err = cudaHostAlloc((void**)&word, 64, cudaHostAllocPortable | cudaHostAllocMapped);
+        cudaThreadExchangeStreamCaptureMode(&mode);
         if (g_status_err == cudaSuccess) {
-            for (int i = 0; i < 16; ++i) g_status_host[i] = 0;
-        } else {
-            g_status_host = nullptr;
+            for (int i = 0; i < 16; ++i) word[i] = 0;
+            g_status_host.store(word);
         }
     });
     return g_status_host;
@@ -74,7 +80,7 @@ static const char* origin_name(int origin) {
 }
 
 int take_sticky_status(const char* who) {
-    int* sticky = sticky_status_word();
+    int* sticky = g_status_host.load();  // without one nothing has been recorded
     if (!sticky) return PCCNN_OK;
     const int v = *(volatile int*)sticky;
     if (v == 0) return PCCNN_OK;

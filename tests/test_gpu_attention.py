@@ -467,6 +467,44 @@ def test_attention_reports_a_wait_that_ran_out_and_recovers(dtype, size):
     run_and_check(q, k, v, qe, ke, g, lengths)
 
 
+def test_the_first_call_of_a_process_can_be_a_captured_one():
+    """In a fresh process, without a call in front of the capture: kernels and the pinned status word are set up inside."""
+    import subprocess
+    import sys
+    from conftest import ROOT
+    code = """
+import sys; sys.path[:0] = [%r, %r]
+import torch, test_gpu_attention as t
+from pccnn_lib_b200 import ops
+cases = [t.attention_case(t.LENGTHS["tiles"], (4, 2), 64, dtype) for dtype in t.TYPES]
+x, w = torch.ones(9, 64, device="cuda"), torch.ones(64, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    ops.layer_norm(x, w, w)
+    held = [ops.cross_attention(*c[:5]) for c in cases]
+    held = [h + ops.cross_attention_grads(*c[:5], *h, c[5]) for c, h in zip(cases, held)]
+graph.replay()
+torch.cuda.synchronize()
+for (q, k, v, _, _, g), h in zip(cases, held):
+    t.check_attention(h[:2], t.attention(q, k, v, *t.LENGTHS["tiles"], 0.125, g), h[2:])
+ops.check_status()
+print("captured")
+""" % (ROOT, ROOT + "/tests")
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-3000:]
+
+
+def test_strides_of_single_rows_and_heads_mean_nothing():
+    lengths = ([300], [400])
+    q, k, v, qe, ke, g = attention_case(lengths, (1, 1), 64, torch.bfloat16)
+    odd = [torch.as_strided(x, x.shape, (64, 3, 1)) for x in (q, k, v, g)]  # one head: any head stride
+    run_and_check(*odd[:3], qe, ke, odd[3], lengths)
+    one = ([1], [400])
+    q, k, v, qe, ke, g = attention_case(one, (4, 4), 64, torch.bfloat16)
+    run_and_check(torch.as_strided(q, q.shape, (5, 64, 1)), k, v, qe, ke, torch.as_strided(g, g.shape, (5, 64, 1)), one)
+
+
 def test_attention_on_two_streams_at_once():
     from pccnn_lib_b200 import ops
     cases = [attention_case(LENGTHS["tiles"], (4, 2), 64, dtype, seed=90 + i) for i, dtype in enumerate(TYPES * 2)]
