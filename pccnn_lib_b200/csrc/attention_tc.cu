@@ -138,10 +138,13 @@ bool tc_layout(const AttentionCall& a, const HeadRows* grads) {
     return !a.is_bf16 || (tc_heads(a.q) && tc_heads(a.k) && tc_heads(a.v) && (!grads || tc_heads(*grads)));
 }
 
-// Splits of the streamed rows so that the blocks fill the GPU twice, as long as a split keeps at least four tiles (on average).
-static int tc_splits(int64_t blocks, int64_t streamed_per_cloud, int tile) {
+// Splits of the streamed rows where the blocks do not fill the GPU twice: enough for two blocks per SM, as long as a split keeps at
+// least 512 rows (on average).  A block costs several microseconds beside its units: 1024 latents on 120007 points take 209 us with
+// two blocks per SM, 216 us with three and 252 us with six.
+static int tc_splits(int64_t blocks, int64_t streamed_per_cloud) {
+    if (blocks >= 2 * (int64_t)sm_count()) return 1;
     int64_t s = (2 * (int64_t)sm_count() + blocks - 1) / (blocks > 0 ? blocks : 1);
-    const int64_t most = streamed_per_cloud / (4 * tile);
+    const int64_t most = streamed_per_cloud / 512;
     if (s > most) s = most;
     return (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
 }
@@ -150,7 +153,7 @@ static int64_t tc_blocks(int64_t rows, int per_block, int clouds) { return rows 
 static int tc_forward_splits(const AttentionCall& a) {
     const int per_block = a.is_bf16 ? 256 : 128, clouds = a.clouds > 0 ? a.clouds : 1;
     const int64_t blocks = ((a.num_queries + per_block - 1) / per_block + clouds / 2) * a.heads;
-    return tc_splits(blocks, a.num_keys / clouds, a.is_bf16 ? 128 : 64);
+    return tc_splits(blocks, a.num_keys / clouds);
 }
 
 size_t tc_forward_workspace(const AttentionCall& a) {
@@ -214,7 +217,7 @@ static int tc_grad_splits(const AttentionCall& a, bool keys) {
     const int64_t rows = keys ? a.num_keys : a.num_queries, streamed = keys ? a.num_queries : a.num_keys;
     const int clouds = a.clouds > 0 ? a.clouds : 1;
     const int64_t blocks = ((rows + kTcRows - 1) / kTcRows + clouds / 2) * (keys ? a.kv_heads : a.heads);
-    return tc_splits(blocks, streamed / clouds * (keys ? a.heads / a.kv_heads : 1), 64);
+    return tc_splits(blocks, streamed / clouds * (keys ? a.heads / a.kv_heads : 1));
 }
 
 size_t tc_grads_workspace(const AttentionCall& a) {

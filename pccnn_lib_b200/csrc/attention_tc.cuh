@@ -79,26 +79,57 @@ __device__ __forceinline__ void tc_arrive_warp(uint64_t* bar) {
     if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
-// The cloud of block `slot` of a grid with rows / ROWS + clouds + 1 blocks: cloud b's blocks start at
-// begin(b) / ROWS + b, which leaves room for all of them without a prefix sum.  Cloud `clouds` is the rest of the rows.
-// All lanes of a warp search together.  Returns false for a block without rows.
+// What block `slot` of a grid with rows / ROWS + clouds + 1 blocks works on: rows [row0, row_end) of a cloud (its end, not the
+// block's) and the cloud's streamed rows [begin, end).  Cloud b's blocks start at begin(b) / ROWS + b, which leaves room for
+// all of them without a prefix sum.  Cloud `clouds` is the rest of the rows; it streams nothing.  All lanes of a warp work
+// together.  Returns false for a block without rows.
 template <int ROWS>
-__device__ __forceinline__ bool tc_block_rows(const int32_t* __restrict__ ends, int clouds, int64_t n, int64_t slot, int& cloud,
-                                              int64_t& row0, int64_t& row_end) {
-    int lo = 0, hi = clouds + 1;  // the answer lies in [lo, hi)
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32, b = lo + (int)(threadIdx.x & 31) * step;
-        const bool before = b < hi && cloud_begin(ends, b, n) / ROWS + b <= slot;
-        const int count = __popc(__ballot_sync(kFullMask, before));  // lane 0's is always true for a valid range
-        const int at = lo + (count > 0 ? count - 1 : 0) * step;
-        hi = min(hi, at + step);
-        lo = at;
+__device__ __forceinline__ bool tc_block_rows(const int32_t* __restrict__ row_ends, const int32_t* __restrict__ stream_ends, int clouds,
+                                              int64_t num_rows, int64_t num_stream, int64_t slot, int64_t& row0, int64_t& row_end,
+                                              int64_t& begin, int64_t& end) {
+    const int lane = threadIdx.x & 31;
+    int64_t first;
+    int cloud;
+    if (clouds <= 30) {  // lane b has the first rows of cloud b: one round of loads
+        const int64_t rows_at = lane <= clouds ? cloud_begin(row_ends, lane, num_rows) : num_rows;
+        const int64_t stream_at = lane <= clouds ? cloud_begin(stream_ends, lane, num_stream) : num_stream;
+        const int count = __popc(__ballot_sync(kFullMask, lane <= clouds && rows_at / ROWS + lane <= slot));
+        cloud = count > 0 ? count - 1 : 0;
+        first = __shfl_sync(kFullMask, rows_at, cloud);
+        row_end = max(first, __shfl_sync(kFullMask, rows_at, cloud + 1));
+        begin = __shfl_sync(kFullMask, stream_at, cloud);
+        end = max(begin, __shfl_sync(kFullMask, stream_at, cloud + 1));
+    } else {
+        int lo = 0, hi = clouds + 1;  // the answer lies in [lo, hi)
+        while (hi - lo > 1) {
+            const int step = (hi - lo + 31) / 32, b = lo + lane * step;
+            const bool before = b < hi && cloud_begin(row_ends, b, num_rows) / ROWS + b <= slot;
+            const int count = __popc(__ballot_sync(kFullMask, before));  // lane 0's is always true for a valid range
+            const int at = lo + (count > 0 ? count - 1 : 0) * step;
+            hi = min(hi, at + step);
+            lo = at;
+        }
+        cloud = lo;
+        first = cloud_begin(row_ends, cloud, num_rows);
+        row_end = cloud_end(row_ends, cloud, clouds, num_rows);
+        begin = cloud_begin(stream_ends, cloud, num_stream);
+        end = cloud_end(stream_ends, cloud, clouds, num_stream);
     }
-    cloud = lo;
-    const int64_t begin = cloud_begin(ends, lo, n);
-    row_end = cloud_end(ends, lo, clouds, n);
-    row0 = begin + (slot - (begin / ROWS + lo)) * ROWS;
-    return row0 >= begin && row0 < row_end;
+    if (cloud >= clouds) begin = end = 0;
+    row0 = first + (slot - (first / ROWS + cloud)) * ROWS;
+    return row0 >= first && row0 < row_end;
+}
+
+// Tiles of a split: an equal share, but at least 512 rows' while there are more, so that small clouds make few splits and
+// the splits of large ones are not longer than need be.
+template <int BN>
+__device__ __forceinline__ int64_t tc_tiles_of_split(int64_t tiles, int splits) {
+    const int64_t share = (tiles + splits - 1) / splits;
+    return splits > 1 && share < 512 / BN ? 512 / BN : share;
+}
+
+__device__ __forceinline__ void tc_prefetch_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
 // ---- loads ------------------------------------------------------------------------------------------------------
@@ -405,16 +436,16 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int h = blockIdx.y, kv = h / (a.heads / a.kv_heads), split = blockIdx.z;
-    int cloud;
-    int64_t row0, row_end, begin = 0, end = 0;
-    if (!tc_block_rows<QT * kTcRows>(a.query_ends, a.clouds, a.num_queries, blockIdx.x, cloud, row0, row_end)) return;
-    const int rows_here = (int)min((int64_t)(QT * kTcRows), row_end - row0);
-    if (cloud < a.clouds) {
-        begin = cloud_begin(a.key_ends, cloud, a.num_keys);
-        end = cloud_end(a.key_ends, cloud, a.clouds, a.num_keys);
+    if (threadIdx.x == 0) {
+        tc_prefetch_map(&map_q);
+        tc_prefetch_map(&map_k);
+        tc_prefetch_map(&map_v);
     }
+    int64_t row0, row_end, begin, end;
+    if (!tc_block_rows<QT * kTcRows>(a.query_ends, a.key_ends, a.clouds, a.num_queries, a.num_keys, blockIdx.x, row0, row_end, begin, end)) return;
+    const int rows_here = (int)min((int64_t)(QT * kTcRows), row_end - row0);
     {  // this split's keys, in whole tiles
-        const int64_t tiles = (end - begin + BN - 1) / BN, per = (tiles + splits - 1) / splits;
+        const int64_t tiles = (end - begin + BN - 1) / BN, per = tc_tiles_of_split<BN>(tiles, splits);
         const int64_t lo = begin + split * per * BN;
         end = min(end, lo + per * BN);
         begin = min(lo, end);
@@ -708,7 +739,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 // memory and columns of their own: queries' gradient 534 us, keys' 598 us.
 template <bool KEYS, int GR, int NP>
 struct TcBackward {
-    static constexpr bool kKeepInTmem = NP == 3, kInPlace = NP == 3 && KEYS;
+    static constexpr bool kKeepInTmem = NP == 3 || (!KEYS && GR == 1), kInPlace = NP == 3 && KEYS;
     // streamed rows of a unit: as many as leave columns for s, t, the weights and the accumulators, and three slots of the ring (a
     // slot is held until its unit has been added, and the logits run ahead by two units)
     static constexpr int kBN = NP == 3 || (KEYS && GR == 2) ? 32 : 64;
@@ -753,16 +784,19 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
     const int32_t* row_ends = KEYS ? a.key_ends : a.query_ends;
     const int32_t* stream_ends = KEYS ? a.query_ends : a.key_ends;
     const int out_heads = KEYS ? a.kv_heads : a.heads;
-    int cloud;
-    int64_t row0, row_end, begin = 0, end = 0;
-    if (!tc_block_rows<kTcRows>(row_ends, a.clouds, num_rows, blockIdx.x, cloud, row0, row_end)) return;
-    const int rows_here = (int)min((int64_t)kTcRows, row_end - row0);
-    if (cloud < a.clouds) {
-        begin = cloud_begin(stream_ends, cloud, num_stream);
-        end = cloud_end(stream_ends, cloud, a.clouds, num_stream);
+    if (threadIdx.x == 0) {
+        if (!Cfg::kKeepInTmem) {
+            tc_prefetch_map(&map_f1);
+            tc_prefetch_map(&map_f2);
+        }
+        tc_prefetch_map(&map_y1);
+        tc_prefetch_map(&map_y2);
     }
+    int64_t row0, row_end, begin, end;
+    if (!tc_block_rows<kTcRows>(row_ends, stream_ends, a.clouds, num_rows, num_stream, blockIdx.x, row0, row_end, begin, end)) return;
+    const int rows_here = (int)min((int64_t)kTcRows, row_end - row0);
     {
-        const int64_t tiles = (end - begin + BN - 1) / BN, per = (tiles + splits - 1) / splits;
+        const int64_t tiles = (end - begin + BN - 1) / BN, per = tc_tiles_of_split<BN>(tiles, splits);
         const int64_t lo = begin + split * per * BN;
         end = min(end, lo + per * BN);
         begin = min(lo, end);
