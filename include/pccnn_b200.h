@@ -526,7 +526,10 @@ int pccnn_rotary_positions_grads(int64_t rows, int heads, int size, const void* 
  * int32 on the device, non-decreasing and within the number of rows (offsets that are not are clamped: no access leaves
  * the tensors, but the result is not defined).  heads is a multiple of kv_heads; head h reads key head
  * h / (heads / kv_heads).  size <= 256.  out [num_queries, heads, size], out_lse [heads, num_queries] float32 (natural
- * logarithm).  A query without keys (an empty cloud, a row behind the last cloud) gets zeros and an lse of minus infinity. */
+ * logarithm).  A query without keys (an empty cloud, a row behind the last cloud) gets zeros and an lse of minus infinity.
+ * Rows of other clouds never reach a result, whatever they hold; an infinity in a cloud's own features may give NaN where
+ * the formula has a limit.  A kernel that gives up a bounded wait reports as the convolutions do: PCCNN_ERR_DEVICE from the
+ * next attention or convolution call and from pccnn_check_status. */
 size_t pccnn_cross_attention_workspace_bytes(int64_t num_queries, int64_t num_keys, int clouds, int heads, int kv_heads, int size,
                                              int is_bf16);
 int pccnn_cross_attention(int64_t num_queries, int64_t num_keys, int clouds, int heads, int kv_heads, int size, int is_bf16,

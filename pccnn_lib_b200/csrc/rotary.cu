@@ -4,7 +4,8 @@
 //
 //   dx = the gradient turned by -t;      dpts[n, a] = sum_{j of a} f_j sum_h (g1 y0 - g0 y1),  y = the turned features
 //
-// Both directions are bound by HBM.  The angle of a far position has no correct digit left in 32 bits, so the product (exact
+// Both directions are bound by HBM (150000 x 8 x 64 float, 30 pairs: 102 us forward, 170 us backward with the coordinates' gradient,
+// 93% and 84% of the measured copy bandwidth).  The angle of a far position has no correct digit left in 32 bits, so the product (exact
 // in 64 bits: 24 + 24 bits) and its reduction to a fraction of a turn are 64-bit, once per (row, pair) and not per head; the
 // fraction is at most half a turn and its sine and cosine are taken in 32 bits.  A row belongs to 4 to 32 lanes of one warp,
 // which compute the row's angles into shared memory and then walk its heads; the coordinates' gradient is a sum over
