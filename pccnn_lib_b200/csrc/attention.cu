@@ -614,10 +614,10 @@ struct RowLayout {
     bool vectors;
     int chunks, lanes;
 };
-static RowLayout row_layout(const AttentionCall& a, const HeadRows* grads) {
+static RowLayout row_layout(const AttentionCall& a, const HeadRows* grads, bool outputs_aligned) {
     const int v = a.is_bf16 ? 8 : 4;
     RowLayout l;
-    l.vectors = a.size % v == 0 && vector_heads(a.q, v) && vector_heads(a.k, v) && vector_heads(a.v, v) && (!grads || vector_heads(*grads, v));
+    l.vectors = outputs_aligned && a.size % v == 0 && vector_heads(a.q, v) && vector_heads(a.k, v) && vector_heads(a.v, v) && (!grads || vector_heads(*grads, v));
     const int n = l.vectors ? a.size / v : a.size;
     l.lanes = 4;  // at least: the forward kernel spreads four keys over a row's lanes
     while (l.lanes < 32 && l.lanes < n) l.lanes *= 2;
@@ -822,7 +822,7 @@ int pccnn_cross_attention(int64_t num_queries, int64_t num_keys, int clouds, int
     }
     if (int rc = take_sticky_status("cross_attention")) return rc;  // an earlier call's tensor-core kernel gave up
     if (num_keys > 0 && tc_shape(a) && tc_layout(a, nullptr) && aligned16(out)) return tc_forward(a, out, out_lse, (char*)workspace, (cudaStream_t)stream);
-    const ForwardRows f{a, row_layout(a, nullptr), out, out_lse, (char*)workspace, (cudaStream_t)stream};
+    const ForwardRows f{a, row_layout(a, nullptr, aligned16(out)), out, out_lse, (char*)workspace, (cudaStream_t)stream};
     return is_bf16 ? dispatch_rows<__nv_bfloat16>(f.l, f) : dispatch_rows<float>(f.l, f);
 }
 
@@ -861,10 +861,10 @@ int pccnn_cross_attention_grads(int64_t num_queries, int64_t num_keys, int cloud
     char* rest = (char*)workspace + align_up((size_t)num_queries * heads * 4 + 256);
     if (num_queries > 0)
         if (int rc = launch_delta(a, out, grads, delta, s)) return rc;
-    if (num_queries > 0 && num_keys > 0 && tc_grads_shape(a) && tc_layout(a, &grads) && aligned16(out_query_grads) && aligned16(out_key_grads) &&
-        aligned16(out_value_grads))
+    const bool outputs_aligned = aligned16(out_query_grads) && aligned16(out_key_grads) && aligned16(out_value_grads);
+    if (num_queries > 0 && num_keys > 0 && tc_grads_shape(a) && tc_layout(a, &grads) && outputs_aligned)
         return tc_grads(a, grads, lse, delta, out_query_grads, out_key_grads, out_value_grads, rest, s);
-    const BackwardRows b{a, grads, row_layout(a, &grads), lse, delta, out_query_grads, out_key_grads, out_value_grads, rest, s};
+    const BackwardRows b{a, grads, row_layout(a, &grads, outputs_aligned), lse, delta, out_query_grads, out_key_grads, out_value_grads, rest, s};
     return is_bf16 ? dispatch_rows<__nv_bfloat16>(b.l, b) : dispatch_rows<float>(b.l, b);
 }
 

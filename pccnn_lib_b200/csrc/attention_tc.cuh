@@ -133,7 +133,7 @@ __device__ __forceinline__ void tc_prefetch_map(const CUtensorMap* map) {
 }
 
 // ---- loads ------------------------------------------------------------------------------------------------------
-// R rows from row0 of `head` into the tile at dst ([plane][64 features][R rows]), by one thread; completes `bytes` of `bar`.
+// R rows from row0 of `head` into the tile at dst ([plane][64 features][R rows]), by one thread; `bar` has been told the bytes.
 template <int R, int NP, int GR>
 __device__ __forceinline__ void tc_load_whole(uint8_t* dst, const CUtensorMap* map, int64_t plane_rows, int head, int64_t row0, uint64_t* bar) {
 #pragma unroll
@@ -187,7 +187,7 @@ __device__ __forceinline__ bool tc_elect() {
     return yes != 0;
 }
 
-// ---- products (one elected thread of a converged warp) ----------------------------------------------------------------------------------------
+// ---- products (one elected thread of a converged warp) ----------------------------------------------------------
 // The plane pairs of a product, smallest first; one pair (0, 0) for bf16 features.
 template <int NP> struct TcPairs;
 template <> struct TcPairs<1> {

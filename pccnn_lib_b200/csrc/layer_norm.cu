@@ -448,6 +448,12 @@ static int row_width(const void* p, int64_t ld, int channels, int element) {
     return v;
 }
 
+// The same for float columns: 16-byte alignment serves vectors of 8 elements as well (two accesses).
+static int column_width(const float* p, int channels) {
+    const int v = row_width(p, channels, channels, 4);
+    return v == 4 ? 8 : v;
+}
+
 struct NormForward {
     int64_t rows; int channels; const void* feats; int64_t ld; const float *weights, *bias; float eps;
     void* out; float *mean, *rstd; cudaStream_t s;
@@ -507,9 +513,8 @@ int pccnn_layer_norm(int64_t rows, int channels, const void* feats, int64_t ld_f
     PCCNN_CHECK_ARG(feats && weights && bias && out && out_mean && out_rstd, "layer_norm: null pointer");
     const NormForward f{rows, channels, feats, ld_feats, weights, bias, eps, out, out_mean, out_rstd, (cudaStream_t)stream};
     const int e = is_bf16 ? 2 : 4;
-    int width = row_width(feats, rows > 1 ? ld_feats : channels, channels, e);
-    width = std::min({width, row_width(out, channels, channels, e), row_width(weights, channels, channels, 4) * (channels % 8 ? 1 : 2),
-                      row_width(bias, channels, channels, 4) * (channels % 8 ? 1 : 2)});
+    const int width = std::min({row_width(feats, rows > 1 ? ld_feats : channels, channels, e), row_width(out, channels, channels, e),
+                                column_width(weights, channels), column_width(bias, channels)});
     return is_bf16 ? dispatch_norm<__nv_bfloat16>(channels, width, f) : dispatch_norm<float>(channels, width, f);
 }
 
@@ -544,7 +549,7 @@ int pccnn_layer_norm_grads(int64_t rows, int channels, const void* feats, int64_
     const int e = is_bf16 ? 2 : 4;
     const int width = std::min({row_width(feats, rows > 1 ? ld_feats : channels, channels, e), row_width(out_feat_grads, channels, channels, e),
                                 row_width(in_grads, rows > 1 ? ld_grads : channels, channels, e),
-                                row_width(weights, channels, channels, 4) * (channels % 8 ? 1 : 2)});
+                                column_width(weights, channels)});
     return is_bf16 ? dispatch_norm<__nv_bfloat16>(channels, width, b) : dispatch_norm<float>(channels, width, b);
 }
 

@@ -79,6 +79,20 @@ def test_layer_norm_reads_strided_and_unaligned_rows(dtype):
                   if other.numel() else other.double(), "unaligned")
 
 
+@pytest.mark.parametrize("channels", [64, 100, 130])
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+def test_layer_norm_with_weights_off_any_vector_boundary(channels, dtype):
+    from pccnn_lib_b200 import ops
+    x, g = draw((70, channels), 1, dtype), draw((70, channels), 2, dtype)
+    for shift_w, shift_b in ((1, 0), (0, 1), (2, 3), (3, 2)):
+        w, b = (1 + draw((channels + 4,), 3))[shift_w:shift_w + channels], draw((channels + 4,), 4)[shift_b:shift_b + channels]
+        want = norm_reference(x, w, b, 1e-5, g)
+        out, mean, rstd = ops.layer_norm(x, w, b, 1e-5)
+        check(out, want["out"], want["out_bound"], "out")
+        for got, name in zip(ops.layer_norm_grads(x, w, mean, rstd, g), ("dx", "dw", "db")):
+            check(got, want[name], want[name + "_bound"], name)
+
+
 def test_layer_norm_of_constant_rows_and_of_rows_with_infinities():
     from pccnn_lib_b200 import ops
     x = torch.full((4, 96), 3.25, device="cuda")
