@@ -145,6 +145,12 @@ layer_norm_kernel(int64_t rows, int channels, const T* __restrict__ feats, int64
             }
     };
     fetch(((int64_t)blockIdx.x * kGroups + group) * R);
+    constexpr bool kKeepColumns = K * V <= 4;  // weights and bias stay in registers where they are few
+    Row w, b;
+    if (kKeepColumns) {
+        load_columns<V, TPR, K>(weights, t, channels, w);
+        load_columns<V, TPR, K>(bias, t, channels, b);
+    }
     for (int64_t base = (int64_t)blockIdx.x * kGroups * R; base < rows; base += stride) {  // the same for the block
         const int64_t row0 = base + group * R;
         Row x[R];
@@ -177,9 +183,10 @@ layer_norm_kernel(int64_t rows, int channels, const T* __restrict__ feats, int64
             rstd[i] = sum_of(sq);
         }
         row_sums<TPR, R>(rstd, &slots[1]);
-        Row w, b;
-        load_columns<V, TPR, K>(weights, t, channels, w);
-        load_columns<V, TPR, K>(bias, t, channels, b);
+        if (!kKeepColumns) {
+            load_columns<V, TPR, K>(weights, t, channels, w);
+            load_columns<V, TPR, K>(bias, t, channels, b);
+        }
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             rstd[i] = rsqrtf(rstd[i] * inv + eps);
