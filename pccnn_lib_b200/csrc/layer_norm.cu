@@ -4,12 +4,12 @@
 //   dx = r (g w - mean_c(g w) - xhat mean_c(g w xhat)),   dw = sum_n g xhat,   db = sum_n g,   xhat = (x - mu) r
 //
 // Both directions are bound by HBM: the forward pass reads x and writes y once, the backward pass reads x and g and writes dx
-// once (500000 x 128 float: 86 us and 126 us, 92% and 94% of the measured copy bandwidth).  A row is held in the registers of TPR
+// once (500000 x 128 float: 78 us and 131 us, 102% and 91% of the measured copy bandwidth).  A row is held in the registers of TPR
 // threads (a part of a warp, a warp, or a block), so the variance is taken around the finished mean without a second read.
 // The backward kernel keeps the column sums of its rows in registers, every block writes one row of partial sums, and a
 // second small kernel adds the blocks' rows in a fixed order: no atomics, the same bits on every run.  Statistics and sums are
 // 32-bit floats whatever the features' type.  Rows of an odd number of bf16 channels are read two bytes at a time and are bound
-// by instructions: 20011 x 1001 takes 36 us forward and 41 us backward, 2.2 and 2.9 TB/s.
+// by instructions: 20011 x 1001 takes 31 us forward and 41 us backward, 2.6 and 2.9 TB/s.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -420,7 +420,7 @@ static int dispatch_rows_of(int n, const Launch& launch) {
     if constexpr (V * sizeof(T) >= 8) {
         if (n <= 8) return launch.template run<T, V, 8, 1, 4>();
         if (n <= 16) return launch.template run<T, V, 8, 2, 2>();
-        if (n <= 32) return launch.template run<T, V, 32, 1, 4>();
+        if (n <= 32) return launch.template run<T, V, 32, 1, Launch::template warp_rows<T>()>();
         if (n <= 64) return launch.template run<T, V, 32, 2, 2>();
         if (n <= 128) return launch.template run<T, V, 32, 4, 1>();
         if (n <= 256) return launch.template run<T, V, 256, 1, 4>();
@@ -464,6 +464,10 @@ static int column_width(const float* p, int channels) {
 struct NormForward {
     int64_t rows; int channels; const void* feats; int64_t ld; const float *weights, *bias; float eps;
     void* out; float *mean, *rstd; cudaStream_t s;
+    // Rows at once of a warp with one vector per lane: three 32-bit ones (500000 x 128 78 us, 100000 x 128 16.6 us; with four
+    // 90 and 17.7 us, with two 77 and 15.8 us, but 500001 x 100 69 against 66 us), four bf16 ones (200000 x 256 34.6 us;
+    // with three 42.6, with two 39.0 us).
+    template <class T> static constexpr int warp_rows() { return sizeof(T) == 4 ? 3 : 4; }
     template <class T, int V, int TPR, int K, int R> int run() const {
         const int blocks = norm_blocks(layer_norm_kernel<T, V, TPR, K, R>, 0, rows, kNormThreads / TPR * R);
         layer_norm_kernel<T, V, TPR, K, R><<<blocks, kNormThreads, 0, s>>>(rows, channels, (const T*)feats, ld, weights, bias,
@@ -482,6 +486,8 @@ struct NormForward {
 struct NormBackward {
     int64_t rows; int channels; const void* feats; int64_t ld; const float *weights, *mean, *rstd; const void* grads;
     int64_t ld_g; void* out; float *weight_grads, *bias_grads, *partial; cudaStream_t s;
+    // Four of either type: 500001 x 100 float 100 us, 700000 x 96 132 us, 500000 x 128 131 us; with three 105, 141 and 121 us.
+    template <class T> static constexpr int warp_rows() { return 4; }
     int sums(int blocks) const {
         column_sums_kernel<<<(2 * channels + 31) / 32, 1024, 0, s>>>(blocks, 2 * channels, partial, channels, weight_grads, bias_grads);
         PCCNN_LAUNCH_CHECK();
