@@ -139,26 +139,36 @@ bool tc_layout(const AttentionCall& a, const HeadRows* grads) {
 }
 
 // Splits of the streamed rows where the blocks do not fill the GPU twice: enough for two blocks per SM, as long as a split keeps at
-// least 512 rows (on average).  A block costs several microseconds beside its units: 1024 latents on 120007 points take 209 us with
-// two blocks per SM, 216 us with three and 252 us with six.
+// least 512 rows (on average).  A block costs several microseconds beside its units: 1024 latents on 120007 points took 209 us with
+// two blocks per SM, 216 us with three and 252 us with six (203 us since).
 static int tc_splits(int64_t blocks, int64_t streamed_per_cloud) {
     if (blocks >= 2 * (int64_t)sm_count()) return 1;
     int64_t s = (2 * (int64_t)sm_count() + blocks - 1) / (blocks > 0 ? blocks : 1);
-    const int64_t most = streamed_per_cloud / 512;
+    const int64_t most = streamed_per_cloud / kTcSplitRows;
     if (s > most) s = most;
     return (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
 }
 static int64_t tc_blocks(int64_t rows, int per_block, int clouds) { return rows / per_block + clouds + 1; }
 
-static int tc_forward_splits(const AttentionCall& a) {
+// Forward: a split's rows go by the mean cloud, and clouds of up to twice its keys make more splits instead of longer ones; splits
+// that a cloud does not fill write nothing but their statistics.  (Against equal numbers for all clouds, clouds of a fifth to
+// nine fifths of the mean: 1024 queries, 120007 keys, 8 heads on 4 of 64, 32 bits 650 us, so 554 us; 2000 queries, 200000 keys,
+// 16 clouds, bf16 200 us, so 184 us; 1280 queries, 20000 keys, 5 clouds 51 us, so 57 us.)
+struct TcForwardSplits {
+    int count, rows;
+};
+static TcForwardSplits tc_forward_splits(const AttentionCall& a) {
     const int per_block = a.is_bf16 ? 256 : 128, clouds = a.clouds > 0 ? a.clouds : 1;
-    const int64_t blocks = ((a.num_queries + per_block - 1) / per_block + clouds / 2) * a.heads;
-    return tc_splits(blocks, a.num_keys / clouds);
+    const int64_t blocks = ((a.num_queries + per_block - 1) / per_block + clouds / 2) * a.heads, mean = a.num_keys / clouds;
+    const int s = tc_splits(blocks, mean);
+    if (s == 1 || clouds == 1) return {s, kTcSplitRows};
+    const int64_t rows = (mean + s - 1) / s;
+    return {2 * s < kMaxSplits ? 2 * s : kMaxSplits, (int)(rows > kTcSplitRows ? rows : kTcSplitRows)};
 }
 
 size_t tc_forward_workspace(const AttentionCall& a) {
     const bool planes = !a.is_bf16;
-    const int splits = tc_forward_splits(a);
+    const int splits = tc_forward_splits(a).count;
     const size_t rows = splits > 1 ? (size_t)splits * a.num_queries * a.heads : 0;
     return operand_bytes(a.num_queries, a.heads, a.size, planes) + 2 * operand_bytes(a.num_keys, a.kv_heads, a.size, planes) +
            align_up(rows * sizeof(float2)) + align_up(rows * a.size * 4) + 256;
@@ -188,11 +198,11 @@ static int launch_forward(const AttentionCall& a, void* out, float* lse, char* w
     if (int rc = operand_map(&map_v, v, a.size, NP == 3, BN)) return rc;
     if (int rc = operand_map(&map_k8, k, a.size, NP == 3, 8)) return rc;
     if (int rc = operand_map(&map_v8, v, a.size, NP == 3, 8)) return rc;
-    const int splits = tc_forward_splits(a);
+    const auto [splits, split_rows] = tc_forward_splits(a);
     float2* stat = (float2*)ws;
     float* part = (float*)(ws + align_up((size_t)splits * a.num_queries * a.heads * sizeof(float2)));
     const dim3 grid((unsigned)tc_blocks(a.num_queries, QT * kTcRows, a.clouds), (unsigned)a.heads, (unsigned)splits);
-    kernel<<<grid, kTcThreads, Cfg::kBytes, s>>>(map_q, map_k, map_v, map_k8, map_v8, a, k.rows, v.rows, splits, (T*)out, lse, part, stat, ctl);
+    kernel<<<grid, kTcThreads, Cfg::kBytes, s>>>(map_q, map_k, map_v, map_k8, map_v8, a, k.rows, v.rows, splits, split_rows, (T*)out, lse, part, stat, ctl);
     PCCNN_LAUNCH_CHECK();
     return splits > 1 ? join_splits(a, splits, part, stat, out, lse, s) : PCCNN_OK;
 }

@@ -120,12 +120,14 @@ __device__ __forceinline__ bool tc_block_rows(const int32_t* __restrict__ row_en
     return row0 >= first && row0 < row_end;
 }
 
-// Tiles of a split: an equal share, but at least 512 rows' while there are more, so that small clouds make few splits and
-// the splits of large ones are not longer than need be.
+constexpr int kTcSplitRows = 512;  // rows that a split has at least while there are more
+
+// Tiles of a split: an equal share, but at least that of `least` rows while there are more, so that small clouds make few
+// splits and the splits of large ones are not longer than need be.
 template <int BN>
-__device__ __forceinline__ int64_t tc_tiles_of_split(int64_t tiles, int splits) {
-    const int64_t share = (tiles + splits - 1) / splits;
-    return splits > 1 && share < 512 / BN ? 512 / BN : share;
+__device__ __forceinline__ int64_t tc_tiles_of_split(int64_t tiles, int splits, int least) {
+    const int64_t share = (tiles + splits - 1) / splits, floor = (least + BN - 1) / BN;
+    return splits > 1 && share < floor ? floor : share;
 }
 
 __device__ __forceinline__ void tc_prefetch_map(const CUtensorMap* map) {
@@ -429,7 +431,7 @@ template <int GR, int BN, int NP, int QT, class T>
 __global__ void __launch_bounds__(kTcThreads, 1)
 attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_k8,
-                    const __grid_constant__ CUtensorMap map_v8, AttentionCall a, TcRows rows_k, TcRows rows_v, int splits,
+                    const __grid_constant__ CUtensorMap map_v8, AttentionCall a, TcRows rows_k, TcRows rows_v, int splits, int split_rows,
                     T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part_out, float2* __restrict__ part_stat,
                     TcControl ctl) {
     using Cfg = TcForward<GR, BN, NP, QT>;
@@ -450,7 +452,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     if (!tc_block_rows<QT * kTcRows>(a.query_ends, a.key_ends, a.clouds, a.num_queries, a.num_keys, blockIdx.x, row0, row_end, begin, end)) return;
     const int rows_here = (int)min((int64_t)(QT * kTcRows), row_end - row0);
     {  // this split's keys, in whole tiles
-        const int64_t tiles = (end - begin + BN - 1) / BN, per = tc_tiles_of_split<BN>(tiles, splits);
+        const int64_t tiles = (end - begin + BN - 1) / BN, per = tc_tiles_of_split<BN>(tiles, splits, split_rows);
         const int64_t lo = begin + split * per * BN;
         end = min(end, lo + per * BN);
         begin = min(lo, end);
@@ -805,7 +807,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
     if (!tc_block_rows<kTcRows>(row_ends, stream_ends, a.clouds, num_rows, num_stream, blockIdx.x, row0, row_end, begin, end)) return;
     const int rows_here = (int)min((int64_t)kTcRows, row_end - row0);
     {
-        const int64_t tiles = (end - begin + BN - 1) / BN, per = tc_tiles_of_split<BN>(tiles, splits);
+        const int64_t tiles = (end - begin + BN - 1) / BN, per = tc_tiles_of_split<BN>(tiles, splits, kTcSplitRows);
         const int64_t lo = begin + split * per * BN;
         end = min(end, lo + per * BN);
         begin = min(lo, end);

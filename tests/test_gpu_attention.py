@@ -303,6 +303,15 @@ def test_cross_attention_of_flat_and_peaked_rows_and_other_scales(scale_q, dtype
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("size", [64, 104])
+@pytest.mark.parametrize("lengths", [([40, 3, 5], [9000, 100, 700]), ([20, 0, 28], [3400, 3300, 3100]), ([300, 1], [5000, 0])],
+                         ids=["one-large", "equal", "one-empty"])
+def test_keys_split_between_blocks_for_clouds_of_all_sizes(lengths, size, dtype):
+    """Few queries on many keys: a split goes by the mean cloud, so clouds have more, fewer or no splits."""
+    run_and_check(*attention_case(lengths, (4, 2), size, dtype, behind=(3, 200)), lengths)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
 def test_logits_that_grow_along_the_keys(dtype):
     """Every block of keys raises the maximum, so all that was summed before has to fade."""
     lengths = ([140, 3], [900, 1000])
