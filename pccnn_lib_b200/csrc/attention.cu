@@ -171,13 +171,82 @@ __device__ __forceinline__ float sum_and_spread(const float (&s)[U], int lanes_p
     return v;
 }
 
+// The end of a block: joins the row groups of a warp, then the warps of a head in ascending order, and writes.
+template <class T, int V, int NC, int GH>
+__device__ __forceinline__ void finish_rows(const AttentionCall& a, int64_t m, int h0, int lanes_per_row, int warp_heads, int splits,
+                                            const float (&top)[GH], const float (&total)[GH], float (&acc)[GH][NC][V],
+                                            T* __restrict__ out, float* __restrict__ lse, float* __restrict__ part_out,
+                                            float2* __restrict__ part_stat) {
+    __shared__ float scratch[kRowWarps * NC * 32 * V];
+    __shared__ float stat[kRowWarps][2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slice = warp / warp_heads, split = blockIdx.z;
+    const int group = a.heads / a.kv_heads, heads_here = min(GH, (h0 / group + 1) * group - h0);
+#pragma unroll
+    for (int g = 0; g < GH; ++g) {
+        if (g >= heads_here) break;  // the same for the whole block
+        float now = top[g];
+        for (int o = lanes_per_row; o < 32; o <<= 1) now = fmaxf(now, __shfl_xor_sync(kFullMask, now, o));
+        if (lane == 0) stat[warp][0] = now;
+        __syncthreads();
+        for (int w = warp % warp_heads; w < kRowWarps; w += warp_heads) now = fmaxf(now, stat[w][0]);
+        const float from = now == -INFINITY ? 0.f : now;
+        const float fade = exp2_fast(top[g] - from);
+        float sum = total[g] * fade;
+        sum = warp_sum(sum);
+        if (lane == 0) stat[warp][1] = sum;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                acc[g][c][e] *= fade;
+                for (int o = lanes_per_row; o < 32; o <<= 1) acc[g][c][e] += __shfl_xor_sync(kFullMask, acc[g][c][e], o);
+                if (slice > 0 && lane < lanes_per_row) scratch[((warp * NC + c) * 32 + lane) * V + e] = acc[g][c][e];
+            }
+        __syncthreads();
+        if (slice == 0) {
+            for (int w = warp + warp_heads; w < kRowWarps; w += warp_heads) {
+                sum += stat[w][1];
+                if (lane < lanes_per_row) {
+#pragma unroll
+                    for (int c = 0; c < NC; ++c)
+#pragma unroll
+                        for (int e = 0; e < V; ++e) acc[g][c][e] += scratch[((w * NC + c) * 32 + lane) * V + e];
+                }
+            }
+            const int64_t at = m * a.heads + h0 + g;
+            if (splits > 1) {
+                const int64_t slot = (int64_t)split * a.num_queries * a.heads + at;
+                if (lane == 0) part_stat[slot] = make_float2(now, sum);
+                if (lane < lanes_per_row) {
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        const int d = (c * lanes_per_row + lane) * V;
+                        if (d < a.size) store_vec<float, V>(part_out + slot * a.size + d, acc[g][c]);
+                    }
+                }
+            } else {
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                if (lane == 0) lse[(int64_t)(h0 + g) * a.num_queries + m] = sum == 0.f ? -INFINITY : (now + log2f(sum)) * kLn2;
+                if (lane < lanes_per_row) {
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        const int d = (c * lanes_per_row + lane) * V;
+#pragma unroll
+                        for (int e = 0; e < V; ++e) acc[g][c][e] *= inv;
+                        if (d < a.size) store_vec<T, V>(out + at * a.size + d, acc[g][c]);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
 template <class T, int V, int NC, int GH>
 __global__ void __launch_bounds__(kRowThreads)
 attention_row_kernel(AttentionCall a, int lanes_per_row, int warp_heads, int splits, T* __restrict__ out, float* __restrict__ lse,
                      float* __restrict__ part_out, float2* __restrict__ part_stat) {
     constexpr int kUnroll = NC * V * GH > 32 ? 2 : 4;
-    __shared__ float scratch[kRowWarps * NC * 32 * V];
-    __shared__ float stat[kRowWarps][2];
     const int64_t m = blockIdx.x;
     const int group = a.heads / a.kv_heads, parts = (group + GH - 1) / GH;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slices = kRowWarps / warp_heads, slice = warp / warp_heads;
@@ -306,66 +375,165 @@ attention_row_kernel(AttentionCall a, int lanes_per_row, int warp_heads, int spl
 #pragma unroll
         for (int c = 0; c < NC; ++c) sums[g][c].get(acc[g][c]);
     }
-    // join the row groups of a warp, then the warps of a head in ascending order
+    finish_rows<T, V, NC, GH>(a, m, h0, lanes_per_row, warp_heads, splits, top, total, acc, out, lse, part_out, part_stat);
+}
+
+// d += a b for 16 rows (a), 8 columns (b) and 16 features of bf16: a0, a2 belong to the lane's first row, a1, a3 to the one eight behind.
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same for bf16 with the logits on the tensor cores: 16 keys are the rows of a product, lane (g, t) holds features of keys g
+// and g + 8 as they lie in memory, and the queries of the heads that share them are its columns, repeated, so that every
+// lane finds the logits of its own keys in its own registers: no sums over lanes, and softmax statistics per four lanes until the
+// end.  The features of a product may come in any order as long as both sides have the same one.  Values are added as above.
+template <int NC, int GH>
+__global__ void __launch_bounds__(kRowThreads)
+attention_row_products_kernel(AttentionCall a, int warp_heads, int splits, __nv_bfloat16* __restrict__ out, float* __restrict__ lse,
+                              float* __restrict__ part_out, float2* __restrict__ part_stat) {
+    using T = __nv_bfloat16;
+    static_assert(GH == 1 || GH == 4, "a column's head is its own or its lane's neighbor's");
+    constexpr int V = 8, kLanes = 4, kTiles = NC * GH > 1 ? 1 : 2;  // of 16 keys in flight; with two for heads of 64 and 1 block per SM 205 us, with one 175 us
+    const int64_t m = blockIdx.x;
+    const int group = a.heads / a.kv_heads, parts = (group + GH - 1) / GH;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slices = kRowWarps / warp_heads, slice = warp / warp_heads;
+    const int kv = blockIdx.y / parts * warp_heads + warp % warp_heads, h0 = kv * group + (blockIdx.y % parts) * GH;
+    const int heads_here = min(GH, (kv + 1) * group - h0), split = blockIdx.z;
+    const int in_row = lane % kLanes, sub = lane / kLanes;
+
+    const int b = cloud_of_row(a.query_ends, a.clouds, m);
+    int64_t begin = 0, end = 0;
+    if (b < a.clouds) {
+        begin = cloud_begin(a.key_ends, b, a.num_keys);
+        end = cloud_end(a.key_ends, b, a.clouds, a.num_keys);
+    }
+    split_range(begin, end, split, splits);
+
+    const float c2 = a.scale * kLog2e;
+    RawVec<T, V> q[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int d = (c * kLanes + in_row) * V;
+        if (d < a.size) q[c].load((const T*)a.q.data + m * a.q.row + (h0 + min(sub % GH, heads_here - 1)) * a.q.head + d);
+        else q[c].clear();
+    }
+    Lanes<V> sums[GH][NC];
+    float top[GH], total[GH];
 #pragma unroll
     for (int g = 0; g < GH; ++g) {
-        if (g >= heads_here) break;  // the same for the whole block
-        float now = top[g];
-        for (int o = lanes_per_row; o < 32; o <<= 1) now = fmaxf(now, __shfl_xor_sync(kFullMask, now, o));
-        if (lane == 0) stat[warp][0] = now;
-        __syncthreads();
-        for (int w = warp % warp_heads; w < kRowWarps; w += warp_heads) now = fmaxf(now, stat[w][0]);
-        const float from = now == -INFINITY ? 0.f : now;
-        const float fade = exp2_fast(top[g] - from);
-        float sum = total[g] * fade;
-        sum = warp_sum(sum);
-        if (lane == 0) stat[warp][1] = sum;
+        top[g] = -INFINITY;
+        total[g] = 0.f;
+        const float zero[V] = {};
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+        for (int c = 0; c < NC; ++c) sums[g][c].set(zero);
+    }
+    const T* keys = (const T*)a.k.data + kv * a.k.head;
+    const T* values = (const T*)a.v.data + kv * a.v.head;
+    const int step = slices * 16;
+    RawVec<T, V> key[kTiles][2][NC], val[kTiles][2][NC];
+    auto fetch = [&](int64_t first) {
+        const bool whole = first + (int64_t)step * (kTiles - 1) + 16 <= end;  // the same for the warp
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                acc[g][c][e] *= fade;
-                for (int o = lanes_per_row; o < 32; o <<= 1) acc[g][c][e] += __shfl_xor_sync(kFullMask, acc[g][c][e], o);
-                if (slice > 0 && lane < lanes_per_row) scratch[((warp * NC + c) * 32 + lane) * V + e] = acc[g][c][e];
-            }
-        __syncthreads();
-        if (slice == 0) {
-            for (int w = warp + warp_heads; w < kRowWarps; w += warp_heads) {
-                sum += stat[w][1];
-                if (lane < lanes_per_row) {
+        for (int u = 0; u < kTiles; ++u)
 #pragma unroll
-                    for (int c = 0; c < NC; ++c)
+            for (int r = 0; r < 2; ++r) {
+                const int64_t row = first + u * step + r * 8 + sub;
+                const T *k0 = keys + row * a.k.row, *v0 = values + row * a.v.row;
 #pragma unroll
-                        for (int e = 0; e < V; ++e) acc[g][c][e] += scratch[((w * NC + c) * 32 + lane) * V + e];
-                }
-            }
-            const int64_t at = m * a.heads + h0 + g;
-            if (splits > 1) {
-                const int64_t slot = (int64_t)split * a.num_queries * a.heads + at;
-                if (lane == 0) part_stat[slot] = make_float2(now, sum);
-                if (lane < lanes_per_row) {
-#pragma unroll
-                    for (int c = 0; c < NC; ++c) {
-                        const int d = (c * lanes_per_row + lane) * V;
-                        if (d < a.size) store_vec<float, V>(part_out + slot * a.size + d, acc[g][c]);
+                for (int c = 0; c < NC; ++c) {
+                    const int d = (c * kLanes + in_row) * V;
+                    if ((whole || row < end) && d < a.size) {
+                        key[u][r][c].load(k0 + d);
+                        val[u][r][c].load(v0 + d);
+                    } else {
+                        key[u][r][c].clear();
+                        val[u][r][c].clear();
                     }
                 }
-            } else {
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                if (lane == 0) lse[(int64_t)(h0 + g) * a.num_queries + m] = sum == 0.f ? -INFINITY : (now + log2f(sum)) * kLn2;
-                if (lane < lanes_per_row) {
+            }
+    };
+    const int64_t start = begin + slice * 16;
+    if (start < end) fetch(start);
+    for (int64_t first = start; first < end; first += (int64_t)step * kTiles) {  // the same for the warp's lanes
+        float s[GH][kTiles][2];
 #pragma unroll
-                    for (int c = 0; c < NC; ++c) {
-                        const int d = (c * lanes_per_row + lane) * V;
+        for (int u = 0; u < kTiles; ++u) {
+            float d[4] = {0.f, 0.f, 0.f, 0.f};  // keys (g, g, g + 8, g + 8), columns (2t, 2t + 1) twice
 #pragma unroll
-                        for (int e = 0; e < V; ++e) acc[g][c][e] *= inv;
-                        if (d < a.size) store_vec<T, V>(out + at * a.size + d, acc[g][c]);
-                    }
+            for (int c = 0; c < NC; ++c) {
+                mma_16x8x16(d, key[u][0][c].v.x, key[u][1][c].v.x, key[u][0][c].v.y, key[u][1][c].v.y, q[c].v.x, q[c].v.y);
+                mma_16x8x16(d, key[u][0][c].v.z, key[u][1][c].v.z, key[u][0][c].v.w, key[u][1][c].v.w, q[c].v.z, q[c].v.w);
+            }
+            if constexpr (GH == 1) {
+                s[0][u][0] = d[0];
+                s[0][u][1] = d[2];
+            } else {  // an even lane has heads 0 and 1, an odd one 2 and 3
+                const bool odd = lane & 1;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float other = __shfl_xor_sync(kFullMask, d[i], 1);
+                    s[i & 1][u][i >> 1] = odd ? other : d[i];
+                    s[2 + (i & 1)][u][i >> 1] = odd ? d[i] : other;
                 }
             }
         }
-        __syncthreads();
+        RawVec<T, V> now_val[kTiles][2][NC];
+#pragma unroll
+        for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                now_val[u][0][c] = val[u][0][c];
+                now_val[u][1][c] = val[u][1][c];
+            }
+        if (first + (int64_t)step * kTiles < end) fetch(first + (int64_t)step * kTiles);
+#pragma unroll
+        for (int g = 0; g < GH; ++g) {
+            float now = top[g];
+#pragma unroll
+            for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    s[g][u][r] = first + u * step + r * 8 + sub < end ? s[g][u][r] * c2 : -INFINITY;
+                    now = fmaxf(now, s[g][u][r]);
+                }
+            const float from = now == -INFINITY ? 0.f : now;
+            const float fade = exp2_fast(top[g] - from);
+            top[g] = now;
+            total[g] *= fade;
+#pragma unroll
+            for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    s[g][u][r] = exp2_fast(s[g][u][r] - from);
+                    total[g] += s[g][u][r];
+                }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) sums[g][c].scale(fade);
+        }
+#pragma unroll
+        for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    float f[V];
+                    now_val[u][r][c].widen(f);
+                    Lanes<V> x;
+                    x.set(f);
+#pragma unroll
+                    for (int g = 0; g < GH; ++g) sums[g][c].add_scaled(x, s[g][u][r]);
+                }
     }
+    float acc[GH][NC][V];
+#pragma unroll
+    for (int g = 0; g < GH; ++g) {
+        total[g] *= 1.f / kLanes;  // every probability is held by the lanes of its row
+#pragma unroll
+        for (int c = 0; c < NC; ++c) sums[g][c].get(acc[g][c]);
+    }
+    finish_rows<T, V, NC, GH>(a, m, h0, kLanes, warp_heads, splits, top, total, acc, out, lse, part_out, part_stat);
 }
 
 // Joins the splits of a query: W warps of a block per (query, head), each with every W-th split, joined in ascending order.
@@ -639,8 +807,8 @@ static RowLayout row_layout(const AttentionCall& a, const HeadRows* grads, bool 
 // How many blocks share the `streamed` rows of a cloud (on average) when there are `units` blocks without a split: enough to
 // give every SM about twelve blocks (clouds differ in size, and the last blocks should be short), as long as a block keeps
 // at least 256 rows.
-static int choose_splits(int64_t units, int64_t streamed_per_cloud) {
-    const int64_t want = (int64_t)sm_count() * 12;
+static int choose_splits(int64_t units, int64_t streamed_per_cloud, int blocks_per_sm = 12) {
+    const int64_t want = (int64_t)sm_count() * blocks_per_sm;
     int64_t s = units > 0 ? (want + units - 1) / units : 1;
     const int64_t most = streamed_per_cloud / 256;
     if (s > most) s = most;
@@ -661,8 +829,15 @@ static int warp_heads(const AttentionCall& a) {
     while (a.kv_heads % n) n /= 2;
     return n;
 }
+// Logits on the tensor cores, for bf16 rows that are read in vectors: 16 queries, 400000 keys, 8 heads of 64 on 2: 185 us without, 135
+// us with them and 95 us with three blocks per SM (six: 111 us); 6 heads of 32
+// on 2: 127, 62 and 52 us; 8 heads of 64 that share none 178 and 175 us, 150 queries on 301 keys, 4 heads of 32 8.3 and 6.9 us.
+// Heads of 128 that share none were slower with them (178 and 195 us), so wider ones stay with the plain kernel.
+static bool use_products(const AttentionCall& a) { return a.is_bf16 && a.size > 16 && a.size <= 64; }
+
 static int forward_splits(const AttentionCall& a) {
-    return choose_splits(a.num_queries * (a.kv_heads / warp_heads(a)) * forward_parts(a), mean_rows(a.num_keys, a.clouds));
+    const bool shared = use_products(a) && a.heads > a.kv_heads;
+    return choose_splits(a.num_queries * (a.kv_heads / warp_heads(a)) * forward_parts(a), mean_rows(a.num_keys, a.clouds), shared ? 3 : 12);
 }
 static int query_grad_splits(const AttentionCall& a) {
     return choose_splits(a.num_queries * a.heads, mean_rows(a.num_keys, a.clouds));
@@ -697,6 +872,16 @@ static int launch_rows(const AttentionCall& a, const RowLayout& l, void* out, fl
     float* part = (float*)(ws + align_up((size_t)splits * a.num_queries * a.heads * sizeof(float2)));
     const int side_by_side = warp_heads(a);
     const dim3 grid((unsigned)a.num_queries, (unsigned)(a.kv_heads / side_by_side * forward_parts(a)), (unsigned)splits);
+    if constexpr (sizeof(T) == 2 && V == 8) {
+        if (use_products(a)) {
+            const auto kernel = a.heads > a.kv_heads ? (a.size <= 32 ? attention_row_products_kernel<1, 4> : attention_row_products_kernel<2, 4>)
+                                : a.size <= 32       ? attention_row_products_kernel<1, 1>
+                                                     : attention_row_products_kernel<2, 1>;
+            kernel<<<grid, kRowThreads, 0, s>>>(a, side_by_side, splits, (T*)out, lse, part, stat);
+            PCCNN_LAUNCH_CHECK();
+            return splits > 1 ? join_splits(a, splits, part, stat, out, lse, s) : PCCNN_OK;
+        }
+    }
     if (a.heads > a.kv_heads)
         attention_row_kernel<T, V, NC, 4><<<grid, kRowThreads, 0, s>>>(a, l.lanes, side_by_side, splits, (T*)out, lse, part, stat);
     else

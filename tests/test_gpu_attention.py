@@ -311,6 +311,15 @@ def test_keys_split_between_blocks_for_clouds_of_all_sizes(lengths, size, dtype)
     run_and_check(*attention_case(lengths, (4, 2), size, dtype, behind=(3, 200)), lengths)
 
 
+@pytest.mark.parametrize("heads", [(3, 3), (8, 8), (6, 2), (5, 1), (14, 2)], ids=str)
+@pytest.mark.parametrize("size", [24, 32, 40, 64])
+def test_single_queries_in_bf16_with_logits_from_products_of_16_keys(size, heads):
+    """One query per cloud and key counts around 8 and 16, with one, two, three, four and five heads to a part of four columns."""
+    keys = [0, 1, 7, 8, 9, 15, 16, 17, 31, 33, 255, 257, 1000]
+    lengths = ([1] * len(keys), keys)
+    run_and_check(*attention_case(lengths, heads, size, torch.bfloat16, behind=(2, 5)), lengths)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
 def test_logits_that_grow_along_the_keys(dtype):
     """Every block of keys raises the maximum, so all that was summed before has to fade."""
