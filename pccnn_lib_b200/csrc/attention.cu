@@ -833,7 +833,7 @@ static int warp_heads(const AttentionCall& a) {
 // us with them and 95 us with three blocks per SM (six: 111 us); 6 heads of 32
 // on 2: 127, 62 and 52 us; 8 heads of 64 that share none 178 and 175 us, 150 queries on 301 keys, 4 heads of 32 8.3 and 6.9 us.
 // Heads of 128 that share none were slower with them (178 and 195 us), so wider ones stay with the plain kernel.
-static bool use_products(const AttentionCall& a) { return a.is_bf16 && a.size > 16 && a.size <= 64; }
+bool use_products(const AttentionCall& a) { return a.is_bf16 && a.size > 16 && a.size <= 64; }
 
 static int forward_splits(const AttentionCall& a) {
     const bool shared = use_products(a) && a.heads > a.kv_heads;

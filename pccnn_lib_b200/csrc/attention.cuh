@@ -23,6 +23,9 @@ struct AttentionCall {
 
 constexpr int kMaxSplits = 128;
 
+// Whether the row kernel of the forward pass takes its logits from products of 16 keys (bf16).
+bool use_products(const AttentionCall& a);
+
 // Tensor-core kernels (attention_tc.cu).  Whether a call may use them goes by its shape (tc_shape: the workspace does not
 // depend on anything else) and then by the layout of its tensors (tc_layout).
 bool tc_shape(const AttentionCall& a);

@@ -126,12 +126,16 @@ static double tc_work(const AttentionCall& a) {
 // Forward: tiles, except for
 //  - small calls: 150 queries, 301 keys, 2 clouds, 4 heads of 32: 9.7 us with rows, 13.5 us with tiles in bf16, 11.7 and 20 us in
 //    32 bits; one cloud of 64 queries, 300 keys, 4 heads of 64 (5e6 multiply-adds): 14.1 and 11.6, 21.2 and 19.3 us;
-//  - a query per cloud (or four 32-bit ones, which would have to be split into planes first): 16 queries, 40000 keys, 8 heads
-//    on 2: 35 us with rows, 42 us with tiles in bf16; 64 queries, 40000 keys, 16 clouds, 8 heads, 32 bits: 146 and 183 us,
-//    with 256 queries 458 and 181 us.
+//  - few queries per cloud: one in bf16 (16 queries, 40000 keys, 8 heads of 64: 21 us with rows, 47 us with tiles; 32 queries 27 and
+//    47 us, but with 400000 keys 239 and 191 us); three where heads share keys (48 queries, 8 heads on 2 of 64: 35 and 46 us with
+//    40000 keys, 182 and 190 us with 400000; four queries per cloud: 48 and 47, 237 and 191 us), six for heads of up to 32 features
+//    (96 queries, 4 heads on 1: 26 and 25, 88 and 100 us); four 32-bit ones, which would have to be split into planes first (64
+//    queries, 40000 keys, 16 clouds, 8 heads: 146 and 183 us, with 256 queries 458 and 181 us).
 bool tc_shape(const AttentionCall& a) {
     if (!tc_any_shape(a) || tc_work(a) < 4e6) return false;
-    return a.is_bf16 ? a.num_queries > a.clouds : a.num_queries * (a.heads / a.kv_heads) > 4 * (int64_t)a.clouds;
+    if (!a.is_bf16) return a.num_queries * (a.heads / a.kv_heads) > 4 * (int64_t)a.clouds;
+    const int rows = use_products(a) && a.heads > a.kv_heads ? a.size > 32 ? 3 : 6 : 1;
+    return a.num_queries > rows * (int64_t)a.clouds;
 }
 static bool tc_heads(const HeadRows& x) { return aligned16(x.data) && x.row % 8 == 0 && x.head % 8 == 0; }
 bool tc_layout(const AttentionCall& a, const HeadRows* grads) {
