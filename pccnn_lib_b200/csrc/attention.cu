@@ -305,7 +305,7 @@ attention_row_kernel(AttentionCall a, int lanes_per_row, int warp_heads, int spl
     };
     // A logit is summed over the lanes of its row while the four of an iteration part: every lane ends with one of them, and
     // its exponential is taken once and handed round.  The kernel is bound by the instructions it issues (68% of the slots
-    // with a full sum and exponential in every lane: 199 us for 400000 keys, 8 heads of 64, bf16, 16 queries; so 179 us, 4.6 TB/s).
+    // with a full sum and exponential in every lane: 199 us for 400000 keys, 8 heads of 64, bf16, 16 queries; so 178 us).
     const int64_t start = begin + slice * per_warp;
     if (start < end) fetch(start);
     for (int64_t first = start; first < end; first += (int64_t)step * kUnroll) {  // the same for the warp's lanes
