@@ -625,8 +625,9 @@ attention_delta_kernel(int64_t num_queries, int heads, int size, int lanes_per_r
 }
 
 // Queries' gradient: block = one query and head x one split of its keys.
-// DELTA: instead of the gradient, delta = sum_n p dp itself, for clouds of few keys (splits = 1): the rounding of a bf16 output is a
-// large part of dp - delta there (see attention_tc_grads_kernel).
+// DELTA: instead of the gradient, delta = sum_n p dp itself, for clouds of at most kDeltaKeys keys (splits = 1): the rounding of a
+// bf16 output is a large part of dp - delta there (see attention_tc_grads_kernel).  Larger clouds keep what is in delta.
+constexpr int kDeltaKeys = 256;
 template <class T, int V, int NC, bool DELTA>
 __global__ void __launch_bounds__(kRowThreads)
 attention_query_grads_row_kernel(AttentionCall a, HeadRows grads, int lanes_per_row, int splits, const float* __restrict__ lse,
@@ -642,6 +643,7 @@ attention_query_grads_row_kernel(AttentionCall a, HeadRows grads, int lanes_per_
         begin = cloud_begin(a.key_ends, b, a.num_keys);
         end = cloud_end(a.key_ends, b, a.clouds, a.num_keys);
     }
+    if (DELTA && end - begin > kDeltaKeys) return;  // the same for the block
     split_range(begin, end, split, splits);
     const float c2 = a.scale * kLog2e;
     const float row_lse = lse[(int64_t)h * a.num_queries + m], base = row_lse == -INFINITY ? INFINITY : row_lse * kLog2e;
@@ -905,11 +907,9 @@ static int launch_grad_rows(const AttentionCall& a, const HeadRows& grads, const
     if (a.num_queries > 0) {
         const int splits = query_grad_splits(a);
         if constexpr (sizeof(T) == 2) {
-            if (mean_rows(a.num_keys, a.clouds) <= 256) {
-                attention_query_grads_row_kernel<T, V, NC, true><<<dim3((unsigned)a.num_queries, (unsigned)a.heads), kRowThreads, 0, s>>>(
-                    a, grads, l.lanes, 1, lse, delta, (T*)dq, part);
-                PCCNN_LAUNCH_CHECK();
-            }
+            attention_query_grads_row_kernel<T, V, NC, true><<<dim3((unsigned)a.num_queries, (unsigned)a.heads), kRowThreads, 0, s>>>(
+                a, grads, l.lanes, 1, lse, delta, (T*)dq, part);
+            PCCNN_LAUNCH_CHECK();
         }
         attention_query_grads_row_kernel<T, V, NC, false><<<dim3((unsigned)a.num_queries, (unsigned)a.heads, (unsigned)splits), kRowThreads, 0, s>>>(
             a, grads, l.lanes, splits, lse, delta, (T*)dq, part);

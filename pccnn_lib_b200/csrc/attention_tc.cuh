@@ -806,9 +806,11 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
     int64_t row0, row_end, begin, end;
     if (!tc_block_rows<kTcRows>(row_ends, stream_ends, a.clouds, num_rows, num_stream, blockIdx.x, row0, row_end, begin, end)) return;
     const int rows_here = (int)min((int64_t)kTcRows, row_end - row0);
+    bool all_streamed;  // this split has all rows of the cloud (the cloud's other splits have none)
     {
         const int64_t tiles = (end - begin + BN - 1) / BN, per = tc_tiles_of_split<BN>(tiles, splits, kTcSplitRows);
         const int64_t lo = begin + split * per * BN;
+        all_streamed = per >= tiles;
         end = min(end, lo + per * BN);
         begin = min(lo, end);
     }
@@ -943,7 +945,8 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
     // KEYS = false: of this thread's query (an absent one: probability 0).  delta comes from the forward pass' output, in bf16 rounded to
     // 8 bits; with few keys dp - delta is a small difference of the two (two keys: 0.4% of the gradients).  The sum of p dp over
     // the row, which delta is, comes out here: a cloud of one unit uses it at once, and the keys' kernel, which runs after this one,
-    // finds it in delta's place wherever the keys have not been split.
+    // finds it in delta's place wherever the cloud's keys are in one split (any number of keys below kTcSplitRows, whatever the
+    // call's other clouds are: a small cloud's gradients do not depend on what it is batched with).
     float row_base = INFINITY, row_delta = 0.f, weighted_sum = 0.f;
     const int my_columns = KEYS ? n_out : min(max(n_out - group * (Cfg::kAcc / 2), 0), Cfg::kAcc / 2);
     if (warp < 8) {
@@ -983,7 +986,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                 }
             }
         };
-        const bool whole = splits == 1 && units == 1;  // this unit has all keys of the cloud
+        const bool whole = all_streamed && units == 1;  // this unit has all keys of the cloud
         if (!KEYS && row < rows_here) {
             const float l = lse[(int64_t)head * num_rows + row0 + row];
             row_base = l == -INFINITY ? INFINITY : l * kLog2e;
@@ -1090,7 +1093,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
     __syncthreads();
     const bool good = !*failed;
     if (!good && warp == 8) tc_drain_loads(sh, issued, kStages, limit);
-    if (!KEYS && NP == 1 && splits == 1) {
+    if (!KEYS && NP == 1 && all_streamed) {  // the same for the block; no other block reads or writes these rows' delta
         float* swap = (float*)smem;  // all products have finished
         if (good && warp >= 4 && warp < 8) swap[row] = weighted_sum;
         __syncthreads();
