@@ -255,6 +255,7 @@ layer_norm_grads_kernel(int64_t rows, int channels, const T* __restrict__ feats,
     const int64_t stride = (int64_t)gridDim.x * kGroups * R;
     RawVec<T, V> next_x[R][K], next_g[R][K];
     float next_mu[R], next_r[R];
+    const bool ragged = channels < TPR * K * V;  // some elements of the threads lie behind the row
     auto fetch = [&](int64_t row0) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
@@ -287,6 +288,14 @@ layer_norm_grads_kernel(int64_t rows, int channels, const T* __restrict__ feats,
             r[i] = next_r[i];
             widen_row<T, V, K>(next_x[i], x[i]);
             widen_row<T, V, K>(next_g[i], g[i]);
+            // behind the row x becomes the mean: (0 - mean) rstd may overflow, and an infinity times the zero gradient there would
+            // reach the row's sums
+            if (ragged) {
+#pragma unroll
+                for (int e = 0; e < K * V; ++e)
+                    if (((e / V) * TPR + t) * V >= channels) x[i].set(e, next_mu[i]);
+            }
+            if ((K * V) % 2) x[i].set(K * V, next_mu[i]);
         }
         if (base + stride < rows) fetch(row0 + stride);
 #pragma unroll

@@ -58,3 +58,28 @@ def test_gradients_of_a_small_cloud_do_not_depend_on_the_clouds_beside_it(size):
             check(x, want[name], bound[name], name + " alone")
             check(y[:rows], want[name], bound[name], name + " beside a large cloud")
         assert torch.equal(x, y[:rows]), name
+
+
+# ---- layer norm ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("channels", [1, 7, 20, 33, 60, 100, 120])
+def test_layer_norm_gradients_of_large_constant_rows_are_finite(channels, dtype):
+    """mean * rstd overflows, but every x - mean is zero: the normalised row is zero and the gradient is that of its mean alone."""
+    from pccnn_lib_b200 import ops
+    value = 2.0 ** 121  # up to 127 of them add up to an exact 32-bit number
+    x = draw((9, channels), 1, dtype)
+    x[2], x[5] = value, -value
+    w, b, g = 1 + draw((channels,), 2, scale=0.3), draw((channels,), 3), draw((9, channels), 4, dtype)
+    out, mean, rstd = ops.layer_norm(x, w, b)
+    assert mean[2] == value and mean[5] == -value and bool(torch.isinf(mean[2] * rstd[2]))
+    assert bool(torch.isfinite(out).all())
+    dx, dw, db = ops.layer_norm_grads(x, w, mean, rstd, g)
+    gw = (g.double() * w.double())[[2, 5]]
+    want = (gw - gw.mean(1, keepdim=True)) / math.sqrt(1e-5)
+    size = (gw.abs() + gw.abs().mean(1, keepdim=True)) / math.sqrt(1e-5)
+    check(dx[[2, 5]], want, (channels + 16) * U * size + (BF16 if dtype == torch.bfloat16 else 2 * U) * want.abs() + 1e-30, "dx")
+    rest = [0, 1, 3, 4, 6, 7, 8]
+    for got, other in zip((dx[rest], dw), ops.layer_norm_grads(x[rest], w, mean[rest], rstd[rest], g[rest])):
+        # the two rows add exact zeros to the weights' gradient; its terms (a normalised value is at most sqrt(channels)) may be added in
+        # another order
+        check(got, other.double(), 34 * U * math.sqrt(channels) * g[rest].double().abs().sum(0) if got.dim() == 1 else 0 * other.double(), "other rows")
