@@ -83,3 +83,13 @@ def test_layer_norm_gradients_of_large_constant_rows_are_finite(channels, dtype)
         # the two rows add exact zeros to the weights' gradient; its terms (a normalised value is at most sqrt(channels)) may be added in
         # another order
         check(got, other.double(), 34 * U * math.sqrt(channels) * g[rest].double().abs().sum(0) if got.dim() == 1 else 0 * other.double(), "other rows")
+
+
+# ---- layers ----------------------------------------------------------------------------------------
+def test_a_layer_cast_to_bf16_turns_by_the_same_angles():
+    from pccnn_lib_b200.pc import RotaryPositions
+    x, pts = draw((40, 4, 64), 1, torch.bfloat16), draw((40, 3), 2, scale=500.0)
+    layer = RotaryPositions(3, 64, (0.1, 10.0)).cuda()
+    want = layer(x, pts)
+    assert torch.equal(layer.bfloat16()(x, pts), want)
+    assert torch.equal(RotaryPositions(3, 64, (0.1, 10.0)).to("cuda", torch.bfloat16)(x, pts), want)
