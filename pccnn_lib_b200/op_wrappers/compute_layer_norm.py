@@ -4,7 +4,8 @@ from .. import ops
 
 
 class ComputeLayerNorm(torch.autograd.Function):
-    """Layer norm over the channels with gradients for features, weights and bias (no counterpart in the reference)."""
+    """Layer norm over the channels with gradients for features, weights and bias (no counterpart in the reference).
+    eps has none, and backward refuses one that requires it."""
 
     @staticmethod
     def forward(ctx, p_features, p_weights, p_bias, p_eps=1e-5):
@@ -15,5 +16,7 @@ class ComputeLayerNorm(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, p_grads):
+        if any(ctx.needs_input_grad[3:]):
+            raise RuntimeError("layer norm has no gradient for its eps: pass a number")
         feat_grads, weight_grads, bias_grads = ops.layer_norm_grads(*ctx.saved_tensors, p_grads)
         return feat_grads, weight_grads, bias_grads, None

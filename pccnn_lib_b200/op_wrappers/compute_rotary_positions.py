@@ -5,7 +5,8 @@ from .. import ops
 
 class ComputeRotaryPositions(torch.autograd.Function):
     """Rotary positions from point coordinates with gradients for features and points (no counterpart in the reference).
-    backward returns gradients in the positional order of forward's inputs: (features, pts, None, None)."""
+    backward returns gradients in the positional order of forward's inputs: (features, pts, None, None); frequencies have
+    none, and backward refuses ones that require it."""
 
     @staticmethod
     def forward(ctx, p_features, p_pts, p_frequencies, p_axis_pairs):
@@ -16,6 +17,8 @@ class ComputeRotaryPositions(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, p_grads):
+        if ctx.needs_input_grad[2]:
+            raise RuntimeError("rotary positions have no gradient for their frequencies: pass them without requires_grad")
         features, pts, frequencies = ctx.saved_tensors
         feat_grads, pt_grads = ops.rotary_positions_grads(features, pts, frequencies, ctx.axis_pairs_, p_grads,
                                                           with_pts=ctx.needs_input_grad[1])

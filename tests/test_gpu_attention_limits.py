@@ -93,3 +93,22 @@ def test_a_layer_cast_to_bf16_turns_by_the_same_angles():
     want = layer(x, pts)
     assert torch.equal(layer.bfloat16()(x, pts), want)
     assert torch.equal(RotaryPositions(3, 64, (0.1, 10.0)).to("cuda", torch.bfloat16)(x, pts), want)
+
+
+# ---- wrappers ----------------------------------------------------------------------------------------------
+def test_a_gradient_that_no_operator_computes_is_refused_instead_of_left_out():
+    from pccnn_lib_b200.op_wrappers import ComputeCrossAttention, ComputeLayerNorm, ComputeRotaryPositions
+    x, pts, freq = draw((20, 2, 32), 1).requires_grad_(), draw((20, 3), 2), torch.exp(draw((15,), 3)).requires_grad_()
+    out = ComputeRotaryPositions.apply(x, pts, freq, [5, 5, 5])
+    with pytest.raises(RuntimeError, match="frequencies"):
+        out.backward(torch.ones_like(out))
+    q, k, v, qe, ke, g = attention_case(([20], [30]), (2, 2), 32, torch.float32)
+    out = ComputeCrossAttention.apply(q.requires_grad_(), k, v, qe, ke, torch.tensor(0.3, requires_grad=True))
+    with pytest.raises(RuntimeError, match="scale"):
+        out.backward(g)
+    f, w = draw((20, 32), 1).requires_grad_(), draw((32,), 2)
+    out = ComputeLayerNorm.apply(f, w, w, torch.tensor(1e-5, requires_grad=True))
+    with pytest.raises(RuntimeError, match="eps"):
+        out.backward(torch.ones_like(out))
+    with torch.no_grad():  # nothing to differentiate, nothing to refuse
+        ComputeRotaryPositions.apply(x, pts, freq, [5, 5, 5])
