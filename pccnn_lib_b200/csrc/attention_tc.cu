@@ -137,7 +137,10 @@ bool tc_shape(const AttentionCall& a) {
     const int rows = use_products(a) && a.heads > a.kv_heads ? a.size > 32 ? 3 : 6 : 1;
     return a.num_queries > rows * (int64_t)a.clouds;
 }
-static bool tc_heads(const HeadRows& x) { return aligned16(x.data) && x.row % 8 == 0 && x.head % 8 == 0; }
+// What a tensor map describes: 16-byte aligned rows at positive strides below 2^40 bytes.  (A row or head that is repeated or runs
+// backwards goes to the row kernels; 32-bit features are brought into planes first and may lie in any way.)
+static bool tc_stride(int64_t s) { return s > 0 && s % 8 == 0 && s < (1ll << 39); }
+static bool tc_heads(const HeadRows& x) { return aligned16(x.data) && tc_stride(x.row) && tc_stride(x.head); }
 bool tc_layout(const AttentionCall& a, const HeadRows* grads) {
     return !a.is_bf16 || (tc_heads(a.q) && tc_heads(a.k) && tc_heads(a.v) && (!grads || tc_heads(*grads)));
 }

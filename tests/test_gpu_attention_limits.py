@@ -112,3 +112,63 @@ def test_a_gradient_that_no_operator_computes_is_refused_instead_of_left_out():
         out.backward(torch.ones_like(out))
     with torch.no_grad():  # nothing to differentiate, nothing to refuse
         ComputeRotaryPositions.apply(x, pts, freq, [5, 5, 5])
+
+
+# ---- strides that the C interface allows -------------------------------------------------------------
+def strided(t, how):
+    """(storage, address, strides) of a layout that torch itself cannot pass on, and the dense tensor it stands for."""
+    rows, heads, size = t.shape
+    e = t.element_size()
+    if how == "rows reversed":
+        return t, t.data_ptr() + (rows - 1) * heads * size * e, (-heads * size, size), t.flip(0)
+    if how == "heads reversed":
+        return t, t.data_ptr() + (heads - 1) * size * e, (heads * size, -size), t.flip(1)
+    if how == "one head for all":
+        return t, t.data_ptr(), (heads * size, 0), t[:, :1].expand(rows, heads, size)
+    return t, t.data_ptr(), (0, size), t[:1].expand(rows, heads, size)  # one row for all
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("how", ["rows reversed", "heads reversed", "one head for all", "one row for all"])
+@pytest.mark.parametrize("which", ["queries", "keys", "values", "grads"])
+def test_attention_takes_zero_and_negative_strides_through_the_c_interface(which, how, dtype):
+    from pccnn_lib_b200 import _capi, ops
+    lib, lengths = _capi.lib, ([300, 40], [260, 200])  # large enough for tiles
+    q, k, v, qe, ke, g = attention_case(lengths, (4, 4), 64, dtype, seed=7)
+    tensors = {"queries": q, "keys": k, "values": v, "grads": g}
+    passed = {n: (t, t.data_ptr(), (256, 64), t) for n, t in tensors.items()}
+    passed[which] = strided(tensors[which], how)
+    dense = [passed[n][3] for n in ("queries", "keys", "values", "grads")]
+    m, n = q.shape[0], k.shape[0]
+    shape = (m, n, 2, 4, 4, 64, int(dtype == torch.bfloat16))
+    pair = lambda s: (ctypes.c_int64 * 2)(*s)  # noqa: E731
+    inputs = [x for name in ("queries", "keys", "values") for x in (passed[name][1], pair(passed[name][2]))]
+    inputs += [qe.data_ptr(), ke.data_ptr(), 0.125]
+    out, lse = torch.empty_like(q), torch.empty((4, m), device="cuda")
+    grads = [torch.empty_like(t) for t in (q, k, v)]
+    stream = torch.cuda.current_stream().cuda_stream
+    ws = torch.empty(lib.pccnn_cross_attention_workspace_bytes(*shape), dtype=torch.uint8, device="cuda")
+    _capi.check(lib.pccnn_cross_attention(*shape, *inputs, out.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(), stream), "forward")
+    ws = torch.empty(lib.pccnn_cross_attention_grads_workspace_bytes(*shape), dtype=torch.uint8, device="cuda")
+    _capi.check(lib.pccnn_cross_attention_grads(*shape, *inputs, out.data_ptr(), lse.data_ptr(), passed["grads"][1], pair(passed["grads"][2]),
+                                                *[t.data_ptr() for t in grads], ws.data_ptr(), ws.numel(), stream), "gradients")
+    ops.check_status()
+    check_attention([out, lse], attention(*dense[:3], *lengths, 0.125, dense[3]), grads)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("how", ["rows reversed", "heads reversed", "one head for all", "one row for all"])
+def test_rotary_positions_take_zero_and_negative_strides_through_the_c_interface(how, dtype):
+    from pccnn_lib_b200 import _capi, ops
+    x, g, pts = draw((50, 4, 32), 1, dtype), draw((50, 4, 32), 2, dtype), draw((50, 3), 3)
+    freq, pairs = torch.exp(draw((15,), 4)), (ctypes.c_int32 * 3)(5, 5, 5)
+    _, px, sx, dense_x = strided(x, how)
+    _, pg, sg, dense_g = strided(g, how)
+    out, dx, dp = torch.empty_like(x), torch.empty_like(x), torch.empty_like(pts)
+    bf16, stream = int(dtype == torch.bfloat16), torch.cuda.current_stream().cuda_stream
+    _capi.check(_capi.lib.pccnn_rotary_positions(50, 4, 32, px, *sx, bf16, 3, pts.data_ptr(), freq.data_ptr(), pairs, out.data_ptr(), stream), "forward")
+    _capi.check(_capi.lib.pccnn_rotary_positions_grads(50, 4, 32, px, *sx, bf16, 3, pts.data_ptr(), freq.data_ptr(), pairs, pg, *sg, dx.data_ptr(),
+                                                       dp.data_ptr(), stream), "gradients")
+    assert torch.equal(out, ops.rotary_positions(dense_x.contiguous(), pts, freq, [5, 5, 5]))
+    want = ops.rotary_positions_grads(dense_x.contiguous(), pts, freq, [5, 5, 5], dense_g.contiguous())
+    assert torch.equal(dx, want[0]) and torch.equal(dp, want[1])
