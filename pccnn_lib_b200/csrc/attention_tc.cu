@@ -148,10 +148,10 @@ bool tc_layout(const AttentionCall& a, const HeadRows* grads) {
 // Splits of the streamed rows where the blocks do not fill the GPU twice: enough for two blocks per SM, as long as a split keeps at
 // least 512 rows (on average).  A block costs several microseconds beside its units: 1024 latents on 120007 points took 209 us with
 // two blocks per SM, 216 us with three and 252 us with six (203 us since).
-static int tc_splits(int64_t blocks, int64_t streamed_per_cloud) {
+static int tc_splits(int64_t blocks, int64_t streamed_per_cloud, int least_rows = kTcSplitRows) {
     if (blocks >= 2 * (int64_t)sm_count()) return 1;
     int64_t s = (2 * (int64_t)sm_count() + blocks - 1) / (blocks > 0 ? blocks : 1);
-    const int64_t most = streamed_per_cloud / kTcSplitRows;
+    const int64_t most = streamed_per_cloud / least_rows;
     if (s > most) s = most;
     return (int)(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
 }
@@ -230,11 +230,25 @@ bool tc_grads_shape(const AttentionCall& a) {
            (a.num_queries / 32 + 1) * (a.heads / a.kv_heads) < 0x7fffffffLL;
 }
 
+// Streamed rows that a split has at least, for the host's choice and the kernel's ranges alike: kTcSplitRows, where a query counts
+// once for every head that shares the block's keys, in whole tiles.  (With 512 queries a split whatever the heads, most of the
+// splits that the host counted had none: both passes for 1000 queries, 300 keys, bf16 heads of 64, 8 on 1 85 us, so 56 us, 8 on 2 59
+// and 45 us; 2000 queries, 1000 keys, 4 clouds, 8 on 1 90 and 60 us.  Where the splits run over into a second wave it is slower:
+// 4000 queries, 300 keys, 8 on 4 59 and 66 us.)
+static int tc_grad_split_rows(const AttentionCall& a, bool keys) {
+    const int rows = kTcSplitRows / (keys ? a.heads / a.kv_heads : 1);
+    return rows > kTcGradRows ? rows : kTcGradRows;
+}
+
 static int tc_grad_splits(const AttentionCall& a, bool keys) {
     const int64_t rows = keys ? a.num_keys : a.num_queries, streamed = keys ? a.num_queries : a.num_keys;
     const int clouds = a.clouds > 0 ? a.clouds : 1;
     const int64_t blocks = ((rows + kTcRows - 1) / kTcRows + clouds / 2) * (keys ? a.kv_heads : a.heads);
-    return tc_splits(blocks, streamed / clouds * (keys ? a.heads / a.kv_heads : 1));
+    const int s = tc_splits(blocks, streamed / clouds, tc_grad_split_rows(a, keys));
+    if (clouds > 1 || s == 1) return s;
+    // one cloud: as many splits as its tiles fill
+    const int64_t tiles = (streamed + kTcGradRows - 1) / kTcGradRows, per = (tiles + s - 1) / s;
+    return (int)((tiles + per - 1) / per);
 }
 
 size_t tc_grads_workspace(const AttentionCall& a) {
@@ -266,7 +280,7 @@ static int launch_grads(const AttentionCall& a, const TcOperand& f1, const TcOpe
     const int64_t count = rows * heads * a.size;
     float* part = (float*)ws;
     const dim3 grid((unsigned)tc_blocks(rows, kTcRows, a.clouds), (unsigned)heads, (unsigned)splits);
-    kernel<<<grid, kTcThreads, Cfg::kBytes, s>>>(m[0], m[1], m[2], m[3], m[4], m[5], a, f1.rows, f2.rows, y1.rows, y2.rows, splits, lse, delta, (T*)out1,
+    kernel<<<grid, kTcThreads, Cfg::kBytes, s>>>(m[0], m[1], m[2], m[3], m[4], m[5], a, f1.rows, f2.rows, y1.rows, y2.rows, splits, tc_grad_split_rows(a, KEYS), lse, delta, (T*)out1,
                                                  (T*)out2, part, part + splits * count, ctl);
     PCCNN_LAUNCH_CHECK();
     if (splits > 1) {

@@ -121,6 +121,7 @@ __device__ __forceinline__ bool tc_block_rows(const int32_t* __restrict__ row_en
 }
 
 constexpr int kTcSplitRows = 512;  // rows that a split has at least while there are more
+constexpr int kTcGradRows = 64;    // rows of the gradients' largest streamed tiles
 
 // Tiles of a split: an equal share, but at least that of `least` rows while there are more, so that small clouds make few
 // splits and the splits of large ones are not longer than need be.
@@ -771,6 +772,7 @@ struct TcBackward {
     static constexpr int kKept = NP == 3 ? (KEYS ? kAcc : kAcc / 2) : 1;      // columns that a thread adds up in registers
     static constexpr int kBytes = 2 * kFixed + kStages * (2 * kTile + 2 * kBN * 4) + 1024 + 512;
     static_assert(kStages >= 3 && kKeep + (kKeepInTmem ? 2 * kKeepCols : 0) <= 512 && kBytes <= 227 * 1024, "does not fit");
+    static_assert(kTcGradRows % kBN == 0, "a split has whole tiles");
 };
 
 template <bool KEYS, int GR, int NP, class T>
@@ -778,7 +780,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __grid_constant__ CUtensorMap map_f2,
                           const __grid_constant__ CUtensorMap map_y1, const __grid_constant__ CUtensorMap map_y2,
                           const __grid_constant__ CUtensorMap map_y18, const __grid_constant__ CUtensorMap map_y28, AttentionCall a,
-                          TcRows rows_f1, TcRows rows_f2, TcRows rows_y1, TcRows rows_y2, int splits, const float* __restrict__ lse,
+                          TcRows rows_f1, TcRows rows_f2, TcRows rows_y1, TcRows rows_y2, int splits, int split_rows, const float* __restrict__ lse,
                           float* __restrict__ delta, T* __restrict__ out1, T* __restrict__ out2, float* __restrict__ part1,
                           float* __restrict__ part2, TcControl ctl) {
     using Cfg = TcBackward<KEYS, GR, NP>;
@@ -808,7 +810,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
     const int rows_here = (int)min((int64_t)kTcRows, row_end - row0);
     bool all_streamed;  // this split has all rows of the cloud (the cloud's other splits have none)
     {
-        const int64_t tiles = (end - begin + BN - 1) / BN, per = tc_tiles_of_split<BN>(tiles, splits, kTcSplitRows);
+        const int64_t tiles = (end - begin + BN - 1) / BN, per = tc_tiles_of_split<BN>(tiles, splits, split_rows);
         const int64_t lo = begin + split * per * BN;
         all_streamed = per >= tiles;
         end = min(end, lo + per * BN);

@@ -172,3 +172,31 @@ def test_rotary_positions_take_zero_and_negative_strides_through_the_c_interface
     assert torch.equal(out, ops.rotary_positions(dense_x.contiguous(), pts, freq, [5, 5, 5]))
     want = ops.rotary_positions_grads(dense_x.contiguous(), pts, freq, [5, 5, 5], dense_g.contiguous())
     assert torch.equal(dx, want[0]) and torch.equal(dp, want[1])
+
+
+# ---- splits of the keys' gradient ----------------------------------------------------------------------
+@pytest.mark.parametrize("queries,heads", [(1000, (8, 1)), (1000, (8, 2)), (3000, (8, 1)), (600, (4, 1)), (2500, (3, 3)), (70, (32, 1)), (500, (48, 2))], ids=str)
+def test_every_split_of_the_keys_gradients_has_queries_of_its_own(queries, heads):
+    """One cloud: the parts in the workspace, one per split, are all written and none of them is only zeros."""
+    from pccnn_lib_b200 import _capi, ops
+    lib, keys = _capi.lib, 300
+    q, k, v, qe, ke, g = attention_case(([queries], [keys]), heads, 64, torch.bfloat16, seed=3)
+    out, lse = ops.cross_attention(q, k, v, qe, ke)
+    shape = (queries, keys, 1, heads[0], heads[1], 64, 1)
+    need, count = lib.pccnn_cross_attention_grads_workspace_bytes(*shape), keys * heads[1] * 64
+    ws = torch.full((need // 4,), float("nan"), device="cuda")
+    pair = lambda t: (ctypes.c_int64 * 2)(*t.stride()[:2])  # noqa: E731
+    grads = [torch.empty_like(t) for t in (q, k, v)]
+    _capi.check(lib.pccnn_cross_attention_grads(
+        *shape, q.data_ptr(), pair(q), k.data_ptr(), pair(k), v.data_ptr(), pair(v), qe.data_ptr(), ke.data_ptr(), 0.125, out.data_ptr(), lse.data_ptr(),
+        g.data_ptr(), pair(g), *[t.data_ptr() for t in grads], ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream), "gradients")
+    ops.check_status()
+    check_attention([out, lse], attention(q, k, v, [queries], [keys], 0.125, g), grads)
+    delta = (queries * heads[0] * 4 + 256 + 255) // 256 * 256  # the row sums lie in front of the parts
+    parts = ws[delta // 4:]
+    parts = parts[:len(parts) // count * count].view(-1, count)
+    written = ~torch.isnan(parts).any(1)
+    splits = int(written.sum())
+    assert splits % 2 == 0 and bool(written[:splits].all())  # dK's parts, then dV's
+    assert splits <= 2 or bool((parts[:splits] != 0).any(1).all()), (parts[:splits] != 0).any(1).tolist()
+    assert need <= delta + splits * count * 4 + 4096  # nothing is asked for that no split uses
