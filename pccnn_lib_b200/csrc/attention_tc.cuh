@@ -29,6 +29,7 @@ namespace pccnn {
 constexpr int kTcThreads = 352;
 constexpr int kTcRows = 128;  // rows of the tile whose products have them as the M dimension
 constexpr int kTcMaxStages = 8;
+constexpr int kTcRoundRows = 65536;  // streamed rows that a bf16 accumulator takes before it is emptied: 4096 sums of 16 rows, each truncated by at most 2^-23
 
 // bf16 rows [planes][rows, heads, size] for the loads that TMA does not do.
 struct TcRows {
@@ -321,6 +322,19 @@ __device__ __forceinline__ void tc_add_columns(uint32_t from, int n, float (&sum
     }
 }
 
+// sum[c] = sum[c] fade + column c, or the column alone where the sums start.  For sums of rounds of many units: they lie in local
+// memory (the loop keeps them out of the registers), which only calls with long clouds reach.
+template <int N>
+__device__ __forceinline__ void tc_empty_columns(uint32_t from, int n, bool start, float fade, float (&sum)[N]) {
+#pragma unroll 1
+    for (int c = 0; c < n; c += 16) {
+        uint32_t r[16];
+        tc_ld_32x16(from + c, r);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum[c + i] = start ? __uint_as_float(r[i]) : fmaf(sum[c + i], fade, __uint_as_float(r[i]));
+    }
+}
+
 template <class T>
 __device__ __forceinline__ void tc_write16(T* __restrict__ dst, int c, int size, const float (&x)[16]) {
 #pragma unroll
@@ -401,8 +415,10 @@ __device__ __forceinline__ void tc_drain_loads(TcShared* sh, int issued, int sta
 // (keys u / 2, tile u % 2); with one, unit u is key tile u, and the two element-wise groups take every other one, each with an
 // accumulator, running maximum and sum of its own that are joined at the end.
 // The tensor cores truncate when they add to an accumulator (measured on 32-bit heads of 64, 1000 keys: 3.7e-6 of the output with
-// one accumulator for all keys), which bf16 weights hide and 32-bit features do not: for those every unit starts its
-// accumulator anew and the thread of a row adds the units up in registers, rounding to nearest.
+// one accumulator for all keys).  For 32-bit features every unit starts its accumulator anew and the thread of a row adds the
+// units up in registers, rounding to nearest.  bf16 weights hide the truncation of some 10^4 keys but not of any number (3 million
+// keys: 1.6% of the output), so there an accumulator is emptied every kTcRoundRows rows, which bounds it by 2^-11, an eighth of the
+// bf16 output's half step.
 // Measured: 40001 queries, 20003 keys, 16 clouds, 8 heads on 2 of 128, bf16: 371 us, 727 TFLOP/s (44% of a cuBLAS product), tensor
 // pipe 38% active: bound by the chain logits, probabilities, sums with two units in flight, and by products of 64 keys, which
 // read their 128 rows from shared memory longer (48 cycles) than they compute (32).  Heads of 64, 30011 queries and
@@ -422,6 +438,7 @@ struct TcForward {
     static constexpr int kWeights = 2 * BN;             // columns of the probabilities, behind the logits of both groups
     static constexpr int kWeightCols = NP * (BN / 2);   // of one group
     static constexpr int kAcc = kWeights + 2 * kWeightCols;
+    static constexpr int kRound = kTcRoundRows / BN;    // units of a group between two emptyings (bf16)
     static constexpr int kBytes = kQ + kStages * kSlot + 1024 + 512;
     static_assert(QT == 1 || NP == 1, "two query tiles are loaded as one plane");
     static_assert(kStages >= 4 && kStages % 2 == 0 && kAcc + 2 * GR * 64 <= 512, "does not fit");
@@ -551,7 +568,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             tc_fence_after();
             if (leader) {
                 tc_weights_by_rows<NP, GR, BN>(acc + (u & 1) * GR * 64, tmem + Cfg::kWeights + (u & 1) * Cfg::kWeightCols,
-                                               smem_u32(ring + slot * Cfg::kSlot), n_out, (valid + 15) >> 4, NP == 1 && u >= 2);
+                                               smem_u32(ring + slot * Cfg::kSlot), n_out, (valid + 15) >> 4, NP == 1 && (u >> 1) % Cfg::kRound != 0);
                 if (last) tc_commit(&sh->empty[slot]);
                 tc_commit(&sh->e_done[u & 1]);
             }
@@ -564,9 +581,13 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of tensor memory, in the address's upper half
     const float c2 = a.scale * kLog2e;
     float base = -INFINITY, total = 0.f;  // reference of the exponents (log2 units) and sum of the probabilities
-    float kept[NP == 3 ? GR * 64 : 1];    // the output of all units but the last, for 32-bit features
+    float kept[GR * 64];  // the output of all units but the last, for 32-bit features; of the emptied rounds in bf16, relative to kept_base
+    if constexpr (NP == 3) {
 #pragma unroll
-    for (int c = 0; c < (NP == 3 ? GR * 64 : 1); ++c) kept[c] = 0.f;
+        for (int c = 0; c < GR * 64; ++c) kept[c] = 0.f;
+    }
+    bool emptied = false;
+    float kept_base = -INFINITY, kept_fade = 0.f;
     bool ok = true;
     if (warp < 8) {
         // ---- element-wise: logits to probabilities
@@ -603,8 +624,13 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 if (!(ok = tc_wait_warp(&sh->e_done[group], ((u >> 1) - 1) & 1, limit, failed))) break;
                 tc_fence_after();
             }
+            const bool fresh = (u >> 1) % Cfg::kRound == 0;
             if constexpr (NP == 3) {
                 if (u >= 2) tc_add_columns<GR * 64>(my_acc, n_out, kept);
+            } else if (u >= 2 && fresh) {
+                tc_empty_columns<GR * 64>(my_acc, n_out, !emptied, exp2_fast(kept_base - (base == -INFINITY ? 0.f : base)), kept);
+                kept_base = base;
+                emptied = true;
             }
             if (__any_sync(kFullMask, live && !(top <= base + 8.f))) {
                 const float now = fmaxf(base, top), fade = exp2_fast(base - (now == -INFINITY ? 0.f : now));
@@ -613,7 +639,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 if constexpr (NP == 3) {
 #pragma unroll
                     for (int c = 0; c < GR * 64; ++c) kept[c] *= fade;
-                } else if (u >= 2) {
+                } else if (u >= 2 && !fresh) {
 #pragma unroll 1
                     for (int c = 0; c < n_out; c += 16) {
                         uint32_t r[16];
@@ -660,6 +686,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         if constexpr (NP == 3) {
             if (ok && group < units) tc_add_columns<GR * 64>(my_acc, n_out, kept);
         }
+        kept_fade = exp2_fast(kept_base - (base == -INFINITY ? 0.f : base));
     }
     __syncthreads();
     const bool good = !*failed;
@@ -678,6 +705,10 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             tc_ld_32x16(acc + lanes + group * GR * 64 + c, r);
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(r[i]);
+            if (emptied) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = fmaf(kept[c + i], kept_fade, x[i]);
+            }
         }
     };
     // ---- joining the two groups of a single query tile, through the shared memory of the tiles
@@ -739,7 +770,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 //   s = Q K^T, t = dO V^T, e = exp(scale s - lse) (t - delta),  dQ += e K.
 // KEYS = true: block = 128 keys of one cloud and key head; it keeps K and V and streams Q and dO of every head that shares them:
 //   s = K Q^T, t = V dO^T, p = exp(scale s - lse), e = p (t - delta),  dK += e Q,  dV += p dO.
-// For 32-bit features the accumulators are emptied into registers every kRound units (see the forward kernel on truncation).
+// The accumulators are emptied every kRound units, for 32-bit features into registers (see the forward kernel on truncation).
 // Measured on the calls of the forward kernel: bf16 618 us (queries) and 797 us (keys), tensor pipe 36% active; the queries'
 // kernel waits for logits 40% of the time, the keys' is bound by its products, which take 82 cycles each where 32 to 48
 // would do (two warps issue them in turn; with one warp they take 45 to 58, but it waits as long in between).  32 bits:
@@ -768,8 +799,8 @@ struct TcBackward {
     static constexpr int kAcc = GR * 64;
     static constexpr int kKeep = kAccStart + (KEYS ? 2 : 1) * kAcc;           // the tiles that stay: planes of GR x 32 columns
     static constexpr int kKeepCols = NP * GR * 32;
-    static constexpr int kRound = 4;                                          // even: both groups have units in a round
-    static constexpr int kKept = NP == 3 ? (KEYS ? kAcc : kAcc / 2) : 1;      // columns that a thread adds up in registers
+    static constexpr int kRound = NP == 3 ? 4 : kTcRoundRows / kBN;           // even: both groups have units in a round
+    static constexpr int kKept = KEYS ? kAcc : kAcc / 2;                      // columns of which a thread adds the rounds up
     static constexpr int kBytes = 2 * kFixed + kStages * (2 * kTile + 2 * kBN * 4) + 1024 + 512;
     static_assert(kStages >= 3 && kKeep + (kKeepInTmem ? 2 * kKeepCols : 0) <= 512 && kBytes <= 227 * 1024, "does not fit");
     static_assert(kTcGradRows % kBN == 0, "a split has whole tiles");
@@ -917,7 +948,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
         bool ok = true;
         for (int u = 0; u < units && ok; ++u) {
             ok = tc_wait_warp(&sh->e_ready[u & 1], (u >> 1) & 1, limit, failed);
-            const bool fresh = u == 0 || (NP == 3 && u % Cfg::kRound == 0);
+            const bool fresh = u % Cfg::kRound == 0;
             if (u > 0 && fresh) ok = ok && tc_wait_warp(&sh->acc_free, (u / Cfg::kRound - 1) & 1, limit, failed);
             if (!ok) break;
             tc_fence_after();
@@ -930,7 +961,7 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                                                    !fresh);
                 tc_commit(&sh->empty[s]);
                 tc_commit(&sh->e_done[u & 1]);
-                if (NP == 3 && (u + 1) % Cfg::kRound == 0 && u + 1 < units) tc_commit(&sh->round_done);
+                if ((u + 1) % Cfg::kRound == 0 && u + 1 < units) tc_commit(&sh->round_done);
             }
             __syncwarp();
         }
@@ -940,8 +971,11 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
     const int group = warp >> 2, row = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     float kept[Cfg::kKept];
+    if constexpr (NP == 3) {
 #pragma unroll
-    for (int c = 0; c < Cfg::kKept; ++c) kept[c] = 0.f;
+        for (int c = 0; c < Cfg::kKept; ++c) kept[c] = 0.f;
+    }
+    int emptied = 0;  // rounds
     // KEYS: the first group holds dK, the second dV.  Otherwise each group holds half the columns of dQ.
     const uint32_t my_acc = acc + lanes + group * (KEYS ? Cfg::kAcc : Cfg::kAcc / 2);
     // KEYS = false: of this thread's query (an absent one: probability 0).  delta comes from the forward pass' output, in bf16 rounded to
@@ -977,15 +1011,13 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
             tc_wait_st();
             tc_arrive_warp(&sh->fixed_full);
         }
-        int emptied = 0;
-        auto empty_until = [&](int round) {  // the accumulators of the rounds before `round` into registers
-            if constexpr (NP == 3) {
-                for (; emptied < round && ok; ++emptied) {
-                    if (!(ok = tc_wait_warp(&sh->round_done, emptied & 1, limit, failed))) break;
-                    tc_fence_after();
-                    tc_add_columns<Cfg::kKept>(my_acc, my_columns, kept);
-                    tc_arrive_warp(&sh->acc_free);
-                }
+        auto empty_until = [&](int round) {  // adds up the accumulators of the rounds before `round`
+            for (; emptied < round && ok; ++emptied) {
+                if (!(ok = tc_wait_warp(&sh->round_done, emptied & 1, limit, failed))) break;
+                tc_fence_after();
+                if constexpr (NP == 3) tc_add_columns<Cfg::kKept>(my_acc, my_columns, kept);
+                else tc_empty_columns<Cfg::kKept>(my_acc, my_columns, emptied == 0, 1.f, kept);
+                tc_arrive_warp(&sh->acc_free);
             }
         };
         const bool whole = all_streamed && units == 1;  // this unit has all keys of the cloud
@@ -1118,7 +1150,13 @@ attention_tc_grads_kernel(const __grid_constant__ CUtensorMap map_f1, const __gr
                 uint32_t r[16];
                 tc_ld_32x16(my_acc + c, r);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(r[i]) * factor;
+                for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(r[i]);
+                if (emptied > 0) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] += kept[c + i];
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] *= factor;
             }
             if (row < rows_here) {
                 if (splits > 1) tc_write16<float>(part + shift + at, column0 + c, a.size, x);

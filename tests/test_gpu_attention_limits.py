@@ -200,3 +200,85 @@ def test_every_split_of_the_keys_gradients_has_queries_of_its_own(queries, heads
     assert splits % 2 == 0 and bool(written[:splits].all())  # dK's parts, then dV's
     assert splits <= 2 or bool((parts[:splits] != 0).any(1).all()), (parts[:splits] != 0).any(1).tolist()
     assert need <= delta + splits * count * 4 + 4096  # nothing is asked for that no split uses
+
+
+# ---- long clouds -----------------------------------------------------------------------------------------
+# The tensor cores truncate when they add to an accumulator: up to 2^-23 of it for every 16 rows.  Emptied every 65536 rows, that
+# stays below (65536 / 16) 2^-23 = 2^-11 whatever the length; the sums of the emptied parts are rounded to nearest.
+LONG_DRIFT = 2.0 ** -11
+# The probabilities' roundings to bf16 (2^-8 of each at most) are independent and of mean zero: 2^-8 sqrt(sum p^2) / sum p of a sum, which is
+# 2^-8 e^(s^2 / 2) / sqrt(n) for logits of spread s, here below 1.5: 7e-6 for three million.  Fourteen of them, with the
+# 32-bit roundings of logits and sums (below 1e-5).
+LONG_SPREAD = 1e-4
+
+
+def half_step(x):
+    """Half the distance of bf16 numbers at x."""
+    return 2.0 ** (math.floor(math.log2(abs(x))) - 8)
+
+
+@pytest.mark.parametrize("size", [64, 128])
+def test_bf16_outputs_of_a_cloud_of_three_million_keys_do_not_drift(size):
+    """All values of a feature are the same, so the output is that value whatever the probabilities are."""
+    from pccnn_lib_b200 import ops
+    n, m, heads = 3000000, 9600, 8  # enough blocks that the keys are not split
+    q, k = draw((m, heads, size), 1, torch.bfloat16), draw((n, 1, size), 2, torch.bfloat16)
+    v = torch.ones((n, 1, size), dtype=torch.bfloat16, device="cuda")
+    value = 1.9921875  # 255 / 128: half a step of bf16 is 2^-8 of 2
+    v[:, :, 1::2] = -value
+    v[:, :, 0::2] = value
+    out, lse = ops.cross_attention(q, k, v, ends_of([m]), ends_of([n]))
+    ops.check_status()
+    bound = half_step(value) + value * (LONG_DRIFT + LONG_SPREAD)
+    assert float((out[..., 0::2].double() - value).abs().max()) <= bound
+    assert float((out[..., 1::2].double() + value).abs().max()) <= bound
+
+
+def test_bf16_value_gradients_of_a_cloud_of_three_million_queries_do_not_drift():
+    from pccnn_lib_b200 import ops
+    n, m, size = 49056, 3000000, 64
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(3)
+    q, k, v = draw((m, 1, size), 1, torch.bfloat16, 0.5), draw((n, 1, size), 2, torch.bfloat16), draw((n, 1, size), 3, torch.bfloat16)
+    g = torch.full((m, 1, size), 1.3359375, dtype=torch.bfloat16, device="cuda")
+    qe, ke = ends_of([m]), ends_of([n])
+    out, lse = ops.cross_attention(q, k, v, qe, ke)
+    dv = ops.cross_attention_grads(q, k, v, qe, ke, out, lse, g)[2]
+    ops.check_status()
+    some = torch.arange(0, n, 1531, device="cuda")
+    total = torch.zeros(len(some), dtype=torch.float64, device="cuda")
+    for a in range(0, m, 250000):  # lse is a 32-bit result, tested elsewhere: off by some 2^-22
+        logits = q[a:a + 250000, 0].double() @ k[some, 0].double().t() / math.sqrt(size)
+        total += torch.exp(logits - lse[0, a:a + 250000].double()[:, None]).sum(0)
+    want = (1.3359375 * total)[:, None].expand(-1, size)
+    off = torch.tensor([half_step(float(x)) for x in want[:, 0]], device="cuda", dtype=torch.float64)[:, None]
+    check(dv[some, 0], want, off + want * (LONG_DRIFT + LONG_SPREAD), "dv")
+
+
+@pytest.mark.parametrize("size", [64, 128])
+def test_bf16_rounds_of_a_long_cloud_fade_as_the_maximum_grows(size):
+    """Logits that grow by 12 along 300000 keys, whose first values are positive and last ones negative: the output and the queries'
+    gradient tell how much each part weighs."""
+    from pccnn_lib_b200 import ops
+    n, m, heads, scale = 300000, 9600, 8, size ** -0.5
+    q, k = draw((m, heads, size), 1, torch.bfloat16, 0.1), draw((n, 1, size), 2, torch.bfloat16, 0.1)
+    q[..., 0] = 1 / scale
+    k[:, 0, 0] = torch.linspace(0, 12, n, device="cuda").to(torch.bfloat16)
+    v, g = torch.full((n, 1, size), 1.3359375, dtype=torch.bfloat16, device="cuda"), torch.zeros_like(q)
+    v[n - 20000:], g[..., 0] = -1.3359375, 1.0
+    qe, ke = ends_of([m]), ends_of([n])
+    out, lse = ops.cross_attention(q, k, v, qe, ke)
+    dq = ops.cross_attention_grads(q, k, v, qe, ke, out, lse, g)[0]
+    ops.check_status()
+    Q, K, V = q[::1200].double(), k[:, 0].double(), v[:, 0, 0].double()
+    s = Q @ K.t() * scale
+    p = torch.softmax(s, -1)
+    # 25000 keys weigh 1 / e of the largest or more: the probabilities' roundings add up to 2^-8 * 3 / sqrt(25000) = 7e-5 of the sums;
+    # fourteen of them.  A logit of up to 12 is summed in 32 bits: 100 U of a probability.
+    spread = 1e-3 + 200 * U
+    want = (p * V).sum(-1)
+    check(out[::1200], want[..., None].expand(-1, -1, size), (BF16 * want.abs() + 1.3359375 * (LONG_DRIFT + spread))[..., None].expand(-1, -1, size), "out")
+    ds = p * (V - want[..., None])
+    # delta comes from the rounded output
+    bound = scale * ((ds.abs() * (LONG_DRIFT + spread) + p * (BF16 * want.abs() + 1.3359375 * (LONG_DRIFT + spread))[..., None]) @ K.abs())
+    check(dq[::1200], scale * ds @ K, bound + BF16 * ((scale * ds @ K).abs() + bound), "dq")
