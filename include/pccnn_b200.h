@@ -515,7 +515,8 @@ int pccnn_layer_norm_grads(int64_t rows, int channels, const void* feats, int64_
 int pccnn_rotary_positions(int64_t rows, int heads, int size, const void* feats, int64_t row_stride, int64_t head_stride,
                            int is_bf16, int num_axes, const float* pts, const float* frequencies, const int32_t* axis_pairs_host,
                            void* out, void* stream);
-/* Its gradients: features [rows, heads, size] and, where out_pt_grads is not null, points [rows, num_axes]. */
+/* Its gradients: features [rows, heads, size] and, where out_pt_grads is not null, points [rows, num_axes]
+ * (feats is read for them alone and may be null otherwise). */
 int pccnn_rotary_positions_grads(int64_t rows, int heads, int size, const void* feats, int64_t row_stride, int64_t head_stride,
                                  int is_bf16, int num_axes, const float* pts, const float* frequencies,
                                  const int32_t* axis_pairs_host, const void* in_grads, int64_t grad_row_stride,

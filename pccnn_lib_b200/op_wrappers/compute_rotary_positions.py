@@ -10,7 +10,8 @@ class ComputeRotaryPositions(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, p_features, p_pts, p_frequencies, p_axis_pairs):
-        ctx.save_for_backward(p_features, p_pts, p_frequencies)
+        # only the points' gradient reads the features
+        ctx.save_for_backward(p_features if ctx.needs_input_grad[1] else None, p_pts, p_frequencies)
         ctx.axis_pairs_ = p_axis_pairs
         return ops.rotary_positions(p_features, p_pts, p_frequencies, p_axis_pairs)
 

@@ -1075,18 +1075,22 @@ def rotary_positions(features, pts, frequencies, axis_pairs):
 
 
 def rotary_positions_grads(features, pts, frequencies, axis_pairs, in_grads, with_pts=True):
-    """[dFeatures [N, H, D], dPts [N, A] (None where with_pts is false)] of rotary_positions."""
-    features, pts, frequencies, pairs, axes = _rotary_args(features, pts, frequencies, axis_pairs)
-    in_grads = _feature_rows(in_grads, "in_grads", 3, features.dtype)
-    _same_device(features, in_grads)
-    n, h, d = features.shape
+    """[dFeatures [N, H, D], dPts [N, A] (None where with_pts is false)] of rotary_positions.  Only the points' gradient reads
+    the features: without it they may be None."""
+    if features is None and with_pts:
+        raise RuntimeError("the points' gradient needs the features")
+    like = in_grads if features is None else features
+    rows, pts, frequencies, pairs, axes = _rotary_args(like, pts, frequencies, axis_pairs)
+    in_grads = rows if features is None else _feature_rows(in_grads, "in_grads", 3, rows.dtype)
+    _same_device(rows, in_grads)
+    n, h, d = rows.shape
     if tuple(in_grads.shape) != (n, h, d):
         raise RuntimeError("in_grads must be [N, H, D] as features")
-    d_f = _packed_like(features)
+    d_f = _packed_like(in_grads)
     d_p = _packed_like(pts) if with_pts else None
-    with _on(features.device):
-        _capi.check(_lib.pccnn_rotary_positions_grads(n, h, d, _p(features), features.stride(0), features.stride(1),
-                                                      features.dtype == torch.bfloat16, axes, _p(pts), _p(frequencies), pairs,
+    with _on(rows.device):
+        _capi.check(_lib.pccnn_rotary_positions_grads(n, h, d, _p(rows) if with_pts else None, rows.stride(0), rows.stride(1),
+                                                      rows.dtype == torch.bfloat16, axes, _p(pts), _p(frequencies), pairs,
                                                       _p(in_grads), in_grads.stride(0), in_grads.stride(1), _p(d_f), _p(d_p),
                                                       _stream()), "rotary_positions_grads")
     return [d_f, d_p]

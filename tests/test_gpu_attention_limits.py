@@ -282,3 +282,21 @@ def test_bf16_rounds_of_a_long_cloud_fade_as_the_maximum_grows(size):
     # delta comes from the rounded output
     bound = scale * ((ds.abs() * (LONG_DRIFT + spread) + p * (BF16 * want.abs() + 1.3359375 * (LONG_DRIFT + spread))[..., None]) @ K.abs())
     check(dq[::1200], scale * ds @ K, bound + BF16 * ((scale * ds @ K).abs() + bound), "dq")
+
+
+def test_rotary_positions_keep_their_features_only_for_the_points_gradient():
+    from pccnn_lib_b200 import ops
+    from pccnn_lib_b200.op_wrappers import ComputeRotaryPositions
+    x, pts, freq, g = draw((50, 3, 32), 1).requires_grad_(), draw((50, 3), 2), torch.exp(draw((15,), 3)), draw((50, 3, 32), 4)
+    out = ComputeRotaryPositions.apply(x, pts, freq, [5, 5, 5])
+    assert all(t is None or t.shape != x.shape for t in out.grad_fn.saved_tensors)
+    out.backward(g)
+    dx, none = ops.rotary_positions_grads(None, pts, freq, [5, 5, 5], g, with_pts=False)
+    assert none is None and torch.equal(x.grad, dx) and torch.equal(dx, ops.rotary_positions_grads(x.detach(), pts, freq, [5, 5, 5], g)[0])
+    with pytest.raises(RuntimeError, match="features"):
+        ops.rotary_positions_grads(None, pts, freq, [5, 5, 5], g)
+    with pytest.raises(RuntimeError, match="in_grads"):
+        ops.rotary_positions_grads(x.detach(), pts, freq, [5, 5, 5], g[:, :2])
+    wide = draw((50, 3, 48), 5)[:, :, 8:40]  # a view as the gradient
+    assert torch.equal(ops.rotary_positions_grads(None, pts, freq, [5, 5, 5], wide, with_pts=False)[0],
+                       ops.rotary_positions_grads(x.detach(), pts, freq, [5, 5, 5], wide)[0])
