@@ -300,3 +300,22 @@ def test_rotary_positions_keep_their_features_only_for_the_points_gradient():
     wide = draw((50, 3, 48), 5)[:, :, 8:40]  # a view as the gradient
     assert torch.equal(ops.rotary_positions_grads(None, pts, freq, [5, 5, 5], wide, with_pts=False)[0],
                        ops.rotary_positions_grads(x.detach(), pts, freq, [5, 5, 5], wide)[0])
+
+
+# ---- 32-bit accuracy -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("heads,size", [((4, 2), 64), ((4, 4), 32), ((3, 3), 128), ((2, 1), 36), ((2, 2), 200)], ids=str)
+@pytest.mark.parametrize("lengths", [([700, 300], [900, 1400]), ([1, 1], [3000, 5000]), ([130, 9], [20000, 64])], ids=["tiles", "rows", "split"])
+def test_32_bit_results_are_right_to_22_bits_in_norm(lengths, heads, size):
+    """The worst-case bounds of the other tests are some 1e-4 wide for heads of 64; what the three planes of a 32-bit feature and the
+    emptied accumulators are for shows in the norm of the error.  Two planes would leave 2^-17 of every product (1e-5 in the gradients),
+    one accumulator for 1000 keys a bias of 64 truncations (4e-6).  Logits of spread 1.5 reach about 7 and are summed in 32 bits:
+    their rounding is 2^-24 * 7, which two of them bring into a probability; sums and the last rounding add a few 2^-24: 2^-19 in all."""
+    from pccnn_lib_b200 import ops
+    q, k, v, qe, ke, g = attention_case(lengths, heads, size, torch.float32, seed=30)
+    want = attention(q, k, v, *lengths, size ** -0.5, g)
+    out, lse = ops.cross_attention(q, k, v, qe, ke)
+    grads = ops.cross_attention_grads(q, k, v, qe, ke, out, lse, g)
+    ops.check_status()
+    for name, got in zip(("out", "dq", "dk", "dv"), [out] + grads):
+        error = float((got.double() - want[name]).norm() / want[name].norm())
+        assert error <= 2.0 ** -19, (name, error)
