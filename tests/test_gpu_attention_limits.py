@@ -319,3 +319,36 @@ def test_32_bit_results_are_right_to_22_bits_in_norm(lengths, heads, size):
     for name, got in zip(("out", "dq", "dk", "dv"), [out] + grads):
         error = float((got.double() - want[name]).norm() / want[name].norm())
         assert error <= 2.0 ** -19, (name, error)
+
+
+# ---- infinities ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("lengths,size", [(([300, 20], [500, 40]), 64), (([2, 1], [700, 90]), 64), (([300, 20], [500, 40]), 36)],
+                         ids=["tiles", "few", "rows"])
+def test_an_infinity_reaches_only_the_results_that_depend_on_it(lengths, size, dtype):
+    """A query's infinity stays in the row of its head, a value's in its feature of its cloud; what they reach is the formula's
+    infinity or NaN (the route decides), everything else is as right as ever."""
+    from pccnn_lib_b200 import ops
+    q, k, v, qe, ke, g = attention_case(lengths, (4, 2), size, dtype)
+    scale, (m, n) = size ** -0.5, (lengths[0][0], lengths[1][0])
+    clean = attention(q, k, v, *lengths, scale)
+
+    def check_rest(got, reached):
+        out, lse = got
+        hit = reached.to(out.device)
+        check(torch.where(hit, 0, out.double()), clean["out"].masked_fill(hit, 0), clean["out_bound"], "out")
+        assert not bool(torch.isfinite(out[hit]).any())
+    for bad in (float("inf"), -float("inf")):
+        spoiled = q.clone()
+        spoiled[1, 2, 5] = bad
+        got = ops.cross_attention(spoiled, k, v, qe, ke)
+        reached = torch.zeros(q.shape, dtype=torch.bool)
+        reached[1, 2] = True
+        check_rest(got, reached)  # among random keys some logit is +infinity, so the formula itself gives NaN
+        assert bool(torch.isnan(got[0][1, 2]).all())
+        spoiled = v.clone()
+        spoiled[7, 1, 9] = bad
+        reached = torch.zeros(q.shape, dtype=torch.bool)
+        reached[:m, 2:, 9] = True
+        check_rest(ops.cross_attention(q, k, spoiled, qe, ke), reached)
+    ops.check_status()
