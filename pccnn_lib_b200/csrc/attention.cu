@@ -934,7 +934,10 @@ static int launch_grad_rows(const AttentionCall& a, const HeadRows& grads, const
 template <class T, class F>
 static int dispatch_rows(const RowLayout& l, const F& f) {
     constexpr int kV = 16 / sizeof(T);
-    if (l.vectors) return l.chunks == 1 ? f.template run<T, kV, 1>() : f.template run<T, kV, 2>();
+    if (l.vectors) {
+        if constexpr (sizeof(T) == 2) return f.template run<T, kV, 1>();  // kMaxHeadSize is one vector of each lane
+        else return l.chunks == 1 ? f.template run<T, kV, 1>() : f.template run<T, kV, 2>();
+    }
     if (l.chunks == 1) return f.template run<T, 1, 1>();
     if (l.chunks == 2) return f.template run<T, 1, 2>();
     return l.chunks == 4 ? f.template run<T, 1, 4>() : f.template run<T, 1, 8>();

@@ -69,11 +69,6 @@ struct Pairs {
     }
 };
 __device__ __forceinline__ unsigned long long both(float x) { return pack_f32x2(x, x); }
-__device__ __forceinline__ unsigned long long add_f32x2(unsigned long long a, unsigned long long b) {
-    unsigned long long r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 __device__ __forceinline__ float sum_of(unsigned long long v) {
     float lo, hi;
     unpack_f32x2(v, lo, hi);
