@@ -494,8 +494,12 @@ int pccnn_point_conv_weight_var(int64_t num_pts, const float* basis, int hidden,
 /* Attention between packed clouds (no counterpart in the reference)          */
 /* ------------------------------------------------------------------------- */
 
-/* Features are float32, or bfloat16 where is_bf16 != 0; every sum, statistic and probability is float32 and a bf16
- * result is rounded once.  Features of heads are [rows, heads, size] with contiguous sizes and any row and head
+/* Features are float32, or bfloat16 where is_bf16 != 0; sums, statistics and probabilities are computed in float32 and a
+ * bf16 result is rounded at the end.  Attention in bf16 has further roundings: on the tensor cores the probabilities, and in the
+ * gradients p (dp - delta), become bf16 operands of the products that follow (errors of 2.3e-3 to 2.5e-3 in norm where the
+ * result's own rounding is 1.7e-3); and delta, the sum of out g over a row, is taken from the rounded output for clouds of more
+ * than 64 keys (queries' gradient on the tensor cores), of more keys than one block has (keys' gradient there) or of
+ * more than 256 keys (other shapes).  Features of heads are [rows, heads, size] with contiguous sizes and any row and head
  * stride in elements (int64 host arrays {row, head}); outputs are contiguous. */
 
 /* Layer norm over the channels: out = (feats - mean) * rstd * weights + bias with the biased variance,

@@ -223,7 +223,8 @@ int tc_forward(const AttentionCall& a, void* out, float* lse, char* ws, cudaStre
 // ---- backward -----------------------------------------------------------------------------------------------------
 // Backward: tiles, except for small 32-bit calls (150 queries, 301 keys, 2 clouds, 4 heads of 32: 24 us with rows, 40 us with
 // tiles; 300 queries, 600 keys, 4 heads of 64: 107 and 65 us; in bf16 tiles are faster from one query on: 20.4 and 19.1 us for
-// one query and 300 keys) and for 32-bit heads of more than 64 features, whose tiles that stay in shared memory take 192 KB.
+// one query and 300 keys) and for 32-bit heads of more than 64 features: the two tiles that stay would take 2 x 192 columns of tensor
+// memory, which leaves too few of the 512 for logits and accumulators.
 // The streamed tiles of all heads that share a key head are counted in 32 bits.
 bool tc_grads_shape(const AttentionCall& a) {
     return tc_any_shape(a) && (a.is_bf16 || (a.size <= 64 && tc_work(a) >= 6e6)) &&

@@ -416,8 +416,9 @@ __device__ __forceinline__ void tc_drain_loads(TcShared* sh, int issued, int sta
 // Measured: 40001 queries, 20003 keys, 16 clouds, 8 heads on 2 of 128, bf16: 371 us, 727 TFLOP/s (44% of a cuBLAS product), tensor
 // pipe 38% active: bound by the chain logits, probabilities, sums with two units in flight, and by products of 64 keys, which
 // read their 128 rows from shared memory longer (48 cycles) than they compute (32).  Heads of 64, 30011 queries and
-// keys, 8 clouds, 8 heads: 478 us, 635 TFLOP/s, the element-wise warps are busy 92% of the time, the exponential unit 66%.
-// 32-bit heads of 64, 16001 x 8003, 8 heads on 4: 322 us, the tensor pipe 42%.
+// keys, 8 clouds, 8 heads: 477 us, 637 TFLOP/s: the element-wise groups have a unit in hand 92% of the time, with the exponential unit
+// 65% and the issue slots 44% busy, so they wait on the latency of their own chain (two warps per scheduler).
+// 32-bit heads of 64, 16001 x 8003, 8 heads on 4: 319 us, the tensor pipe 41%.
 // The accumulator is scaled only when the maximum has grown by more than 2^8 since it was last scaled: the probabilities
 // stay below 2^8, and the final division is by a sum relative to the same reference.
 // The logits and the probabilities have columns of their own: once the rows have been read into registers the logits of the
@@ -765,10 +766,11 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 // KEYS = true: block = 128 keys of one cloud and key head; it keeps K and V and streams Q and dO of every head that shares them:
 //   s = K Q^T, t = V dO^T, p = exp(scale s - lse), e = p (t - delta),  dK += e Q,  dV += p dO.
 // The accumulators are emptied every kRound units, for 32-bit features into registers (see the forward kernel on truncation).
-// Measured on the calls of the forward kernel: bf16 618 us (queries) and 797 us (keys), tensor pipe 36% active; the queries'
+// Measured on the calls of the forward kernel: bf16 647 us (queries) and 798 us (keys), tensor pipe 34 and 36% active; the queries'
 // kernel waits for logits 40% of the time, the keys' is bound by its products, which take 82 cycles each where 32 to 48
 // would do (two warps issue them in turn; with one warp they take 45 to 58, but it waits as long in between).  32 bits:
-// 369 us and 548 us, tensor pipe 55%, products of 32 rows.
+// 369 us and 549 us, tensor pipe 55%, products of 32 rows.  (622 us for the queries' gradient in bf16 before the accumulators were
+// emptied and delta was decided cloud by cloud.)
 // Two kernels, each recomputing the logits, instead of one that adds dQ with atomics: every sum is taken in a fixed order.
 // 32-bit features: the two tiles that stay are kept as planes in tensor memory (kKeepInTmem), which leaves the keys' kernel no
 // columns of their own for the weights: there they take the place of the logits (kInPlace), and the logits of a group's

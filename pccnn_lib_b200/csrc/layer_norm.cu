@@ -162,7 +162,7 @@ layer_norm_kernel(int64_t rows, int channels, const T* __restrict__ feats, int64
         row_sums<TPR, R>(mean, &slots[0]);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            mean[i] /= (float)channels;  // a division: the mean of equal values is that value
+            mean[i] /= (float)channels;  // a division: the mean of equal values is that value wherever their sum is exact
             const unsigned long long m = both(mean[i]);
 #pragma unroll
             for (int e = 0; e < Row::kN; ++e) x[i].w[e] = sub_f32x2(x[i].w[e], m);
